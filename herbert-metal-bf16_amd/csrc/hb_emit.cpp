@@ -10,6 +10,8 @@
 #include <cstdlib>
 #include <cstdio>
 #include <cstring>
+#include <utility>
+#include <vector>
 
 #include "hb_internal.h"
 
@@ -34,6 +36,21 @@ static std::string D(const char* k, uint64_t v) {
 static bool is_gemm(uint32_t kind) {
     return kind == HB_KIND_GEMM || kind == HB_KIND_GEMM_DIRECT || kind == HB_KIND_GEMM_SIMT ||
            kind == HB_KIND_GEMM_SWIGLU;
+}
+
+// The tiles of a packed 4-bit matrix (16 rows x 128 K) and its bytes.
+static uint64_t q4_tiles(uint32_t k, uint32_t n) { return ((uint64_t)k + 127) / 128 * (((uint64_t)n + 15) / 16); }
+static uint64_t q4_bytes(uint32_t k, uint32_t n, uint32_t group) { return q4_tiles(k, n) * (1024 + 4096 / group); }
+static bool q4_shape(uint32_t k, uint32_t n, uint32_t group) {
+    return k && n && k % 8 == 0 && (group == 32 || group == 64 || group == 128) && q4_tiles(k, n) < (1u << 30);
+}
+
+static void q4_defaults(hb_desc* d) {
+    if (!d->mv_m) d->mv_m = d->rows_of == HB_ROWS_DENSE ? 1 : 16;
+    if (!d->rows) d->rows = d->out == HB_OUT_SWIGLU ? 32 : 16;
+    if (!d->mv_waves) d->mv_waves = 4;
+    if (!d->split) d->split = 4;
+    if (!d->unroll) d->unroll = 2;
 }
 
 hb_desc with_defaults(const hb_desc& in) {
@@ -62,6 +79,9 @@ hb_desc with_defaults(const hb_desc& in) {
         if (d.form == 1 || (d.form == 3 && d.rows != 32)) d.rows = 16;
         if (d.form == 4 && d.rows != 8 && d.rows != 16) d.rows = 4;
         if (!d.mv_waves) d.mv_waves = 4;
+    } else if (d.kind >= HB_KIND_Q4_QUANTIZE && d.kind <= HB_KIND_MATVEC_Q4) {
+        if (!d.bk) d.bk = 32;
+        if (d.kind == HB_KIND_MATVEC_Q4) q4_defaults(&d);
     }
     return d;
 }
@@ -351,6 +371,75 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             e->defines = {D("HB_OP", 8), D("HB_E", 64), D("HB_TOPK", 1), D("HB_D", d.n),
                           D("HB_EPS", d.eps_bits), D("HB_PLUS1", d.plus_one)};
             return HB_OK;
+        case HB_KIND_Q4_QUANTIZE:
+        case HB_KIND_Q4_PACK:
+        case HB_KIND_Q4_DEQUANTIZE: {
+            if (!q4_shape(d.k, d.n, d.bk))
+                return fail(HB_ERR_UNSUPPORTED, "q4: K a multiple of 8, groups of 32, 64 or 128");
+            const uint32_t op = d.kind - HB_KIND_Q4_QUANTIZE + 1;
+            snprintf(name, sizeof name, "q4_%s_%ux%u_g%u", op == 1 ? "quantize" : op == 2 ? "pack" : "dequantize",
+                     d.k, d.n, d.bk);
+            e->name = name;
+            e->source = "q4.hip";
+            e->threads = 256;
+            e->nbind = op == 2 ? 3 : 2;
+            e->defines = {D("HB_OP", op), D("HB_K", d.k), D("HB_N", d.n), D("HB_GROUP", d.bk)};
+            return HB_OK;
+        }
+        case HB_KIND_MATVEC_Q4: {
+            const bool experts = d.rows_of != HB_ROWS_DENSE, swi = d.out == HB_OUT_SWIGLU;
+            if (d.out > HB_OUT_SWIGLU || d.rows_of > HB_ROWS_SCATTER)
+                return fail(HB_ERR_INVALID, "matvec_q4: out / rows_of out of range");
+            if (!q4_shape(d.k, d.n, d.bk))
+                return fail(HB_ERR_UNSUPPORTED, "matvec_q4: K a multiple of 8, groups of 32, 64 or 128");
+            if (swi && d.n % 32)
+                return fail(HB_ERR_UNSUPPORTED, "matvec_q4 Out::Swiglu: gate and up rows each a multiple of 16");
+            if (d.mv_m > 16) return fail(HB_ERR_UNSUPPORTED, "matvec_q4: m <= 16");
+            if ((d.rows != 16 && d.rows != 32 && d.rows != 64) || (swi && d.rows == 16))
+                return fail(HB_ERR_UNSUPPORTED, "matvec_q4: 16, 32 or 64 rows a wave (Out::Swiglu 32 or 64)");
+            if (d.mv_waves > 16 || !pow2(d.mv_waves) || !pow2(d.split) || d.split > d.mv_waves || d.unroll > 4)
+                return fail(HB_ERR_UNSUPPORTED, "matvec_q4: 1, 2, 4, 8 or 16 waves, split no more, unroll 1..4");
+            if (experts && (!d.top_k || !d.experts || !d.tiles || !d.rows_max || d.mv_m != 16 ||
+                            (d.out != HB_OUT_BF16 && !swi)))
+                return fail(HB_ERR_INVALID,
+                            "matvec_q4 over experts: top_k, experts, tiles and rows_max, tiles of 16 rows, bf16 out");
+            std::string rows;
+            if (experts) {
+                snprintf(name, sizeof name, "_%s_k%u_e%u_t%u_r%u", d.rows_of == HB_ROWS_GATHER ? "gather" : "scatter",
+                         d.top_k, d.experts, d.tiles, d.rows_max);
+                rows = name;
+            }
+            snprintf(name, sizeof name, "matvec_q4_%ux%u_g%u%s_r%u_k%u_w%u_u%u_m%u%s", d.k, d.n, d.bk,
+                     d.out == HB_OUT_F32 ? "_f32" : d.out == HB_OUT_RESIDUAL ? "_res" : swi ? "_sw" : "", d.rows,
+                     d.split, d.mv_waves, d.unroll, d.mv_m, rows.c_str());
+            e->name = name;
+            e->source = "matvec_q4.hip";
+            e->threads = 64 * d.mv_waves;
+            e->nbind = experts ? 6 : 3;
+            e->defines = {D("HB_K", d.k),          D("HB_N", d.n),         D("HB_GROUP", d.bk),
+                          D("HB_OUT", d.out),      D("HB_MV_M", d.mv_m),   D("HB_RT", d.rows / 16),
+                          D("HB_SPLIT", d.split),  D("HB_WAVES", d.mv_waves), D("HB_UNROLL", d.unroll),
+                          D("HB_ROWS", d.rows_of), D("HB_TOPK", experts ? d.top_k : 1),
+                          D("HB_E", experts ? d.experts : 1)};
+            return HB_OK;
+        }
+        case HB_KIND_BLOCK_NORM: {
+            const uint32_t gate = d.form >> 4, cells = cdiv(d.n, 8);
+            if (!d.n || d.n > 32768) return fail(HB_ERR_UNSUPPORTED, "block_norm: rows of 1 to 32768");
+            if (d.form & ~0x37u) return fail(HB_ERR_INVALID, "block_norm: parts out of range");
+            const bool post = d.form & HB_NORM_POST, pre = d.form & HB_NORM_PRE, scales = d.form & HB_NORM_SCALES;
+            snprintf(name, sizeof name, "block_norm_%u_e%08x%s%s%s%s_g%u", d.n, d.eps_bits, d.plus_one ? "_p1" : "",
+                     post ? "_post" : "", pre ? "_pre" : "", scales ? "_sc" : "", gate);
+            e->name = name;
+            e->source = "block_norm.hip";
+            // A 16-byte chunk of the row a thread, up to 1024 threads.
+            e->threads = cells < 1024 ? cdiv(cells, 64) * 64 : 1024;
+            e->nbind = 3 + (post ? 1 : 0) + (pre ? 2 : 0) + (scales ? 1 : 0) + (gate ? 1 : 0);
+            e->defines = {D("HB_D", d.n),       D("HB_THREADS", e->threads), D("HB_EPS", d.eps_bits),
+                          D("HB_PLUS1", d.plus_one ? 1 : 0), D("HB_POST", post), D("HB_PRE", pre),
+                          D("HB_SCALES", scales), D("HB_GATE", gate)};
+            return HB_OK;
+        }
         case HB_KIND_ROUND_PROBE:
             e->name = "round_probe_bf16";
             e->source = "probe.hip";
@@ -422,8 +511,22 @@ uint32_t groups_of(const hb_desc& d, uint32_t m) {
         case HB_KIND_SWIGLU:
         case HB_KIND_COMBINE:
             return (uint32_t)(((uint64_t)m * (d.n / 8) + 255) / 256);
+        case HB_KIND_Q4_QUANTIZE:
+        case HB_KIND_Q4_PACK:
+        case HB_KIND_Q4_DEQUANTIZE:  // a wave a tile
+            return (uint32_t)((m * q4_tiles(d.k, d.n) + 3) / 4);
+        case HB_KIND_MATVEC_Q4: {
+            const uint32_t per = d.out == HB_OUT_SWIGLU ? d.rows / 32 : d.rows / 16;
+            const uint32_t nt = d.out == HB_OUT_SWIGLU ? d.n / 32 : cdiv(d.n, 16);
+            const uint32_t wgs = cdiv(cdiv(nt, per), d.mv_waves / d.split);
+            if (d.rows_of == HB_ROWS_DENSE) return wgs;
+            // Tiles with rows: no more than pairs, nor than the table holds.
+            const uint64_t pairs = (uint64_t)m * d.top_k;
+            return (uint32_t)((pairs < d.tiles ? pairs : d.tiles) * wgs);
+        }
         case HB_KIND_MOE_OUT:
         case HB_KIND_RMSNORM:
+        case HB_KIND_BLOCK_NORM:
             return m;  // a workgroup per row
         case HB_KIND_ROUND_PROBE:
             return (1u << 24) / 256;  // one pattern per thread
@@ -435,6 +538,74 @@ uint32_t groups_of(const hb_desc& d, uint32_t m) {
 uint64_t workspace_of(const hb_desc& d, uint32_t m) {
     if (d.kind != HB_KIND_GEMM || d.ksplit < 2) return 0;
     return (uint64_t)d.ksplit * m * d.n * 4;
+}
+
+// What a launch of the newer kinds reads or writes at each binding: bytes, the
+// element's size, whether written, and whether it is a row array that an
+// output may be written over (by the thread that has read that element).
+struct Access {
+    const char* what;
+    uint64_t bytes;
+    uint32_t align;
+    bool write, rows;
+};
+
+static std::vector<Access> accesses(const hb_desc& d, uint32_t m) {
+    const uint64_t mm = m, k = d.k, n = d.n;
+    std::vector<Access> a;
+    if (d.kind == HB_KIND_Q4_QUANTIZE || d.kind == HB_KIND_Q4_DEQUANTIZE) {
+        const bool to = d.kind == HB_KIND_Q4_QUANTIZE;
+        a = {{"W", mm * n * k * 2, 2, !to, false}, {"q4", mm * q4_bytes(d.k, d.n, d.bk), 16, to, false}};
+        if (!to) std::swap(a[0], a[1]);
+    } else if (d.kind == HB_KIND_Q4_PACK) {
+        a = {{"codes", mm * n * k / 2, 2, false, false},
+             {"scales", mm * n * cdiv(d.k, d.bk) * 2, 2, false, false},
+             {"q4", mm * q4_bytes(d.k, d.n, d.bk), 16, true, false}};
+    } else if (d.kind == HB_KIND_MATVEC_Q4) {
+        const uint64_t nout = d.out == HB_OUT_SWIGLU ? n / 2 : n;
+        const uint32_t size = out_bytes(d.out);
+        if (d.rows_of == HB_ROWS_DENSE)
+            return {{"q4", q4_bytes(d.k, d.n, d.bk), 16, false, false},
+                    {"x", mm * k * 2, 2, false, false},
+                    {"y", mm * nout * size, size, true, false}};
+        const uint64_t pairs = mm * d.top_k;
+        a = {{"state", 16, 4, false, false},
+             {"q4", d.experts * q4_bytes(d.k, d.n, d.bk), 16, false, false},
+             {"X", (d.rows_of == HB_ROWS_GATHER ? mm : pairs) * k * 2, 2, false, false},
+             {"Y", pairs * nout * size, size, true, false},
+             {"list", pairs * 4, 4, false, false},
+             {"tiles", (1 + 3ull * d.tiles) * 4, 4, false, false}};
+    } else if (d.kind == HB_KIND_BLOCK_NORM) {
+        const uint64_t all = mm * n * 2;
+        a = {{"x", all, 2, false, true}, {"y", all, 2, false, true}, {"xo", all, 2, true, true}};
+        if (d.form & HB_NORM_PRE) a.push_back({"h", all, 2, true, true});
+        if (d.form & HB_NORM_POST) a.push_back({"w_post", n * 2, 2, false, false});
+        const uint32_t gate = d.form & HB_NORM_GATE_CHANNELS;
+        if (gate == HB_NORM_GATE_ROWS) a.push_back({"gate", mm * 2, 2, false, false});
+        if (gate == HB_NORM_GATE_ELEMENTS) a.push_back({"gate", all, 2, false, true});
+        if (gate == HB_NORM_GATE_CHANNELS) a.push_back({"gate", n * 2, 2, false, false});
+        if (d.form & HB_NORM_SCALES) a.push_back({"scales", 8, 4, false, false});
+        if (d.form & HB_NORM_PRE) a.push_back({"w_pre", n * 2, 2, false, false});
+    }
+    return a;
+}
+
+int check_addresses(const hb_desc& d, void* const* ptrs, uint32_t nbind, uint32_t m) {
+    const std::vector<Access> a = accesses(d, m);
+    for (uint32_t i = 0; i < a.size() && i < nbind; i++) {
+        const uintptr_t pi = (uintptr_t)ptrs[i];
+        if (pi % a[i].align)
+            return fail(HB_ERR_INVALID, std::string("binding ") + std::to_string(i) + " (" + a[i].what +
+                                            ") starts at no multiple of " + std::to_string(a[i].align) + " bytes");
+        for (uint32_t j = 0; j < i; j++) {
+            const uintptr_t pj = (uintptr_t)ptrs[j];
+            if ((!a[i].write && !a[j].write) || pi >= pj + a[j].bytes || pj >= pi + a[i].bytes) continue;
+            if (a[i].rows && a[j].rows && pi == pj && !(a[i].write && a[j].write)) continue;
+            return fail(HB_ERR_INVALID, std::string("bindings ") + std::to_string(j) + " (" + a[j].what + ") and " +
+                                            std::to_string(i) + " (" + a[i].what + ") overlap");
+        }
+    }
+    return HB_OK;
 }
 
 static int need(const uint64_t* sizes, uint32_t i, uint64_t bytes, const char* what) {
@@ -480,6 +651,18 @@ int check_bindings(const hb_desc& d, const uint64_t* s, uint32_t nbind, uint32_t
         return HB_OK;
     }
     if (m == 0) return fail(HB_ERR_INVALID, "0 rows");
+    const std::vector<Access> acc = accesses(d, m);
+    if (!acc.empty()) {
+        if (d.kind == HB_KIND_MATVEC_Q4 && d.rows_of == HB_ROWS_DENSE && m > d.mv_m)
+            return fail(HB_ERR_INVALID, "matvec_q4 of " + std::to_string(m) + " rows: 1.." + std::to_string(d.mv_m));
+        if (d.kind == HB_KIND_MATVEC_Q4 && d.rows_of != HB_ROWS_DENSE && m > d.rows_max)
+            return fail(HB_ERR_INVALID, "m beyond the kernel's rows_max");
+        if (d.kind < HB_KIND_MATVEC_Q4 && m * q4_tiles(d.k, d.n) >= (1ull << 32))
+            return fail(HB_ERR_UNSUPPORTED, "q4: too many matrices in one launch");
+        for (uint32_t i = 0; i < acc.size(); i++)
+            if ((rc = need(s, i, acc[i].bytes, acc[i].what))) return rc;
+        return HB_OK;
+    }
     uint64_t mm = m, k2 = 2ull * d.top_k;
     switch (d.kind) {
         case HB_KIND_ROUTE:
@@ -543,3 +726,7 @@ int check_bindings(const hb_desc& d, const uint64_t* s, uint32_t nbind, uint32_t
 }
 
 }  // namespace hb
+
+extern "C" uint64_t hb_q4_bytes(uint32_t k, uint32_t n, uint32_t group) {
+    return hb::q4_shape(k, n, group) ? hb::q4_bytes(k, n, group) : 0;
+}

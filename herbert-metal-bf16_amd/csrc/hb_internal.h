@@ -42,6 +42,14 @@ uint32_t groups_of(const hb_desc& d, uint32_t m);
 // Checks the bindings' byte sizes against what `d` reads and writes over m
 // rows; returns HB_OK or an error naming the binding.
 int check_bindings(const hb_desc& d, const uint64_t* sizes, uint32_t nbind, uint32_t m);
+// Checks what only the addresses tell, for the kinds that define it: each
+// binding at a multiple of its element, nothing written overlapping another
+// binding (sizes as check_bindings found them enough).
+int check_addresses(const hb_desc& d, void* const* ptrs, uint32_t nbind, uint32_t m);
+// A gate|up kernel that writes the SwiGLU of its sums itself.
+inline bool writes_swiglu(const hb_desc& d) {
+    return d.kind == HB_KIND_GEMM_SWIGLU || (d.kind == HB_KIND_MATVEC_Q4 && d.out == HB_OUT_SWIGLU);
+}
 // Fills defaults of the descriptor's zero fields (tile sizes, ...).
 hb_desc with_defaults(const hb_desc& d);
 

@@ -20,10 +20,15 @@ int moe_experts_run(hb_gpu* g, const int32_t kernels[4], int32_t swiglu, int32_t
         return fail(HB_ERR_INVALID, "moe experts: kernels[0] is not a moe_sort");
     // Grouped expert GEMMs only (never a dense split-K pair, whose
     // workspace the static entry point could not allocate).
-    if (gd->rows_of == HB_ROWS_DENSE || kernel_desc(g, dn)->rows_of == HB_ROWS_DENSE ||
-        kernel_desc(g, dn)->kind != HB_KIND_GEMM)
+    const hb_desc* dd = kernel_desc(g, dn);
+    const bool q4 = gd->kind == HB_KIND_MATVEC_Q4;
+    if (gd->rows_of == HB_ROWS_DENSE || dd->rows_of == HB_ROWS_DENSE ||
+        dd->kind != (q4 ? HB_KIND_MATVEC_Q4 : HB_KIND_GEMM))
         return fail(HB_ERR_INVALID, "moe experts: kernels[1] and kernels[2] are grouped expert GEMMs");
-    const bool fused = gd->kind == HB_KIND_GEMM_SWIGLU;
+    if (q4 && (sd->bm != 16 || gd->rows_of != HB_ROWS_GATHER || dd->rows_of != HB_ROWS_SCATTER || gather >= 0))
+        return fail(HB_ERR_INVALID, "moe experts in 4 bits: a sort of 16-row tiles, gathered gate|up rows, "
+                                    "scattered down rows, no gather kernel");
+    const bool fused = writes_swiglu(*gd);
     if (!fused && !kernel_desc(g, swiglu))
         return fail(HB_ERR_INVALID, "moe experts: the gate|up GEMM needs the swiglu_slots kernel");
     const uint32_t top_k = sd->top_k;
@@ -67,7 +72,7 @@ extern "C" int hb_moe_experts_run(hb_gpu* g, const int32_t kernels[4], int32_t s
     // xs is bound only with a gather, egu only when the SwiGLU is not fused
     // into the gate|up GEMM: otherwise those ranges are not looked at.
     const hb_desc* gd = kernel_desc(g, kernels[1]);
-    const bool need_xs = kernels[3] >= 0, need_egu = !gd || gd->kind != HB_KIND_GEMM_SWIGLU;
+    const bool need_xs = kernels[3] >= 0, need_egu = !gd || !writes_swiglu(*gd);
     void* ptr[12];
     uint64_t size[12];
     for (int i = 0; i < 12; i++) {

@@ -343,6 +343,7 @@ int launch_ptrs(hb_gpu* g, int32_t kernel, void* const* ptrs, const uint64_t* si
         return fail(HB_ERR_INVALID, k.em.name + ": " + std::to_string(nbind) +
                                         " bindings given, it takes " + std::to_string(k.em.nbind));
     int rc = check_bindings(k.desc, sizes, nbind, m);
+    if (!rc) rc = check_addresses(k.desc, ptrs, nbind, m);
     if (rc) return fail(rc, k.em.name + ": " + hb_last_error());
     if ((rc = ensure_ws(g, workspace_of(k.desc, m)))) return rc;
     void* p[10];
@@ -636,6 +637,7 @@ static int prepare(hb_gpu* g, const hb_op* ops, uint32_t nops, std::vector<Ready
             ready[i].ptrs[j] = p;
         }
         int rc = check_bindings(k.desc, sizes, op.nbind, op.m);
+        if (!rc) rc = check_addresses(k.desc, ready[i].ptrs, op.nbind, op.m);
         if (rc) return fail(rc, k.em.name + ": " + hb_last_error());
         if ((rc = ensure_ws(g, workspace_of(k.desc, op.m)))) return rc;
         ready[i].k = &k;

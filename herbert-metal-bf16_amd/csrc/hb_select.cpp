@@ -442,7 +442,7 @@ struct hb_engine {
     std::string tune_summary, log;
     std::map<std::string, int32_t> gemm_pick;
     std::map<std::string, std::pair<int32_t, int32_t>> gate_up_pick;
-    std::map<std::string, hb_desc> mv_pick;
+    std::map<std::string, hb_desc> mv_pick, mv_q4_pick;
     struct ExpertsPick {
         int32_t kernels[4];
         uint32_t bm;
@@ -1226,6 +1226,74 @@ int hb_engine_matvec_fused(hb_engine* e, uint32_t k, uint32_t n, uint32_t out, u
     return HB_OK;
 }
 
+// The key a 4-bit matvec's choice is kept under.
+static std::string q4_key(const hb_desc& d) {
+    return std::to_string(d.k) + "x" + std::to_string(d.n) + " q4/" + std::to_string(d.bk) + " " + out_name(d.out) + " m" +
+           std::to_string(d.mv_m);
+}
+
+// The MATVEC_Q4 forms of a shape's timed choice, the defaults first.
+static std::vector<hb_desc> mv_q4_candidates(uint32_t k, uint32_t n, uint32_t out, uint32_t group, uint32_t mv_m) {
+    hb_desc d{};
+    d.kind = HB_KIND_MATVEC_Q4;
+    d.k = k;
+    d.n = n;
+    d.out = out;
+    d.bk = group;
+    d.mv_m = mv_m;
+    std::vector<hb_desc> v = {with_defaults(d)};
+    return v;
+}
+
+int hb_engine_matvec_q4_candidates(hb_engine*, uint32_t k, uint32_t n, uint32_t out, uint32_t group, uint32_t mv_m,
+                                   hb_desc* descs, uint32_t cap, uint32_t* count) {
+    const auto v = mv_q4_candidates(k, n, out, group, mv_m);
+    *count = (uint32_t)v.size();
+    for (uint32_t i = 0; i < v.size() && i < cap; i++) descs[i] = v[i];
+    return HB_OK;
+}
+
+int hb_engine_matvec_q4(hb_engine* e, uint32_t k, uint32_t n, uint32_t out, uint32_t group, uint32_t mv_m,
+                        const hb_range* ws, uint32_t nws, hb_range x, hb_range y, int32_t* kernel) {
+    if (!e->g) return fail(HB_ERR_INVALID, "matvec_q4: an engine without a context");
+    if (!nws) return fail(HB_ERR_INVALID, "matvec_q4: no weights");
+    const auto list = mv_q4_candidates(k, n, out, group, mv_m);
+    if (!e->t["mv.auto"]) return e->build(list[0], kernel);
+    const std::string key = q4_key(list[0]);
+    auto it = e->mv_q4_pick.find(key);
+    if (it != e->mv_q4_pick.end()) return e->build(it->second, kernel);
+    const uint32_t nw = e->t["mv.cold"] ? nws : 1;
+    std::vector<Cand> c;
+    std::vector<hb_desc> descs;
+    int rc;
+    for (const hb_desc& d : list) {
+        int32_t kk;
+        if ((rc = e->build(d, &kk))) {
+            if (c.empty()) return rc;  // the shape's defaults: what refuses them refuses the call
+            e->logf("[autotune] matvec %s: a form not built (%s)", key.c_str(), hb_last_error());
+            continue;
+        }
+        std::vector<hb_op> ops;
+        for (uint32_t i = 0; i < nw; i++) ops.push_back(make_op(kk, mv_m, {ws[i], x, y}));
+        c.push_back({"r" + std::to_string(d.rows) + "k" + std::to_string(d.split) + "w" + std::to_string(d.mv_waves) +
+                         "u" + std::to_string(d.unroll),
+                     kk, ops});
+        descs.push_back(d);
+    }
+    size_t best = 0;
+    if (c.size() > 1) {
+        // Cold as mv_full's, and y as it was (Out::Residual adds into it).
+        std::vector<char> before((uint64_t)mv_m * (out == HB_OUT_SWIGLU ? n / 2 : n) * (out == HB_OUT_F32 ? 4 : 2));
+        if ((rc = hb_download(e->g, y.buf, y.offset, before.data(), before.size()))) return rc;
+        rc = e->pick_flagged("matvec " + key, c, std::vector<bool>(c.size(), true), &best, nullptr, true);
+        const int rc2 = hb_upload(e->g, y.buf, y.offset, before.data(), before.size());
+        if (rc || rc2) return rc ? rc : rc2;
+    }
+    e->mv_q4_pick[key] = descs[best];
+    *kernel = c[best].kernel;
+    return HB_OK;
+}
+
 int hb_engine_experts(hb_engine* e, uint32_t experts, uint32_t top_k, uint32_t hidden,
                       uint32_t inter, uint32_t m, const hb_moe_io* io, int32_t kernels[4],
                       uint32_t* bm_out) {
@@ -1489,6 +1557,12 @@ int hb_engine_picks(hb_engine* e, char* buf, uint64_t cap, uint64_t* len) {
         if (rc) return rc;
         s += "mv\t" + kv.first + "\t" + desc_text(e->g, k) + "\n";
     }
+    for (const auto& kv : e->mv_q4_pick) {
+        int32_t k;
+        int rc = e->build(kv.second, &k);
+        if (rc) return rc;
+        s += "mv_q4\t" + kv.first + "\t" + desc_text(e->g, k) + "\n";
+    }
     for (const auto& kv : e->experts_pick) {
         s += "experts\t" + kv.first + "\t" + std::to_string(kv.second.bm);
         for (int i = 0; i < 4; i++) s += "\t" + desc_text(e->g, kv.second.kernels[i]);
@@ -1592,6 +1666,13 @@ int hb_engine_pin(hb_engine* e, const char* text) {
             if ((rc = kernel_at(2, &k))) return rc;
             if (k < 0) return bad("no matvec kernel");
             e->mv_pick[f[1]] = *kernel_desc(e->g, k);
+        } else if (f[0] == "mv_q4") {
+            int32_t k;
+            if ((rc = kernel_at(2, &k))) return rc;
+            const hb_desc* d = kernel_desc(e->g, k);
+            if (!d || d->kind != HB_KIND_MATVEC_Q4 || d->rows_of != HB_ROWS_DENSE || f[1] != q4_key(*d))
+                return bad("no 4-bit matvec kernel of this key");
+            e->mv_q4_pick[f[1]] = *d;
         } else if (f[0] == "experts") {
             if (f.size() < 11) return bad("too few fields");
             hb_engine::ExpertsPick ep;

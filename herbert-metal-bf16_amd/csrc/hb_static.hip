@@ -62,7 +62,7 @@ extern "C" int hb_moe_experts_run_static(hb_gpu* g, const int32_t kernels[4], in
         gd->rows_of == HB_ROWS_DENSE || dd->rows_of == HB_ROWS_DENSE)
         return fail(HB_ERR_INVALID, "moe experts (static): kernels[0..2] must be a built sort and grouped GEMMs");
     if (m == 0) return fail(HB_ERR_INVALID, "moe experts (static): 0 rows");
-    const bool fused = gd->kind == HB_KIND_GEMM_SWIGLU, gather = kernels[3] >= 0;
+    const bool fused = writes_swiglu(*gd), gather = kernels[3] >= 0;
     const uint64_t pairs = (uint64_t)m * sd->top_k, hidden = dd->n, inter = dd->k;
     // The table's capacity: what the sort and the GEMMs were built for.
     const uint64_t cap_sort = (sd->rows_max * (uint64_t)sd->top_k + sd->bm - 1) / sd->bm + sd->experts;

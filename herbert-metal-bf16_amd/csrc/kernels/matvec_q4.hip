@@ -1,0 +1,204 @@
+// matvec_q4.hip -- y[m][n] = x[m][k] . W^T over weights of 4 bits in the
+// layout of q4.hip, for up to 16 rows of x: a decode step's projections
+// (ROWS 0), and the routed experts of a decode batch over moe_sort's tiles of
+// up to 16 rows (ROWS 1: x rows gathered through the list, y in sorted order;
+// 2: x in sorted order, y rows scattered through the list).
+//
+//   y[m][n] = sum over groups g of s[n][g] * (sum over k in g of (q - 8) x)
+//
+// The codes never become scaled weights: a bf16 of 16 + q is one and-or of a
+// rotated word (two codes each), the MFMA sums (16 + q) x exactly in its
+// products, and starts from the sum of -24 x, an MFMA with a constant operand
+// that the row tiles of a wave share.  The group's scale then multiplies the
+// f32 sum of 16 rows x 16 columns.  Sums are f32 throughout; Out rounds once.
+// (24 x has to be finite: an x beyond 2^123 or an infinity gives NaN.)
+//
+// Bound by the codes' bytes: K N / 2 and 2 K N / GROUP for the scales.
+#include "hb_common.h"
+
+constexpr u32 K = HB_K, N = HB_N, GROUP = HB_GROUP, OUT = HB_OUT, MV = HB_MV_M;
+constexpr u32 KT = (K + 127) / 128, NT = (N + 15) / 16, TILES = KT * NT, GPT = 128 / GROUP, SPG = GROUP / 32;
+constexpr u64 BLOB = (u64)TILES * (1024 + 32 * GPT);
+constexpr u32 RT = HB_RT, SPLIT = HB_SPLIT, WAVES = HB_WAVES, U = HB_UNROLL, ROWS = HB_ROWS, TOPK = HB_TOPK;
+constexpr bool SWI = OUT == 3;
+constexpr u32 NOUT = SWI ? N / 2 : N;
+constexpr u32 OT = SWI ? RT / 2 : RT;                    // output tiles of a wave
+constexpr u32 ONT = SWI ? NT / 2 : NT;                   // output tiles
+constexpr u32 NBLK = (ONT + OT - 1) / OT, GPW = WAVES / SPLIT;
+constexpr u32 NWG = (NBLK + GPW - 1) / GPW;
+static_assert(K % 8 == 0 && (!SWI || (RT % 2 == 0 && N % 32 == 0)), "shape");
+static_assert(WAVES % SPLIT == 0 && MV >= 1 && MV <= 16, "waves");
+
+typedef u32x4 chunk_t __attribute__((aligned(2)));
+typedef u32x2 half_t __attribute__((aligned(2)));
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+
+// Codes 8 i + 0..7 of a word as bf16 16 + q, the MFMA's A operand.
+HB_DEV bf16x8 codes(u32 w) {
+    u32x4 a;
+#pragma unroll
+    for (u32 i = 0; i < 4; i++) a[i] = (__builtin_amdgcn_alignbit(w, w, 4 * i) & 0x00780078u) | 0x41804180u;
+    return __builtin_bit_cast(bf16x8, a);
+}
+
+HB_DEV void store_row(void* yv, u64 row, u32 n, f32x4 v) {
+    if (OUT == 1) {
+        float* y = (float*)yv + row * NOUT + n;
+        if (NOUT % 4 == 0) {
+            *(f32x4_u*)y = v;
+        } else {
+#pragma unroll
+            for (u32 i = 0; i < 4; i++)
+                if (n + i < NOUT) y[i] = v[i];
+        }
+        return;
+    }
+    u16* y = (u16*)yv + row * NOUT + n;
+    if (NOUT % 4 == 0) {
+        if (OUT == 2) {
+            const half_t o = *(half_t*)y;
+            v += f32x4{bf16_lo(o.x), bf16_hi(o.x), bf16_lo(o.y), bf16_hi(o.y)};
+        }
+        *(half_t*)y = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    } else {
+#pragma unroll
+        for (u32 i = 0; i < 4; i++)
+            if (n + i < NOUT) y[i] = (u16)pack_bf16x2(OUT == 2 ? bf16_to_f32(y[i]) + v[i] : v[i], 0.0f);
+    }
+}
+
+#if HB_ROWS == 0
+extern "C" __global__ __launch_bounds__(64 * WAVES) void HB_NAME(const unsigned char* __restrict__ W,
+                                                                   const u16* __restrict__ x, void* yv, u32 rows) {
+#else
+extern "C" __global__ __launch_bounds__(64 * WAVES) void HB_NAME(
+    const u32* __restrict__ state, const unsigned char* __restrict__ W, const u16* __restrict__ x, void* yv,
+    const u32* __restrict__ list, const u32* __restrict__ tiles, u32 m_launch) {
+#endif
+    const u32 tid = threadIdx.x, lane = tid & 63u, col = lane & 15u, quad = lane >> 4;
+    const u32 wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const u32 sp = wave % SPLIT, gi = wave / SPLIT;
+    u32 wg = blockIdx.x;
+#if HB_ROWS == 0
+    // Columns past the rows repeat the last one and are never stored.
+    const u32 cols = rows < MV ? rows : MV;
+    const u64 xrow = col < cols ? col : cols - 1;
+    auto yrow = [&](u32 c) -> u64 { return c; };
+#else
+    const u32 m = rows_of_state(state, m_launch), pairs = m * TOPK;
+    const u32 t = wg / NWG;
+    wg %= NWG;
+    if (t >= tiles[0]) return;
+    const u32 expert = tiles[1 + 3 * t], first = tiles[2 + 3 * t];
+    u32 cols = tiles[3 + 3 * t];
+    if (expert >= HB_E || first >= pairs) return;
+    cols = cols < MV ? cols : MV;
+    cols = cols < pairs - first ? cols : pairs - first;
+    if (cols == 0) return;
+    W += expert * BLOB;
+    const u32 p = first + (col < cols ? col : cols - 1);
+    u64 xrow = p;
+    if (ROWS == 1) {
+        xrow = list[p] / TOPK;
+        xrow = xrow < m ? xrow : m - 1;
+    }
+    auto yrow = [&](u32 c) -> u64 {
+        if (ROWS == 1) return first + c;
+        const u32 r = list[first + c];
+        return r < pairs ? r : pairs - 1;
+    };
+#endif
+    const u16* xp = x + xrow * K;
+    const u16* scales = (const u16*)(W + (u64)TILES * 1024);
+    const u32 blk = wg * GPW + gi;
+    // The wave's W tiles; past the last they repeat it and are never stored.
+    u32 tn[RT];
+#pragma unroll
+    for (u32 r = 0; r < RT; r++) {
+        const u32 o = blk * OT + r % OT;
+        tn[r] = ((o < ONT ? o : ONT - 1) + (r / OT) * ONT) * KT;
+    }
+    const u32 kt0 = sp * KT / SPLIT, kt1 = (sp + 1) * KT / SPLIT;
+    const bf16x8 a24 = __builtin_bit_cast(bf16x8, u32x4{0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u});
+    f32x4 acc[RT];
+#pragma unroll
+    for (u32 r = 0; r < RT; r++) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    for (u32 kt = kt0; kt < kt1; kt += U) {
+        u32x4 w[U][RT], xf[U][4];
+        u32x2 s[U][RT][GPT];
+#pragma unroll
+        for (u32 u = 0; u < U; u++) {
+            const u32 q = kt + u < kt1 ? kt + u : kt1 - 1;
+#pragma unroll
+            for (u32 r = 0; r < RT; r++) {
+                w[u][r] = __builtin_nontemporal_load((const u32x4*)(W + (u64)(tn[r] + q) * 1024) + lane);
+                const u32x2* sp2 = (const u32x2*)(scales + (u64)(tn[r] + q) * 16 * GPT) + quad * GPT;
+#pragma unroll
+                for (u32 g = 0; g < GPT; g++) s[u][r][g] = sp2[g];
+            }
+#pragma unroll
+            for (u32 j = 0; j < 4; j++) {
+                const u32 k = q * 128 + 32 * j + 8 * quad;
+                xf[u][j] = u32x4{0, 0, 0, 0};
+                if (K % 128 == 0 || k < K) xf[u][j] = *(const chunk_t*)(xp + k);
+            }
+        }
+#pragma unroll
+        for (u32 u = 0; u < U; u++) {
+            if (kt + u >= kt1) break;
+#pragma unroll
+            for (u32 g = 0; g < GPT; g++) {
+                f32x4 base = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (u32 j = g * SPG; j < (g + 1) * SPG; j++)
+                    base = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a24, __builtin_bit_cast(bf16x8, xf[u][j]), base, 0, 0, 0);
+#pragma unroll
+                for (u32 r = 0; r < RT; r++) {
+                    f32x4 c = base;
+#pragma unroll
+                    for (u32 j = g * SPG; j < (g + 1) * SPG; j++)
+                        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes(w[u][r][j]), __builtin_bit_cast(bf16x8, xf[u][j]), c, 0, 0, 0);
+                    const u32x2 sv = s[u][r][g];
+                    acc[r][0] = __builtin_fmaf(c[0], bf16_lo(sv.x), acc[r][0]);
+                    acc[r][1] = __builtin_fmaf(c[1], bf16_hi(sv.x), acc[r][1]);
+                    acc[r][2] = __builtin_fmaf(c[2], bf16_lo(sv.y), acc[r][2]);
+                    acc[r][3] = __builtin_fmaf(c[3], bf16_hi(sv.y), acc[r][3]);
+                }
+            }
+        }
+    }
+
+    // Lane (quad, col) holds rows 4 quad .. +3 of each W tile for column col.
+    // A split's parts meet in LDS and are added in wave order.
+    auto put = [&](u32 r, u32 c, u32 qd, f32x4 v, f32x4 up) {
+        const u32 o = blk * OT + r, n = o * 16 + 4 * qd;
+        if (o >= ONT || c >= cols || n >= NOUT) return;
+        if (SWI) {
+            float g[4] = {v[0], v[1], v[2], v[3]}, w[4] = {up[0], up[1], up[2], up[3]}, h[4];
+            swiglu_n<4>(g, w, h);
+            v = f32x4{h[0], h[1], h[2], h[3]};
+        }
+        store_row(yv, yrow(c), n, v);
+    };
+    if constexpr (SPLIT == 1) {
+#pragma unroll
+        for (u32 r = 0; r < OT; r++) put(r, col, quad, acc[r], acc[SWI ? r + OT : r]);
+    } else {
+        __shared__ f32x4 part[WAVES][RT][MV * 4];
+        if (col < MV)
+#pragma unroll
+            for (u32 r = 0; r < RT; r++) part[wave][r][col * 4 + quad] = acc[r];
+        __syncthreads();
+        for (u32 it = sp * 64 + lane; it < OT * MV * 4; it += SPLIT * 64) {
+            const u32 r = it / (MV * 4), c = it % (MV * 4);
+            f32x4 v = part[gi * SPLIT][r][c], up = part[gi * SPLIT][SWI ? r + OT : r][c];
+#pragma unroll
+            for (u32 q = 1; q < SPLIT; q++) {
+                v += part[gi * SPLIT + q][r][c];
+                if (SWI) up += part[gi * SPLIT + q][r + OT][c];
+            }
+            put(r, c / 4, c % 4, v, up);
+        }
+    }
+}

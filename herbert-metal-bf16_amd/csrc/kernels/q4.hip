@@ -1,0 +1,133 @@
+// q4.hip -- weights of 4 bits: quantised from bf16 (HB_OP 1), laid out from
+// codes and scales in row order (2), read back as bf16 (3).
+//
+// A row's elements stand in groups of GROUP along K, the last one may be
+// short: element = (q - 8) * s, q of 0..15, s the group's bf16 scale.
+// The layout is what the matvec's MFMAs read: tiles of 16 rows x 128 K, K
+// fastest, each 1 KiB of codes: lane l of a wave takes 16 bytes, its word j
+// the 8 codes of row l % 16 at K 32 j + 8 (l / 16) of the tile, one MFMA
+// step's operand.  In a word, element e stands at bits 4 (e / 2) (+ 16 for odd
+// e), all rotated left by 3, so that a rotation by 4 i and a mask leave
+// elements 2 i and 2 i + 1 in the top mantissa bits of two bf16.  After the
+// last tile's codes the scales, per tile [row / 4][group][row % 4].  Rows past
+// N and elements past K hold the code 8, their scales 0.
+//
+// All three are bound by the bf16 side's bytes.  A wave handles a tile: 16
+// bytes of bf16 a lane in four passes of 4 rows x 256 bytes.
+#include "hb_common.h"
+
+constexpr u32 K = HB_K, N = HB_N, GROUP = HB_GROUP;
+constexpr u32 KT = (K + 127) / 128, NT = (N + 15) / 16, TILES = KT * NT;
+constexpr u32 GPT = 128 / GROUP;        // groups of a tile
+constexpr u32 GROUPS = (K + GROUP - 1) / GROUP;  // of a row
+constexpr u64 BLOB = (u64)TILES * (1024 + 32 * GPT);  // bytes of a matrix
+static_assert(K % 8 == 0, "K a multiple of 8");
+static_assert(GROUP == 32 || GROUP == 64 || GROUP == 128, "groups of 32, 64 or 128");
+
+// Tensors may start at any element.
+typedef u32x4 chunk_t __attribute__((aligned(2)));
+
+// Word of chunk ch (8 elements) of row `row` within a tile's 256 words.
+HB_DEV u32 word_at(u32 row, u32 ch) { return ((ch & 3u) * 16 + row) * 4 + (ch >> 2); }
+// Scale of group g of row `row` within a tile's 16 * GPT scales.
+HB_DEV u32 scale_at(u32 row, u32 g) { return (row >> 2) * 4 * GPT + g * 4 + (row & 3u); }
+HB_DEV u32 rotl(u32 v, u32 s) { return __builtin_amdgcn_alignbit(v, v, 32 - s); }
+
+#if HB_OP == 1 || HB_OP == 2
+extern "C" __global__ __launch_bounds__(256) void HB_NAME(const u16* __restrict__ src,
+#if HB_OP == 2
+                                                            const u16* __restrict__ scales,
+#endif
+                                                            unsigned char* __restrict__ dst, u32 count) {
+    __shared__ u32 words[4][256];
+    const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const u64 id = (u64)blockIdx.x * 4 + wave, all = (u64)count * TILES;
+    const bool live = id < all;
+    const u64 mat = live ? id / TILES : 0;
+    const u32 tile = live ? (u32)(id % TILES) : 0, nt = tile / KT, kt = tile % KT;
+    unsigned char* blob = dst + mat * BLOB;
+    u16* sc = (u16*)(blob + (u64)TILES * 1024) + (u64)tile * 16 * GPT;
+    const u32 ch = lane & 15u, k = kt * 128 + ch * 8;
+#pragma unroll
+    for (u32 i = 0; i < 4; i++) {
+        const u32 row = 4 * i + (lane >> 4), n = nt * 16 + row;
+        const bool in = live && n < N && k < K;
+        u32 nw = 0x88888888u;
+#if HB_OP == 1
+        u32x4 v = {0, 0, 0, 0};
+        if (in) v = *(const chunk_t*)(src + (mat * N + n) * K + k);
+        // The group's largest and smallest element; a group with a NaN or an
+        // infinity stands for NaN.
+        float hi = 0.0f, lo = 0.0f;
+        u32 bad = 0;
+        float w[8];
+#pragma unroll
+        for (u32 e = 0; e < 8; e++) {
+            w[e] = e & 1 ? bf16_hi(v[e / 2]) : bf16_lo(v[e / 2]);
+            hi = __builtin_fmaxf(hi, w[e]);
+            lo = __builtin_fminf(lo, w[e]);
+            bad |= !(__builtin_fabsf(w[e]) <= 3.4e38f);
+        }
+#pragma unroll
+        for (u32 o = 1; o < GROUP / 8; o *= 2) {
+            hi = __builtin_fmaxf(hi, __shfl_xor(hi, o, 64));
+            lo = __builtin_fminf(lo, __shfl_xor(lo, o, 64));
+            bad |= __shfl_xor(bad, o, 64);
+        }
+        // s = the element of largest size (the positive one of two) / -8,
+        // which loses bits only among the subnormals.
+        const u32 sb = bad ? 0x7fc0u : f32_to_bf16((hi >= -lo ? hi : lo) * -0.125f);
+        const float s = bf16_to_f32(sb);
+        if (!bad && s != 0.0f) {
+            nw = 0;
+#pragma unroll
+            for (u32 e = 0; e < 8; e++) {
+                const float q = __builtin_fminf(__builtin_fmaxf(__builtin_rintf(__fdiv_rn(w[e], s)), -8.0f), 7.0f);
+                nw |= (u32)(int)(q + 8.0f) << (4 * (e / 2) + 16 * (e & 1));
+            }
+        }
+        if (live && ch % (GROUP / 8) == 0) sc[scale_at(row, ch / (GROUP / 8))] = n < N && k < K ? (u16)sb : 0;
+#else
+        // Row order: byte b of a row holds element 2 b in its low half.
+        if (in) {
+            const u16* p = src + ((mat * N + n) * K + k) / 4;
+            const u32 b = p[0] | (u32)p[1] << 16;
+            nw = 0;
+#pragma unroll
+            for (u32 e = 0; e < 8; e++) nw |= (b >> (4 * e) & 15u) << (4 * (e / 2) + 16 * (e & 1));
+        }
+        if (live && ch % (GROUP / 8) == 0)
+            sc[scale_at(row, ch / (GROUP / 8))] = n < N && k < K ? scales[(mat * N + n) * GROUPS + k / GROUP] : 0;
+#endif
+        words[wave][word_at(row, ch)] = rotl(nw, 3);
+    }
+    __syncthreads();
+    if (live) ((u32x4*)(blob + (u64)tile * 1024))[lane] = ((u32x4*)words[wave])[lane];
+}
+
+#elif HB_OP == 3
+extern "C" __global__ __launch_bounds__(256) void HB_NAME(const unsigned char* __restrict__ src,
+                                                            u16* __restrict__ dst, u32 count) {
+    const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const u64 id = (u64)blockIdx.x * 4 + wave;
+    if (id >= (u64)count * TILES) return;
+    const u64 mat = id / TILES;
+    const u32 tile = (u32)(id % TILES), nt = tile / KT, kt = tile % KT;
+    const unsigned char* blob = src + mat * BLOB;
+    const u32* words = (const u32*)(blob + (u64)tile * 1024);
+    const u16* sc = (const u16*)(blob + (u64)TILES * 1024) + (u64)tile * 16 * GPT;
+    const u32 ch = lane & 15u, k = kt * 128 + ch * 8;
+#pragma unroll
+    for (u32 i = 0; i < 4; i++) {
+        const u32 row = 4 * i + (lane >> 4), n = nt * 16 + row;
+        if (n >= N || k >= K) continue;
+        const u32 nw = rotl(words[word_at(row, ch)], 29);
+        const float s = bf16_to_f32(sc[scale_at(row, ch / (GROUP / 8))]);
+        u32x4 o;
+#pragma unroll
+        for (u32 e = 0; e < 4; e++)
+            o[e] = pack_bf16x2((float)((int)(nw >> (4 * e) & 15u) - 8) * s, (float)((int)(nw >> (16 + 4 * e) & 15u) - 8) * s);
+        *(chunk_t*)(dst + (mat * N + n) * K + k) = o;
+    }
+}
+#endif

@@ -89,6 +89,19 @@ class Kind(enum.IntEnum):
     ROUND_PROBE = 11
     MOE_OUT = 12
     RMSNORM = 13
+    Q4_QUANTIZE = 14
+    Q4_PACK = 15
+    Q4_DEQUANTIZE = 16
+    MATVEC_Q4 = 17
+    BLOCK_NORM = 18
+
+
+class Gate(enum.IntEnum):
+    """block_norm's gate on the block's output (enum hb_norm_parts)."""
+    Off = 0
+    Rows = 16
+    Elements = 32
+    Channels = 48
 
 
 class Rows(enum.IntEnum):
@@ -201,6 +214,10 @@ lib.hb_engine_matvec.argtypes = [_P, _u32, _u32, _u32, _u32, ctypes.POINTER(Rang
 lib.hb_engine_matvec_fused.argtypes = [_P, _u32, _u32, _u32, _u32, _u32, _u32, _u32,
                                        ctypes.POINTER(Range), _u32, Range, Range, Range,
                                        ctypes.POINTER(_i32)]
+lib.hb_engine_matvec_q4.argtypes = [_P, _u32, _u32, _u32, _u32, _u32, ctypes.POINTER(Range), _u32, Range, Range,
+                                    ctypes.POINTER(_i32)]
+lib.hb_engine_matvec_q4_candidates.argtypes = [_P, _u32, _u32, _u32, _u32, _u32, ctypes.POINTER(Desc), _u32,
+                                               ctypes.POINTER(_u32)]
 lib.hb_engine_experts.argtypes = [_P, _u32, _u32, _u32, _u32, _u32, ctypes.POINTER(MoeIo),
                                   ctypes.POINTER(_i32), ctypes.POINTER(_u32)]
 lib.hb_engine_gemm_candidates.argtypes = [_P, _u32, _u32, _u32, ctypes.POINTER(Desc), _u32,
@@ -299,6 +316,61 @@ def matvec(kdim, n, out, mv_m=1, rows=4, split=1, persist=0, form=0, unroll=4, x
     return Desc(kind=Kind.MATVEC, k=kdim, n=n, out=out, mv_m=mv_m, rows=rows, split=split,
                 persist=persist, form=form, unroll=unroll, xsrc=xsrc, eps_bits=eps_bits,
                 plus_one=1 if plus_one else 0, x_lds=1 if x_lds else 0, mv_waves=waves)
+
+
+lib.hb_q4_bytes.argtypes = [_u32, _u32, _u32]
+lib.hb_q4_bytes.restype = _u64
+
+
+def q4_bytes(kdim, n, group=32):
+    """Bytes of a packed 4-bit matrix of n rows of kdim (hb_q4_bytes)."""
+    b = lib.hb_q4_bytes(int(kdim), int(n), int(group))
+    if not b:
+        raise HerbertError(HB_ERR_UNSUPPORTED, "q4 %dx%d in groups of %d: K a multiple of 8, groups of 32, 64 or 128" %
+                           (kdim, n, group))
+    return b
+
+
+def q4_quantize(kdim, n, group=32):
+    """W [n][kdim] bf16 -> the packed 4-bit matrix: per group s = bf16(its element of largest size
+    / -8) and q = clamp(round(w / s), -8, 7) + 8, ties to even (bindings W, q4; launched over the
+    count of matrices).  A group with a NaN or an infinity stands for NaN."""
+    return Desc(kind=Kind.Q4_QUANTIZE, k=kdim, n=n, bk=group)
+
+
+def q4_pack(kdim, n, group=32):
+    """Codes [n][kdim / 2] bytes, the even element in a byte's low half, and scales
+    [n][ceil(kdim / group)] bf16 -> the packed 4-bit matrix (bindings codes, scales, q4)."""
+    return Desc(kind=Kind.Q4_PACK, k=kdim, n=n, bk=group)
+
+
+def q4_dequantize(kdim, n, group=32):
+    """The packed 4-bit matrix -> W [n][kdim] bf16, (q - 8) * s (bindings q4, W): what a prefill's
+    GEMM reads."""
+    return Desc(kind=Kind.Q4_DEQUANTIZE, k=kdim, n=n, bk=group)
+
+
+def matvec_q4(kdim, n, out, group=32, mv_m=1, rows=0, split=0, waves=0, unroll=0):
+    """y[m][n] = x[m][kdim].W^T over a packed 4-bit matrix for m <= mv_m <= 16 (bindings q4, x, y);
+    zeros: the shape's defaults.  out Residual adds with one rounding, Swiglu as matvec's."""
+    return Desc(kind=Kind.MATVEC_Q4, k=kdim, n=n, out=out, bk=group, mv_m=mv_m, rows=rows, split=split,
+                mv_waves=waves, unroll=unroll)
+
+
+def experts_q4(kdim, n, out, group, rows_of, top_k, experts, rows_max, rows=0, split=0, waves=0, unroll=0):
+    """matvec_q4 over the routed experts of a block of up to rows_max rows, tiles of moe_sort with
+    bm = 16 (bindings state, q4 of every expert, X, Y, list, tiles)."""
+    return Desc(kind=Kind.MATVEC_Q4, k=kdim, n=n, out=out, bk=group, mv_m=16, rows=rows, split=split, mv_waves=waves,
+                unroll=unroll, rows_of=rows_of, top_k=top_k, experts=experts, rows_max=rows_max,
+                tiles=moe_tiles(rows_max, top_k, experts, 16))
+
+
+def block_norm(d, eps, plus_one=False, post=False, pre=True, gate=Gate.Off, scales=False):
+    """A block's post norm, gate, residual add with the layer's scales and the next block's norm
+    over rows of d (enum hb_norm_parts): bindings x, y, xo[, h][, w_post][, gate][, scales][, w_pre]."""
+    eps_bits = struct.unpack("<I", struct.pack("<f", eps))[0]
+    return Desc(kind=Kind.BLOCK_NORM, n=d, eps_bits=eps_bits, plus_one=1 if plus_one else 0,
+                form=(1 if post else 0) | (2 if pre else 0) | (4 if scales else 0) | int(gate))
 
 
 class Gpu:
@@ -581,6 +653,21 @@ class Engine:
                                          norm_w if norm_w is not None else Range(), ctypes.byref(kern)))
         return kern.value
 
+    def matvec_q4_candidates(self, k, n, out, group, mv_m):
+        """The descriptors mv_q4 times, the shape's defaults first."""
+        cap = 64
+        arr = (Desc * cap)()
+        cnt = _u32()
+        check(lib.hb_engine_matvec_q4_candidates(self.h, k, n, int(out), group, mv_m, arr, cap, ctypes.byref(cnt)))
+        return [arr[i].replace() for i in range(min(cnt.value, cap))]
+
+    def mv_q4(self, k, n, out, group, mv_m, ws, x, y):
+        """mv over packed 4-bit matrices (hb_engine_matvec_q4)."""
+        arr = (Range * len(ws))(*ws)
+        kern = _i32()
+        check(lib.hb_engine_matvec_q4(self.h, k, n, int(out), group, mv_m, arr, len(ws), x, y, ctypes.byref(kern)))
+        return kern.value
+
     def experts(self, experts, top_k, hidden, inter, m, io):
         """io: MoeIo; returns ([sort, gate_up, down, gather or -1], rows per tile)."""
         ks = (_i32 * 4)()
@@ -598,10 +685,15 @@ class MoeLayer:
     (scatter to slot rows) -> moe_combine.  Owns its device buffers; the
     kernels come from Engine.experts (expert_pipes), timed on the route of
     `scores` ([rows][experts] bf16, routed here first: the reference's
-    real_route, qwen.rs:2340) and `x` if given."""
+    real_route, qwen.rs:2340) and `x` if given.
+
+    q4_group: w_gate_up and w_down are packed 4-bit matrices of all experts
+    (q4_quantize / q4_pack over [2 inter][hidden] and [hidden][inter], in
+    groups of q4_group), read by experts_q4 over tiles of 16 rows; the
+    engine times nothing then."""
 
     def __init__(self, gpu, engine, experts, top_k, hidden, inter, rows, w_gate_up, w_down,
-                 scores=None, x=None):
+                 scores=None, x=None, q4_group=0):
         self.gpu, self.e, self.k, self.h, self.mi, self.rows = gpu, experts, top_k, hidden, inter, rows
         pairs = rows * top_k
         g = gpu
@@ -632,6 +724,13 @@ class MoeLayer:
             g.upload(b["scores"], scores)
             g.launch(self.route_k, [r(b["scores"]), r(b["route"])], rows)
             g.sync()
+        if q4_group:
+            self.bm = 16
+            descs = [Desc(kind=Kind.SORT, experts=experts, top_k=top_k, bm=16, rows_max=rows),
+                     experts_q4(hidden, 2 * inter, Out.Swiglu, q4_group, Rows.Gather, top_k, experts, rows),
+                     experts_q4(inter, hidden, Out.Bf16, q4_group, Rows.Scatter, top_k, experts, rows)]
+            self.kernels, self.fused = [gpu.pipeline(d) for d in descs] + [-1], True
+            return
         self.kernels, self.bm = engine.experts(experts, top_k, hidden, inter, rows, self.io)
         self.fused = gpu.kernel_kind(self.kernels[1]) == Kind.GEMM_SWIGLU
 

@@ -83,7 +83,35 @@ enum hb_kind {
     HB_KIND_COMBINE = 10,    /* moe_combine (qwen_kernels.rs:2119-2165) */
     HB_KIND_ROUND_PROBE = 11, /* herbert-metal-probe round (bin/herbert-metal-probe.rs:7-11) */
     HB_KIND_MOE_OUT = 12,    /* moe_out (qwen_kernels.rs:2163-2214): the MoE block's end */
-    HB_KIND_RMSNORM = 13     /* rmsnorm (kernels.rs:48-103): the block's input norm, rows of n */
+    HB_KIND_RMSNORM = 13,    /* rmsnorm (kernels.rs:48-103): the block's input norm, rows of n */
+    /* Weights of 4 bits (the reference's Q4 forms: kernels.rs:451-635,
+     * 990-1452, q4.rs).  A row's elements k in groups of `bk` (32, 64 or 128,
+     * the last one may be short): element = (q - 8) * s, q of 0..15, s the
+     * group's bf16 scale.  k a multiple of 8, any n.  The packed matrix
+     * ("q4", hb_q4_bytes) is a layout of this library. */
+    HB_KIND_Q4_QUANTIZE = 14,   /* W [n][k] bf16 -> q4; m = matrices, one after the other */
+    HB_KIND_Q4_PACK = 15,       /* codes [n][k/2] bytes (element 2 b of a row in byte b's low
+                                 * half), scales [n][ceil(k/bk)] bf16 -> q4; m = matrices */
+    HB_KIND_Q4_DEQUANTIZE = 16, /* q4 -> W [n][k] bf16, (q - 8) * s rounded once; m = matrices */
+    HB_KIND_MATVEC_Q4 = 17,     /* matvec_q4: y[m][n] = x[m][k].W^T, m <= mv_m <= 16; or the
+                                 * experts' over moe_sort's tiles of 16 rows (rows_of) */
+    HB_KIND_BLOCK_NORM = 18     /* a block's post norm, its gate, the residual add and the next
+                                 * block's norm, rows of n (enum hb_norm_parts in `form`) */
+};
+
+/* HB_KIND_BLOCK_NORM's parts, in hb_desc.form.  Per row, in f32:
+ *   u  = y, or y / sqrt(mean(y^2) + eps) * w_post       (HB_NORM_POST)
+ *   v  = u, or gate * u                                 (HB_NORM_GATE_*)
+ *   xo = rne(a * x + b * v), a and b 1 or scales[0..1]  (HB_NORM_SCALES)
+ *   h  = rne(xo / sqrt(mean(xo^2) + eps) * w_pre)       (HB_NORM_PRE)
+ * with the weights used as w + 1 for plus_one; h of xo as it is stored. */
+enum hb_norm_parts {
+    HB_NORM_POST = 1,
+    HB_NORM_PRE = 2,
+    HB_NORM_SCALES = 4,
+    HB_NORM_GATE_ROWS = 16,     /* sigmoid(gate[row]) */
+    HB_NORM_GATE_ELEMENTS = 32, /* sigmoid(gate[row][i]) */
+    HB_NORM_GATE_CHANNELS = 48  /* gate[i] as it is */
 };
 
 enum hb_out { /* Out (kernels.rs:30-43) */
@@ -227,6 +255,20 @@ double hb_compile_seconds(hb_gpu *gpu);
  *   COMBINE: y, route, out    ROUND_PROBE: state (state[0] = chunk), out_int, out_hw
  *   MOE_OUT: xn, shared_gate, experts, shared, x (x updated in place)
  *   RMSNORM: x, w, y (eps_bits, plus_one of the descriptor)
+ *   Q4_QUANTIZE: W, q4    Q4_PACK: codes, scales, q4    Q4_DEQUANTIZE: q4, W
+ *   MATVEC_Q4: q4, x, y; over experts: state, q4 [experts], X, Y, list, tiles
+ *   BLOCK_NORM: x, y, xo, then those its parts name, in this order: h (PRE),
+ *     w_post (POST), gate, scales (2 f32, SCALES), w_pre (PRE).  xo may be x
+ *     or y, h may be y or x, or either an element gate, as a whole; no other
+ *     overlap.
+ * The bindings of these five start at a multiple of their element (2 bytes,
+ * f32 and u32 4, q4 16), and what a launch writes overlaps nothing else it
+ * binds: both are checked.  Of MATVEC_Q4: HB_OUT_BF16, _F32, _RESIDUAL
+ * (y = rne(y + sum), one rounding) and _SWIGLU (n / 2 a multiple of 16, h =
+ * rne(g * sigmoid(g) * u) of the f32 sums).  x beyond 2^123 or infinite
+ * gives NaN.  Over experts (rows_of HB_ROWS_GATHER: x rows through the list,
+ * y rows in sorted order; HB_ROWS_SCATTER: the other way round) the table is
+ * one of tiles of up to 16 rows; y rows of no tile are left as they are.
  * `m` is the rows of the block (the kernels read state[3], never beyond m).
  * A split-K GEMM (ksplit > 1) launched over more rows than any earlier
  * split launch on this context first grows the context's workspace: the
@@ -268,6 +310,11 @@ int hb_graph_time(hb_graph *graph, uint32_t reps, double *seconds);
 void hb_graph_free(hb_graph *graph);
 /* submit_wait (metal/gpu.rs:209-221): wait for the stream. */
 int hb_sync(hb_gpu *gpu);
+
+/* Bytes of a packed 4-bit matrix of n rows of k in groups of `group` (k a
+ * multiple of 8, group 32, 64 or 128), 0 for a shape the kernels refuse.
+ * Matrices of one shape stand one after the other at this distance. */
+uint64_t hb_q4_bytes(uint32_t k, uint32_t n, uint32_t group);
 
 /* ---- synthetic inputs (host side, no GPU) ---- */
 /* n bf16 values ~ N(0, std^2): splitmix64(seed) -> two uniforms -> Box-Muller
@@ -352,6 +399,19 @@ int hb_engine_matvec_candidates(hb_engine *engine, uint32_t k, uint32_t n, uint3
                                 uint32_t xsrc, uint32_t eps_bits, uint32_t plus_one, uint32_t mv_m,
                                 hb_desc *descs, uint32_t cap, uint32_t *count);
 
+/* mv_full (qwen.rs:1311-1511) over weights of 4 bits: with mv.auto the
+ * MATVEC_Q4 forms timed over every matrix of the shape (`ws`, mv.cold) and the
+ * fastest kept under "{k}x{n} q4/{group} {Out} m{mv_m}", y as it was
+ * afterwards; else the form the shape's defaults give. */
+int hb_engine_matvec_q4(hb_engine *engine, uint32_t k, uint32_t n, uint32_t out, uint32_t group,
+                        uint32_t mv_m, const hb_range *ws, uint32_t nws, hb_range x, hb_range y,
+                        int32_t *kernel);
+/* The descriptors hb_engine_matvec_q4 times, the defaults first; *count =
+ * how many, the first min(count, cap) written. */
+int hb_engine_matvec_q4_candidates(hb_engine *engine, uint32_t k, uint32_t n, uint32_t out,
+                                   uint32_t group, uint32_t mv_m, hb_desc *descs, uint32_t cap,
+                                   uint32_t *count);
+
 /* QwenEngine::expert_pipes (qwen.rs:2326-2391): the sort, the grouped
  * gate_up GEMM (Gather) and down GEMM (Scatter) of an MoE layer of `experts`
  * experts, top_k slots, hidden `hidden`, expert intermediate `inter`, for
@@ -385,7 +445,10 @@ int hb_engine_experts(hb_engine *engine, uint32_t experts, uint32_t top_k, uint3
  * HB_KIND_GEMM_SWIGLU); combine: moe_combine (n = hidden).  io as for
  * hb_engine_experts (state[3] = m; route holds the m rows' route; xs is
  * read only with a gather, egu only without the fused SwiGLU); out
- * [m][hidden] bf16.  Every launch's bindings are checked first. */
+ * [m][hidden] bf16.  Every launch's bindings are checked first.  Experts in
+ * 4 bits: kernels[1] and [2] of kind HB_KIND_MATVEC_Q4 over a sort of
+ * 16-row tiles, w_gate_up and w_down the packed matrices of all experts; a
+ * gate|up with HB_OUT_SWIGLU writes EHB itself. */
 int hb_moe_experts_run(hb_gpu *gpu, const int32_t kernels[4], int32_t swiglu, int32_t combine,
                        const hb_moe_io *io, hb_range out, uint32_t m);
 
@@ -424,7 +487,7 @@ const char *hb_engine_log(hb_engine *engine);
 int hb_engine_log_summary(hb_engine *engine);
 /* The engine's timed choices so far as text (no counterpart in the
  * reference, which re-times at every load): one line per choice, tab
- * separated -- "gemm" / "gate_up" / "mv" / "experts", the choice's key (as
+ * separated -- "gemm" / "gate_up" / "mv" / "mv_q4" / "experts", the choice's key (as
  * the [autotune] lines print it), then each kernel of the choice as its
  * name and its descriptor's fields (decimal, hb_desc order; "-" for none;
  * experts: the tile rows first); after a dense GEMM's kernels, for each
