@@ -21,6 +21,7 @@ constexpr u32 KT = (K + 127) / 128, NT = (N + 15) / 16, TILES = KT * NT, GPT = 1
 constexpr u64 BLOB = (u64)TILES * (1024 + 32 * GPT);
 constexpr u32 RT = HB_RT, SPLIT = HB_SPLIT, WAVES = HB_WAVES, U = HB_UNROLL, ROWS = HB_ROWS, TOPK = HB_TOPK;
 constexpr bool SWI = OUT == 3;
+constexpr u32 AR = MV < 4 ? MV : 4;                      // x rows of a lane's sums
 constexpr u32 NOUT = SWI ? N / 2 : N;
 constexpr u32 OT = SWI ? RT / 2 : RT;                    // output tiles of a wave
 constexpr u32 ONT = SWI ? NT / 2 : NT;                   // output tiles
@@ -29,49 +30,59 @@ constexpr u32 NWG = (NBLK + GPW - 1) / GPW;
 static_assert(K % 8 == 0 && (!SWI || (RT % 2 == 0 && N % 32 == 0)), "shape");
 static_assert(WAVES % SPLIT == 0 && MV >= 1 && MV <= 16, "waves");
 
-typedef u32x4 chunk_t __attribute__((aligned(2)));
-typedef u32x2 half_t __attribute__((aligned(2)));
-typedef f32x4 f32x4_u __attribute__((aligned(4)));
+// At most 256 registers: the compiler then keeps the MFMAs' sums in VGPRs,
+// where the scales multiply them, and not in AGPRs.
+#define HB_VGPR_FORM __attribute__((amdgpu_waves_per_eu(2)))
 
-// Codes 8 i + 0..7 of a word as bf16 16 + q, the MFMA's A operand.
-HB_DEV bf16x8 codes(u32 w) {
+typedef u32x4 chunk_t __attribute__((aligned(2)));
+
+// The scales of a row's groups in a tile.
+template <u32 groups>
+struct Scales {
+    typedef u16 type;
+};
+template <>
+struct Scales<2> {
+    typedef u32 type;
+};
+template <>
+struct Scales<4> {
+    typedef u32x2 type;
+};
+typedef Scales<GPT>::type scales_t;
+HB_DEV float scale_of(u16 s, u32) { return bf16_to_f32(s); }
+HB_DEV float scale_of(u32 s, u32 g) { return g ? bf16_hi(s) : bf16_lo(s); }
+HB_DEV float scale_of(u32x2 s, u32 g) { return scale_of(g < 2 ? s.x : s.y, g & 1u); }
+
+HB_DEV f32x4 mfma(u32x4 x, bf16x8 w, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), w, c, 0, 0, 0);
+}
+
+// A word's codes as bf16 16 + q, the MFMA's B operand.  `mask` and `base`
+// are 0x00780078 and 0x41804180 in registers: an and-or takes no literal.
+HB_DEV bf16x8 codes(u32 w, u32 mask, u32 base) {
     u32x4 a;
 #pragma unroll
-    for (u32 i = 0; i < 4; i++) a[i] = (__builtin_amdgcn_alignbit(w, w, 4 * i) & 0x00780078u) | 0x41804180u;
+    for (u32 i = 0; i < 4; i++) a[i] = (__builtin_amdgcn_alignbit(w, w, 4 * i) & mask) | base;
     return __builtin_bit_cast(bf16x8, a);
 }
 
-HB_DEV void store_row(void* yv, u64 row, u32 n, f32x4 v) {
+// Out of the sum of y[row][n].
+HB_DEV void store(void* yv, u64 row, u32 n, float v) {
+    const u64 at = row * NOUT + n;
     if (OUT == 1) {
-        float* y = (float*)yv + row * NOUT + n;
-        if (NOUT % 4 == 0) {
-            *(f32x4_u*)y = v;
-        } else {
-#pragma unroll
-            for (u32 i = 0; i < 4; i++)
-                if (n + i < NOUT) y[i] = v[i];
-        }
-        return;
-    }
-    u16* y = (u16*)yv + row * NOUT + n;
-    if (NOUT % 4 == 0) {
-        if (OUT == 2) {
-            const half_t o = *(half_t*)y;
-            v += f32x4{bf16_lo(o.x), bf16_hi(o.x), bf16_lo(o.y), bf16_hi(o.y)};
-        }
-        *(half_t*)y = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+        ((float*)yv)[at] = v;
     } else {
-#pragma unroll
-        for (u32 i = 0; i < 4; i++)
-            if (n + i < NOUT) y[i] = (u16)pack_bf16x2(OUT == 2 ? bf16_to_f32(y[i]) + v[i] : v[i], 0.0f);
+        u16* y = (u16*)yv + at;
+        *y = (u16)pack_bf16x2(OUT == 2 ? bf16_to_f32(*y) + v : v, 0.0f);
     }
 }
 
 #if HB_ROWS == 0
-extern "C" __global__ __launch_bounds__(64 * WAVES) void HB_NAME(const unsigned char* __restrict__ W,
+extern "C" __global__ __launch_bounds__(64 * WAVES) HB_VGPR_FORM void HB_NAME(const unsigned char* __restrict__ W,
                                                                    const u16* __restrict__ x, void* yv, u32 rows) {
 #else
-extern "C" __global__ __launch_bounds__(64 * WAVES) void HB_NAME(
+extern "C" __global__ __launch_bounds__(64 * WAVES) HB_VGPR_FORM void HB_NAME(
     const u32* __restrict__ state, const unsigned char* __restrict__ W, const u16* __restrict__ x, void* yv,
     const u32* __restrict__ list, const u32* __restrict__ tiles, u32 m_launch) {
 #endif
@@ -119,24 +130,26 @@ extern "C" __global__ __launch_bounds__(64 * WAVES) void HB_NAME(
         tn[r] = ((o < ONT ? o : ONT - 1) + (r / OT) * ONT) * KT;
     }
     const u32 kt0 = sp * KT / SPLIT, kt1 = (sp + 1) * KT / SPLIT;
-    const bf16x8 a24 = __builtin_bit_cast(bf16x8, u32x4{0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u});
-    f32x4 acc[RT];
+    const bf16x8 b24 = __builtin_bit_cast(bf16x8, u32x4{0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u});
+    u32 mask = 0x00780078u, one = 0x41804180u;
+    asm("" : "+v"(mask), "+v"(one));
+    float acc[RT][AR];
 #pragma unroll
-    for (u32 r = 0; r < RT; r++) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (u32 r = 0; r < RT; r++)
+#pragma unroll
+        for (u32 i = 0; i < AR; i++) acc[r][i] = 0.0f;
 
     for (u32 kt = kt0; kt < kt1; kt += U) {
         u32x4 w[U][RT], xf[U][4];
-        u32x2 s[U][RT][GPT];
+        scales_t s[U][RT];
 #pragma unroll
         for (u32 u = 0; u < U; u++) {
             const u32 q = kt + u < kt1 ? kt + u : kt1 - 1;
 #pragma unroll
-            for (u32 r = 0; r < RT; r++) {
+            for (u32 r = 0; r < RT; r++)
                 w[u][r] = __builtin_nontemporal_load((const u32x4*)(W + (u64)(tn[r] + q) * 1024) + lane);
-                const u32x2* sp2 = (const u32x2*)(scales + (u64)(tn[r] + q) * 16 * GPT) + quad * GPT;
 #pragma unroll
-                for (u32 g = 0; g < GPT; g++) s[u][r][g] = sp2[g];
-            }
+            for (u32 r = 0; r < RT; r++) s[u][r] = ((const scales_t*)(scales + (u64)(tn[r] + q) * 16 * GPT))[col];
 #pragma unroll
             for (u32 j = 0; j < 4; j++) {
                 const u32 k = q * 128 + 32 * j + 8 * quad;
@@ -151,54 +164,54 @@ extern "C" __global__ __launch_bounds__(64 * WAVES) void HB_NAME(
             for (u32 g = 0; g < GPT; g++) {
                 f32x4 base = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (u32 j = g * SPG; j < (g + 1) * SPG; j++)
-                    base = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a24, __builtin_bit_cast(bf16x8, xf[u][j]), base, 0, 0, 0);
+                for (u32 j = g * SPG; j < (g + 1) * SPG; j++) base = mfma(xf[u][j], b24, base);
 #pragma unroll
                 for (u32 r = 0; r < RT; r++) {
                     f32x4 c = base;
 #pragma unroll
-                    for (u32 j = g * SPG; j < (g + 1) * SPG; j++)
-                        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes(w[u][r][j]), __builtin_bit_cast(bf16x8, xf[u][j]), c, 0, 0, 0);
-                    const u32x2 sv = s[u][r][g];
-                    acc[r][0] = __builtin_fmaf(c[0], bf16_lo(sv.x), acc[r][0]);
-                    acc[r][1] = __builtin_fmaf(c[1], bf16_hi(sv.x), acc[r][1]);
-                    acc[r][2] = __builtin_fmaf(c[2], bf16_lo(sv.y), acc[r][2]);
-                    acc[r][3] = __builtin_fmaf(c[3], bf16_hi(sv.y), acc[r][3]);
+                    for (u32 j = g * SPG; j < (g + 1) * SPG; j++) c = mfma(xf[u][j], codes(w[u][r][j], mask, one), c);
+                    const float sc = scale_of(s[u][r], g);
+#pragma unroll
+                    for (u32 i = 0; i < AR; i++) acc[r][i] = __builtin_fmaf(sc, c[i], acc[r][i]);
                 }
             }
         }
     }
 
-    // Lane (quad, col) holds rows 4 quad .. +3 of each W tile for column col.
-    // A split's parts meet in LDS and are added in wave order.
-    auto put = [&](u32 r, u32 c, u32 qd, f32x4 v, f32x4 up) {
-        const u32 o = blk * OT + r, n = o * 16 + 4 * qd;
+    // Lane (quad, col) holds row col of each W tile for x rows 4 quad .. +3.
+    auto put = [&](u32 r, u32 c, u32 nr, float v, float up) {
+        const u32 o = blk * OT + r, n = o * 16 + nr;
         if (o >= ONT || c >= cols || n >= NOUT) return;
         if (SWI) {
-            float g[4] = {v[0], v[1], v[2], v[3]}, w[4] = {up[0], up[1], up[2], up[3]}, h[4];
-            swiglu_n<4>(g, w, h);
-            v = f32x4{h[0], h[1], h[2], h[3]};
+            float h;
+            swiglu_n<1>(&v, &up, &h);
+            v = h;
         }
-        store_row(yv, yrow(c), n, v);
+        store(yv, yrow(c), n, v);
     };
     if constexpr (SPLIT == 1) {
 #pragma unroll
-        for (u32 r = 0; r < OT; r++) put(r, col, quad, acc[r], acc[SWI ? r + OT : r]);
-    } else {
-        __shared__ f32x4 part[WAVES][RT][MV * 4];
-        if (col < MV)
+        for (u32 r = 0; r < OT; r++)
 #pragma unroll
-            for (u32 r = 0; r < RT; r++) part[wave][r][col * 4 + quad] = acc[r];
+            for (u32 i = 0; i < AR; i++) put(r, 4 * quad + i, col, acc[r][i], acc[SWI ? r + OT : r][i]);
+    } else {
+        // A split's parts meet in LDS and are added in wave order.
+        __shared__ float part[WAVES][RT][MV * 16];
+#pragma unroll
+        for (u32 r = 0; r < RT; r++)
+#pragma unroll
+            for (u32 i = 0; i < AR; i++)
+                if (4 * quad + i < MV) part[wave][r][(4 * quad + i) * 16 + col] = acc[r][i];
         __syncthreads();
-        for (u32 it = sp * 64 + lane; it < OT * MV * 4; it += SPLIT * 64) {
-            const u32 r = it / (MV * 4), c = it % (MV * 4);
-            f32x4 v = part[gi * SPLIT][r][c], up = part[gi * SPLIT][SWI ? r + OT : r][c];
+        for (u32 it = sp * 64 + lane; it < OT * MV * 16; it += SPLIT * 64) {
+            const u32 r = it / (MV * 16), c = it % (MV * 16);
+            float v = part[gi * SPLIT][r][c], up = part[gi * SPLIT][SWI ? r + OT : r][c];
 #pragma unroll
             for (u32 q = 1; q < SPLIT; q++) {
                 v += part[gi * SPLIT + q][r][c];
                 if (SWI) up += part[gi * SPLIT + q][r + OT][c];
             }
-            put(r, c / 4, c % 4, v, up);
+            put(r, c / 16, c % 16, v, up);
         }
     }
 }

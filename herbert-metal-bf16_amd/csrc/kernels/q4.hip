@@ -9,7 +9,7 @@
 // step's operand.  In a word, element e stands at bits 4 (e / 2) (+ 16 for odd
 // e), all rotated left by 3, so that a rotation by 4 i and a mask leave
 // elements 2 i and 2 i + 1 in the top mantissa bits of two bf16.  After the
-// last tile's codes the scales, per tile [row / 4][group][row % 4].  Rows past
+// last tile's codes the scales, per tile [row][group].  Rows past
 // N and elements past K hold the code 8, their scales 0.
 //
 // All three are bound by the bf16 side's bytes.  A wave handles a tile: 16
@@ -30,7 +30,7 @@ typedef u32x4 chunk_t __attribute__((aligned(2)));
 // Word of chunk ch (8 elements) of row `row` within a tile's 256 words.
 HB_DEV u32 word_at(u32 row, u32 ch) { return ((ch & 3u) * 16 + row) * 4 + (ch >> 2); }
 // Scale of group g of row `row` within a tile's 16 * GPT scales.
-HB_DEV u32 scale_at(u32 row, u32 g) { return (row >> 2) * 4 * GPT + g * 4 + (row & 3u); }
+HB_DEV u32 scale_at(u32 row, u32 g) { return row * GPT + g; }
 HB_DEV u32 rotl(u32 v, u32 s) { return __builtin_amdgcn_alignbit(v, v, 32 - s); }
 
 #if HB_OP == 1 || HB_OP == 2
