@@ -40,7 +40,9 @@ static bool is_gemm(uint32_t kind) {
 
 // The tiles of a packed 4-bit matrix (16 rows x 128 K) and its bytes.
 static uint64_t q4_tiles(uint32_t k, uint32_t n) { return ((uint64_t)k + 127) / 128 * (((uint64_t)n + 15) / 16); }
-static uint64_t q4_bytes(uint32_t k, uint32_t n, uint32_t group) { return q4_tiles(k, n) * (1024 + 4096 / group); }
+static uint64_t q4_bytes(uint32_t k, uint32_t n, uint32_t group) {
+    return q4_tiles(k, n) * 1024 + ((uint64_t)k + 127) / 128 * (((uint64_t)n + 63) / 64) * (16384 / group);
+}
 static bool q4_shape(uint32_t k, uint32_t n, uint32_t group) {
     return k && n && k % 8 == 0 && (group == 32 || group == 64 || group == 128) && q4_tiles(k, n) < (1u << 30);
 }
@@ -395,10 +397,12 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             if (swi && d.n % 32)
                 return fail(HB_ERR_UNSUPPORTED, "matvec_q4 Out::Swiglu: gate and up rows each a multiple of 16");
             if (d.mv_m > 16) return fail(HB_ERR_UNSUPPORTED, "matvec_q4: m <= 16");
-            if ((d.rows != 16 && d.rows != 32 && d.rows != 64) || (swi && d.rows == 16))
-                return fail(HB_ERR_UNSUPPORTED, "matvec_q4: 16, 32 or 64 rows a wave (Out::Swiglu 32 or 64)");
-            if (d.mv_waves > 16 || !pow2(d.mv_waves) || !pow2(d.split) || d.split > d.mv_waves || d.unroll > 4)
-                return fail(HB_ERR_UNSUPPORTED, "matvec_q4: 1, 2, 4, 8 or 16 waves, split no more, unroll 1..4");
+            if ((d.rows != 16 && d.rows != 32 && d.rows != 64 && d.rows != 128) || (swi && d.rows == 16))
+                return fail(HB_ERR_UNSUPPORTED, "matvec_q4: 16, 32, 64 or 128 rows a wave (Out::Swiglu not 16)");
+            if (d.mv_waves > 16 || !pow2(d.mv_waves) || !pow2(d.split) || d.split > d.mv_waves || d.unroll > 4 ||
+                d.dbuf > 1)
+                return fail(HB_ERR_UNSUPPORTED,
+                            "matvec_q4: 1, 2, 4, 8 or 16 waves, split no more, unroll 1..4, dbuf 0 or 1");
             if (experts && (!d.top_k || !d.experts || !d.tiles || !d.rows_max || d.mv_m != 16 ||
                             (d.out != HB_OUT_BF16 && !swi)))
                 return fail(HB_ERR_INVALID,
@@ -409,9 +413,9 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
                          d.top_k, d.experts, d.tiles, d.rows_max);
                 rows = name;
             }
-            snprintf(name, sizeof name, "matvec_q4_%ux%u_g%u%s_r%u_k%u_w%u_u%u_m%u%s", d.k, d.n, d.bk,
+            snprintf(name, sizeof name, "matvec_q4_%ux%u_g%u%s_r%u_k%u_w%u_u%u_d%u_m%u%s", d.k, d.n, d.bk,
                      d.out == HB_OUT_F32 ? "_f32" : d.out == HB_OUT_RESIDUAL ? "_res" : swi ? "_sw" : "", d.rows,
-                     d.split, d.mv_waves, d.unroll, d.mv_m, rows.c_str());
+                     d.split, d.mv_waves, d.unroll, d.dbuf, d.mv_m, rows.c_str());
             e->name = name;
             e->source = "matvec_q4.hip";
             e->threads = 64 * d.mv_waves;
@@ -419,6 +423,7 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             e->defines = {D("HB_K", d.k),          D("HB_N", d.n),         D("HB_GROUP", d.bk),
                           D("HB_OUT", d.out),      D("HB_MV_M", d.mv_m),   D("HB_RT", d.rows / 16),
                           D("HB_SPLIT", d.split),  D("HB_WAVES", d.mv_waves), D("HB_UNROLL", d.unroll),
+                          D("HB_STAGES", d.dbuf + 1),
                           D("HB_ROWS", d.rows_of), D("HB_TOPK", experts ? d.top_k : 1),
                           D("HB_E", experts ? d.experts : 1)};
             return HB_OK;

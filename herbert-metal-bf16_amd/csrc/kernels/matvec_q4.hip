@@ -18,18 +18,20 @@
 
 constexpr u32 K = HB_K, N = HB_N, GROUP = HB_GROUP, OUT = HB_OUT, MV = HB_MV_M;
 constexpr u32 KT = (K + 127) / 128, NT = (N + 15) / 16, TILES = KT * NT, GPT = 128 / GROUP, SPG = GROUP / 32;
-constexpr u64 BLOB = (u64)TILES * (1024 + 32 * GPT);
+constexpr u64 CODES = (u64)TILES * 1024, BLOB = CODES + (u64)((NT + 3) / 4) * KT * 128 * GPT;
 constexpr u32 RT = HB_RT, SPLIT = HB_SPLIT, WAVES = HB_WAVES, U = HB_UNROLL, ROWS = HB_ROWS, TOPK = HB_TOPK;
 constexpr bool SWI = OUT == 3;
-constexpr u32 AR = MV < 4 ? MV : 4;                      // x rows of a lane's sums
 constexpr u32 NOUT = SWI ? N / 2 : N;
 constexpr u32 OT = SWI ? RT / 2 : RT;                    // output tiles of a wave
 constexpr u32 ONT = SWI ? NT / 2 : NT;                   // output tiles
 constexpr u32 NBLK = (ONT + OT - 1) / OT, GPW = WAVES / SPLIT;
 constexpr u32 NWG = (NBLK + GPW - 1) / GPW;
+// Every wave's tiles of K fill its stages.
+constexpr bool WHOLE = KT % (SPLIT * U * HB_STAGES) == 0;
 static_assert(K % 8 == 0 && (!SWI || (RT % 2 == 0 && N % 32 == 0)), "shape");
 static_assert(WAVES % SPLIT == 0 && MV >= 1 && MV <= 16, "waves");
 
+#define HB_INLINE2 __attribute__((always_inline))
 // At most 256 registers: the compiler then keeps the MFMAs' sums in VGPRs,
 // where the scales multiply them, and not in AGPRs.
 #define HB_VGPR_FORM __attribute__((amdgpu_waves_per_eu(2)))
@@ -78,108 +80,128 @@ HB_DEV void store(void* yv, u64 row, u32 n, float v) {
     }
 }
 
-#if HB_ROWS == 0
-extern "C" __global__ __launch_bounds__(64 * WAVES) HB_VGPR_FORM void HB_NAME(const unsigned char* __restrict__ W,
-                                                                   const u16* __restrict__ x, void* yv, u32 rows) {
-#else
-extern "C" __global__ __launch_bounds__(64 * WAVES) HB_VGPR_FORM void HB_NAME(
-    const u32* __restrict__ state, const unsigned char* __restrict__ W, const u16* __restrict__ x, void* yv,
-    const u32* __restrict__ list, const u32* __restrict__ tiles, u32 m_launch) {
-#endif
+// Workgroup `wg` of a matrix: `cols` <= M columns, column c from x row
+// xrow(c) into y row yrow(c).
+//
+// The MFMA's 16 x rows hold C = 16 / TG of them TG times over, so that the
+// quads of lanes all have the sums of a tile's 16 W rows and each quad keeps
+// one of TG tiles: a set of TG tiles takes one load of scales and one
+// register of sums for each of a lane's x rows.
+template <u32 M, typename XRow, typename YRow>
+HB_DEV void rows_of_w(const unsigned char* __restrict__ W, const u16* __restrict__ x, void* yv, float* part, u32 wg,
+                      u32 cols, XRow xrow, YRow yrow) {
+    constexpr u32 REP = M <= 4 ? 4 : M <= 8 ? 2 : 1, TG = RT < REP ? RT : REP, SETS = RT / TG;
+    constexpr u32 C = 16 / TG, AR = M < 4 ? M : 4;
+    static_assert(RT % TG == 0 && M <= C, "tiles in whole sets");
     const u32 tid = threadIdx.x, lane = tid & 63u, col = lane & 15u, quad = lane >> 4;
     const u32 wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const u32 sp = wave % SPLIT, gi = wave / SPLIT;
-    u32 wg = blockIdx.x;
-#if HB_ROWS == 0
+    const u32 mine = quad * TG / 4;     // the lane's tile of a set
+    const u32 row0 = (4 * quad) % C;    // its x rows: row0 .. + AR - 1
     // Columns past the rows repeat the last one and are never stored.
-    const u32 cols = rows < MV ? rows : MV;
-    const u64 xrow = col < cols ? col : cols - 1;
-    auto yrow = [&](u32 c) -> u64 { return c; };
-#else
-    const u32 m = rows_of_state(state, m_launch), pairs = m * TOPK;
-    const u32 t = wg / NWG;
-    wg %= NWG;
-    if (t >= tiles[0]) return;
-    const u32 expert = tiles[1 + 3 * t], first = tiles[2 + 3 * t];
-    u32 cols = tiles[3 + 3 * t];
-    if (expert >= HB_E || first >= pairs) return;
-    cols = cols < MV ? cols : MV;
-    cols = cols < pairs - first ? cols : pairs - first;
-    if (cols == 0) return;
-    W += expert * BLOB;
-    const u32 p = first + (col < cols ? col : cols - 1);
-    u64 xrow = p;
-    if (ROWS == 1) {
-        xrow = list[p] / TOPK;
-        xrow = xrow < m ? xrow : m - 1;
-    }
-    auto yrow = [&](u32 c) -> u64 {
-        if (ROWS == 1) return first + c;
-        const u32 r = list[first + c];
-        return r < pairs ? r : pairs - 1;
-    };
-#endif
-    const u16* xp = x + xrow * K;
-    const u16* scales = (const u16*)(W + (u64)TILES * 1024);
+    const u16* xp = x + xrow(col % C < cols ? col % C : cols - 1) * K;
+    const u16* scales = (const u16*)(W + CODES);
     const u32 blk = wg * GPW + gi;
-    // The wave's W tiles; past the last they repeat it and are never stored.
-    u32 tn[RT];
-#pragma unroll
-    for (u32 r = 0; r < RT; r++) {
+    // Tile r of the wave; past the last they repeat it and are never stored.
+    auto tile = [&](u32 r) HB_INLINE2 -> u32 {
         const u32 o = blk * OT + r % OT;
-        tn[r] = ((o < ONT ? o : ONT - 1) + (r / OT) * ONT) * KT;
+        return (o < ONT ? o : ONT - 1) + (r / OT) * ONT;
+    };
+    u32 tn[RT];
+    const scales_t* sn[SETS];
+#pragma unroll
+    for (u32 r = 0; r < RT; r++) tn[r] = tile(r) * KT;
+#pragma unroll
+    for (u32 g = 0; g < SETS; g++) {
+        const u32 t = tile(g * TG + mine);
+        sn[g] = (const scales_t*)scales + (u64)(t / 4) * KT * 64 + (t % 4) * 16 + col;
     }
     const u32 kt0 = sp * KT / SPLIT, kt1 = (sp + 1) * KT / SPLIT;
     const bf16x8 b24 = __builtin_bit_cast(bf16x8, u32x4{0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u});
     u32 mask = 0x00780078u, one = 0x41804180u;
     asm("" : "+v"(mask), "+v"(one));
-    float acc[RT][AR];
+    float acc[SETS][AR];
 #pragma unroll
-    for (u32 r = 0; r < RT; r++)
+    for (u32 g = 0; g < SETS; g++)
 #pragma unroll
-        for (u32 i = 0; i < AR; i++) acc[r][i] = 0.0f;
+        for (u32 i = 0; i < AR; i++) acc[g][i] = 0.0f;
 
-    for (u32 kt = kt0; kt < kt1; kt += U) {
+    // U tiles of K in flight as registers (tiles past kt1 repeat the last).
+    struct Stage {
         u32x4 w[U][RT], xf[U][4];
-        scales_t s[U][RT];
+        scales_t s[U][SETS];
+    };
+    auto load = [&](Stage& t, u32 kt) HB_INLINE2 {
 #pragma unroll
         for (u32 u = 0; u < U; u++) {
-            const u32 q = kt + u < kt1 ? kt + u : kt1 - 1;
+            const u32 q = WHOLE && HB_STAGES == 1 ? kt + u : kt + u < kt1 ? kt + u : kt1 - 1;
 #pragma unroll
             for (u32 r = 0; r < RT; r++)
-                w[u][r] = __builtin_nontemporal_load((const u32x4*)(W + (u64)(tn[r] + q) * 1024) + lane);
+                t.w[u][r] = __builtin_nontemporal_load((const u32x4*)(W + (u64)(tn[r] + q) * 1024) + lane);
 #pragma unroll
-            for (u32 r = 0; r < RT; r++) s[u][r] = ((const scales_t*)(scales + (u64)(tn[r] + q) * 16 * GPT))[col];
+            for (u32 g = 0; g < SETS; g++) t.s[u][g] = sn[g][(u64)q * 64];
 #pragma unroll
             for (u32 j = 0; j < 4; j++) {
                 const u32 k = q * 128 + 32 * j + 8 * quad;
-                xf[u][j] = u32x4{0, 0, 0, 0};
-                if (K % 128 == 0 || k < K) xf[u][j] = *(const chunk_t*)(xp + k);
+                t.xf[u][j] = u32x4{0, 0, 0, 0};
+                if (K % 128 == 0 || k < K) t.xf[u][j] = *(const chunk_t*)(xp + k);
             }
         }
+    };
+    auto add = [&](const Stage& t, u32 kt) HB_INLINE2 {
 #pragma unroll
         for (u32 u = 0; u < U; u++) {
-            if (kt + u >= kt1) break;
+            if (!WHOLE && kt + u >= kt1) break;
 #pragma unroll
             for (u32 g = 0; g < GPT; g++) {
                 f32x4 base = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (u32 j = g * SPG; j < (g + 1) * SPG; j++) base = mfma(xf[u][j], b24, base);
+                for (u32 j = g * SPG; j < (g + 1) * SPG; j++) base = mfma(t.xf[u][j], b24, base);
 #pragma unroll
-                for (u32 r = 0; r < RT; r++) {
-                    f32x4 c = base;
+                for (u32 e = 0; e < SETS; e++) {
+                    f32x4 c[TG];
 #pragma unroll
-                    for (u32 j = g * SPG; j < (g + 1) * SPG; j++) c = mfma(xf[u][j], codes(w[u][r][j], mask, one), c);
-                    const float sc = scale_of(s[u][r], g);
+                    for (u32 r = 0; r < TG; r++) {
+                        c[r] = base;
 #pragma unroll
-                    for (u32 i = 0; i < AR; i++) acc[r][i] = __builtin_fmaf(sc, c[i], acc[r][i]);
+                        for (u32 j = g * SPG; j < (g + 1) * SPG; j++)
+                            c[r] = mfma(t.xf[u][j], codes(t.w[u][e * TG + r][j], mask, one), c[r]);
+                    }
+                    const float sc = scale_of(t.s[u][e], g);
+#pragma unroll
+                    for (u32 i = 0; i < AR; i++) {
+                        float v = c[0][i];
+#pragma unroll
+                        for (u32 r = 1; r < TG; r++) v = mine == r ? c[r][i] : v;
+                        acc[e][i] = __builtin_fmaf(sc, v, acc[e][i]);
+                    }
                 }
             }
         }
+    };
+    if constexpr (HB_STAGES == 1) {
+        for (u32 kt = kt0; kt < kt1; kt += U) {
+            Stage a;
+            load(a, kt);
+            add(a, kt);
+        }
+    } else {
+        Stage a, b;
+        load(a, kt0);
+        for (u32 kt = kt0; kt < kt1; kt += 2 * U) {
+            load(b, kt + U);
+            __builtin_amdgcn_sched_barrier(0);
+            add(a, kt);
+            __builtin_amdgcn_sched_barrier(0);
+            load(a, kt + 2 * U);
+            __builtin_amdgcn_sched_barrier(0);
+            add(b, kt + U);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 
-    // Lane (quad, col) holds row col of each W tile for x rows 4 quad .. +3.
-    auto put = [&](u32 r, u32 c, u32 nr, float v, float up) {
+    // A lane holds W row `col` of tile `mine` of each set for x rows row0 ..
+    auto put = [&](u32 r, u32 c, u32 nr, float v, float up) HB_INLINE2 {
         const u32 o = blk * OT + r, n = o * 16 + nr;
         if (o >= ONT || c >= cols || n >= NOUT) return;
         if (SWI) {
@@ -189,29 +211,70 @@ extern "C" __global__ __launch_bounds__(64 * WAVES) HB_VGPR_FORM void HB_NAME(
         }
         store(yv, yrow(c), n, v);
     };
-    if constexpr (SPLIT == 1) {
+    if constexpr (SPLIT == 1 && !SWI) {
 #pragma unroll
-        for (u32 r = 0; r < OT; r++)
+        for (u32 g = 0; g < SETS; g++)
 #pragma unroll
-            for (u32 i = 0; i < AR; i++) put(r, 4 * quad + i, col, acc[r][i], acc[SWI ? r + OT : r][i]);
+            for (u32 i = 0; i < AR; i++) put(g * TG + mine, row0 + i, col, acc[g][i], 0.0f);
     } else {
-        // A split's parts meet in LDS and are added in wave order.
-        __shared__ float part[WAVES][RT][MV * 16];
+        // A split's parts, and the gate and up rows, meet in LDS; the parts
+        // are added in wave order.  part[wave][tile][x row][W row].
+        auto at = [&](u32 w, u32 r, u32 c) HB_INLINE2 -> float& { return part[(w * RT + r) * M * 16 + c]; };
 #pragma unroll
-        for (u32 r = 0; r < RT; r++)
+        for (u32 g = 0; g < SETS; g++)
 #pragma unroll
             for (u32 i = 0; i < AR; i++)
-                if (4 * quad + i < MV) part[wave][r][(4 * quad + i) * 16 + col] = acc[r][i];
+                if (row0 + i < M) at(wave, g * TG + mine, (row0 + i) * 16 + col) = acc[g][i];
         __syncthreads();
-        for (u32 it = sp * 64 + lane; it < OT * MV * 16; it += SPLIT * 64) {
-            const u32 r = it / (MV * 16), c = it % (MV * 16);
-            float v = part[gi * SPLIT][r][c], up = part[gi * SPLIT][SWI ? r + OT : r][c];
+        const u32 need = cols * 16;
+        for (u32 it = sp * 64 + lane; it < OT * need; it += SPLIT * 64) {
+            const u32 r = it / need, c = it % need;
+            float v = at(gi * SPLIT, r, c), up = SWI ? at(gi * SPLIT, r + OT, c) : 0.0f;
 #pragma unroll
             for (u32 q = 1; q < SPLIT; q++) {
-                v += part[gi * SPLIT + q][r][c];
-                if (SWI) up += part[gi * SPLIT + q][r + OT][c];
+                v += at(gi * SPLIT + q, r, c);
+                if (SWI) up += at(gi * SPLIT + q, r + OT, c);
             }
             put(r, c / 16, c % 16, v, up);
         }
     }
 }
+
+#if HB_ROWS == 0
+extern "C" __global__ __launch_bounds__(64 * WAVES) HB_VGPR_FORM void HB_NAME(const unsigned char* __restrict__ W,
+                                                                                const u16* __restrict__ x, void* yv,
+                                                                                u32 rows) {
+    __shared__ float part[SPLIT > 1 || SWI ? WAVES * RT * MV * 16 : 1];
+    rows_of_w<MV>(W, x, yv, part, blockIdx.x, rows < MV ? rows : MV, [](u32 c) -> u64 { return c; },
+                  [](u32 c) -> u64 { return c; });
+}
+#else
+extern "C" __global__ __launch_bounds__(64 * WAVES) HB_VGPR_FORM void HB_NAME(
+    const u32* __restrict__ state, const unsigned char* __restrict__ W, const u16* __restrict__ x, void* yv,
+    const u32* __restrict__ list, const u32* __restrict__ tiles, u32 m_launch) {
+    __shared__ float part[SPLIT > 1 || SWI ? WAVES * RT * MV * 16 : 1];
+    const u32 m = rows_of_state(state, m_launch), pairs = m * TOPK, t = blockIdx.x / NWG;
+    if (t >= tiles[0]) return;
+    const u32 expert = tiles[1 + 3 * t], first = tiles[2 + 3 * t];
+    u32 cols = tiles[3 + 3 * t];
+    if (expert >= HB_E || first >= pairs) return;
+    cols = cols < MV ? cols : MV;
+    cols = cols < pairs - first ? cols : pairs - first;
+    if (cols == 0) return;
+    auto xrow = [&](u32 c) -> u64 {
+        if (ROWS != 1) return first + c;
+        const u32 r = list[first + c] / TOPK;
+        return r < m ? r : m - 1;
+    };
+    auto yrow = [&](u32 c) -> u64 {
+        if (ROWS == 1) return first + c;
+        const u32 r = list[first + c];
+        return r < pairs ? r : pairs - 1;
+    };
+    // Most tiles of a decode batch have few rows.
+    if (cols <= 4)
+        rows_of_w<4>(W + expert * BLOB, x, yv, part, blockIdx.x % NWG, cols, xrow, yrow);
+    else
+        rows_of_w<MV>(W + expert * BLOB, x, yv, part, blockIdx.x % NWG, cols, xrow, yrow);
+}
+#endif

@@ -9,8 +9,9 @@
 // step's operand.  In a word, element e stands at bits 4 (e / 2) (+ 16 for odd
 // e), all rotated left by 3, so that a rotation by 4 i and a mask leave
 // elements 2 i and 2 i + 1 in the top mantissa bits of two bf16.  After the
-// last tile's codes the scales, per tile [row][group].  Rows past
-// N and elements past K hold the code 8, their scales 0.
+// last tile's codes the scales, for each four row tiles and 128 K
+// [row 0..63][group].  Rows past N and elements past K hold the code 8, their
+// scales 0.
 //
 // All three are bound by the bf16 side's bytes.  A wave handles a tile: 16
 // bytes of bf16 a lane in four passes of 4 rows x 256 bytes.
@@ -20,7 +21,7 @@ constexpr u32 K = HB_K, N = HB_N, GROUP = HB_GROUP;
 constexpr u32 KT = (K + 127) / 128, NT = (N + 15) / 16, TILES = KT * NT;
 constexpr u32 GPT = 128 / GROUP;        // groups of a tile
 constexpr u32 GROUPS = (K + GROUP - 1) / GROUP;  // of a row
-constexpr u64 BLOB = (u64)TILES * (1024 + 32 * GPT);  // bytes of a matrix
+constexpr u64 CODES = (u64)TILES * 1024, BLOB = CODES + (u64)((NT + 3) / 4) * KT * 128 * GPT;  // bytes of a matrix
 static_assert(K % 8 == 0, "K a multiple of 8");
 static_assert(GROUP == 32 || GROUP == 64 || GROUP == 128, "groups of 32, 64 or 128");
 
@@ -29,8 +30,8 @@ typedef u32x4 chunk_t __attribute__((aligned(2)));
 
 // Word of chunk ch (8 elements) of row `row` within a tile's 256 words.
 HB_DEV u32 word_at(u32 row, u32 ch) { return ((ch & 3u) * 16 + row) * 4 + (ch >> 2); }
-// Scale of group g of row `row` within a tile's 16 * GPT scales.
-HB_DEV u32 scale_at(u32 row, u32 g) { return row * GPT + g; }
+// Scale of group g of row n in the K tile kt.
+HB_DEV u64 scale_at(u32 n, u32 kt, u32 g) { return ((u64)(n / 64 * KT + kt) * 64 + n % 64) * GPT + g; }
 HB_DEV u32 rotl(u32 v, u32 s) { return __builtin_amdgcn_alignbit(v, v, 32 - s); }
 
 #if HB_OP == 1 || HB_OP == 2
@@ -46,7 +47,7 @@ extern "C" __global__ __launch_bounds__(256) void HB_NAME(const u16* __restrict_
     const u64 mat = live ? id / TILES : 0;
     const u32 tile = live ? (u32)(id % TILES) : 0, nt = tile / KT, kt = tile % KT;
     unsigned char* blob = dst + mat * BLOB;
-    u16* sc = (u16*)(blob + (u64)TILES * 1024) + (u64)tile * 16 * GPT;
+    u16* sc = (u16*)(blob + CODES);
     const u32 ch = lane & 15u, k = kt * 128 + ch * 8;
 #pragma unroll
     for (u32 i = 0; i < 4; i++) {
@@ -86,7 +87,7 @@ extern "C" __global__ __launch_bounds__(256) void HB_NAME(const u16* __restrict_
                 nw |= (u32)(int)(q + 8.0f) << (4 * (e / 2) + 16 * (e & 1));
             }
         }
-        if (live && ch % (GROUP / 8) == 0) sc[scale_at(row, ch / (GROUP / 8))] = n < N && k < K ? (u16)sb : 0;
+        if (live && ch % (GROUP / 8) == 0) sc[scale_at(n, kt, ch / (GROUP / 8))] = n < N && k < K ? (u16)sb : 0;
 #else
         // Row order: byte b of a row holds element 2 b in its low half.
         if (in) {
@@ -97,10 +98,13 @@ extern "C" __global__ __launch_bounds__(256) void HB_NAME(const u16* __restrict_
             for (u32 e = 0; e < 8; e++) nw |= (b >> (4 * e) & 15u) << (4 * (e / 2) + 16 * (e & 1));
         }
         if (live && ch % (GROUP / 8) == 0)
-            sc[scale_at(row, ch / (GROUP / 8))] = n < N && k < K ? scales[(mat * N + n) * GROUPS + k / GROUP] : 0;
+            sc[scale_at(n, kt, ch / (GROUP / 8))] = n < N && k < K ? scales[(mat * N + n) * GROUPS + k / GROUP] : 0;
 #endif
         words[wave][word_at(row, ch)] = rotl(nw, 3);
     }
+    // The scales of the rows that a last group of four tiles lacks.
+    if (live && nt == NT - 1 && NT % 4 != 0)
+        for (u32 i = lane; i < (4 - NT % 4) * 16 * GPT; i += 64) sc[scale_at(NT * 16, kt, 0) + i] = 0;
     __syncthreads();
     if (live) ((u32x4*)(blob + (u64)tile * 1024))[lane] = ((u32x4*)words[wave])[lane];
 }
@@ -115,14 +119,14 @@ extern "C" __global__ __launch_bounds__(256) void HB_NAME(const unsigned char* _
     const u32 tile = (u32)(id % TILES), nt = tile / KT, kt = tile % KT;
     const unsigned char* blob = src + mat * BLOB;
     const u32* words = (const u32*)(blob + (u64)tile * 1024);
-    const u16* sc = (const u16*)(blob + (u64)TILES * 1024) + (u64)tile * 16 * GPT;
+    const u16* sc = (const u16*)(blob + CODES);
     const u32 ch = lane & 15u, k = kt * 128 + ch * 8;
 #pragma unroll
     for (u32 i = 0; i < 4; i++) {
         const u32 row = 4 * i + (lane >> 4), n = nt * 16 + row;
         if (n >= N || k >= K) continue;
         const u32 nw = rotl(words[word_at(row, ch)], 29);
-        const float s = bf16_to_f32(sc[scale_at(row, ch / (GROUP / 8))]);
+        const float s = bf16_to_f32(sc[scale_at(n, kt, ch / (GROUP / 8))]);
         u32x4 o;
 #pragma unroll
         for (u32 e = 0; e < 4; e++)

@@ -25,8 +25,8 @@ def gpu(hb):
 
 
 def test_q4_bytes(hb):
-    assert hb.q4_bytes(128, 16, 32) == 1024 + 128
-    assert hb.q4_bytes(136, 17, 64) == 4 * (1024 + 64)
+    assert hb.q4_bytes(128, 16, 32) == 1024 + 512
+    assert hb.q4_bytes(136, 17, 64) == 4 * 1024 + 2 * 256
     assert hb.q4_bytes(2560, 151936, 128) == 20 * 9496 * (1024 + 32)
     for k, n, g in [(0, 1, 32), (8, 0, 32), (12, 1, 32), (8, 1, 16), (8, 1, 0), (8, 1, 256)]:
         with pytest.raises(hb.HerbertError):
@@ -71,7 +71,7 @@ def test_refused_matvec_launches(hb, gpu):
     gpu.launch(k, [R(w), R(x), R(y)], 2)
     gpu.launch(k, [R(w), R(x, 2), R(y, 4)], 2)
     for ranges, m, match in [([R(w), R(x), R(y)], 0, "0 rows"), ([R(w), R(x), R(y)], 3, "rows: 1..2"),
-                             ([R(w, 0, 1151), R(x), R(y)], 1, "q4"), ([R(w), R(x, 0, 511), R(y)], 2, "binding 1"),
+                             ([R(w, 0, 2559), R(x), R(y)], 1, "q4"), ([R(w), R(x, 0, 511), R(y)], 2, "binding 1"),
                              ([R(w), R(x), R(y, 0, 255)], 2, "binding 2"), ([R(w), R(x, 1), R(y)], 1, "multiple of 2"),
                              ([R(w), R(x), R(y, 2)], 1, "multiple of 4"), ([R(y), R(x), R(w, 8)], 1, "binding"),
                              ([R(w), R(x), R(x, 4)], 1, "overlap"), ([R(w), R(x), R(w, 1024)], 1, "overlap"),
