@@ -58,13 +58,13 @@ CHECKS = {
     "q4.hip": ["-DHB_OP=%d -DHB_K=2568 -DHB_N=1000 -DHB_GROUP=%d" % (op, g) for op, g in ((1, 32), (1, 128), (2, 64), (3, 32))],
     "matvec_q4.hip": [
         "-DHB_K=2560 -DHB_N=151936 -DHB_GROUP=32 -DHB_OUT=1 -DHB_MV_M=4 -DHB_RT=2 -DHB_SPLIT=2 -DHB_WAVES=4 -DHB_UNROLL=2 "
-        "-DHB_STAGES=2 -DHB_ROWS=0 -DHB_TOPK=1 -DHB_E=1",
+        "-DHB_ROWS=0 -DHB_TOPK=1 -DHB_E=1",
         "-DHB_K=5000 -DHB_N=7001 -DHB_GROUP=128 -DHB_OUT=2 -DHB_MV_M=3 -DHB_RT=1 -DHB_SPLIT=1 -DHB_WAVES=4 -DHB_UNROLL=1 "
-        "-DHB_STAGES=2 -DHB_ROWS=0 -DHB_TOPK=1 -DHB_E=1",
+        "-DHB_ROWS=0 -DHB_TOPK=1 -DHB_E=1",
         "-DHB_K=2048 -DHB_N=1024 -DHB_GROUP=64 -DHB_OUT=3 -DHB_MV_M=16 -DHB_RT=2 -DHB_SPLIT=4 -DHB_WAVES=8 -DHB_UNROLL=2 "
-        "-DHB_STAGES=2 -DHB_ROWS=1 -DHB_TOPK=8 -DHB_E=256",
+        "-DHB_ROWS=1 -DHB_TOPK=8 -DHB_E=256",
         "-DHB_K=512 -DHB_N=2048 -DHB_GROUP=32 -DHB_OUT=0 -DHB_MV_M=16 -DHB_RT=1 -DHB_SPLIT=1 -DHB_WAVES=4 -DHB_UNROLL=4 "
-        "-DHB_STAGES=2 -DHB_ROWS=2 -DHB_TOPK=8 -DHB_E=256",
+        "-DHB_ROWS=2 -DHB_TOPK=8 -DHB_E=256",
     ],
     "block_norm.hip": [
         "-DHB_D=2560 -DHB_THREADS=320 -DHB_EPS=0x358637bd -DHB_PLUS1=1 -DHB_POST=1 -DHB_PRE=1 -DHB_SCALES=1 -DHB_GATE=1",

@@ -47,12 +47,25 @@ static bool q4_shape(uint32_t k, uint32_t n, uint32_t group) {
     return k && n && k % 8 == 0 && (group == 32 || group == 64 || group == 128) && q4_tiles(k, n) < (1u << 30);
 }
 
+// The 4-bit matvec's form by its row tiles (16 W rows) and K tiles (128 K).
+// A workgroup's waves share a row block's K, so that its loads are in flight
+// at once.  16 rows a wave while every row tile finds a CU of its own (4096 to
+// 2560 at 1 row: 3.5 us, 32 rows 4.9), 32 up to 4096 tiles (2560 to 18432 with
+// the SwiGLU: 7.4 us, 64 rows 8.1), then 64, whose x and scales serve four
+// tiles a load (2560 to 151936 at 4 rows: 36.8 us, 32 rows 41); past 8 x rows
+// 128 (39.9 at 16 rows, 64 rows 42.9).
 static void q4_defaults(hb_desc* d) {
     if (!d->mv_m) d->mv_m = d->rows_of == HB_ROWS_DENSE ? 1 : 16;
-    if (!d->rows) d->rows = d->out == HB_OUT_SWIGLU ? 32 : 16;
-    if (!d->mv_waves) d->mv_waves = 4;
-    if (!d->split) d->split = 4;
-    if (!d->unroll) d->unroll = 2;
+    const uint32_t nt = cdiv(d->n, 16), kt = cdiv(d->k, 128);
+    const bool swi = d->out == HB_OUT_SWIGLU;
+    if (!d->rows) d->rows = nt > 4096 ? (d->mv_m > 8 ? 128 : 64) : nt > 256 || swi ? 32 : 16;
+    if (!d->split) {
+        d->split = d->rows == 16 ? 16 : 8;
+        while (d->split > kt || (d->mv_waves && d->split > d->mv_waves)) d->split /= 2;
+        if (!d->split) d->split = 1;
+    }
+    if (!d->mv_waves) d->mv_waves = d->split < 4 ? 4 : d->split;
+    if (!d->unroll) d->unroll = d->rows == 16 ? 2 : 1;
 }
 
 hb_desc with_defaults(const hb_desc& in) {
@@ -399,10 +412,8 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             if (d.mv_m > 16) return fail(HB_ERR_UNSUPPORTED, "matvec_q4: m <= 16");
             if ((d.rows != 16 && d.rows != 32 && d.rows != 64 && d.rows != 128) || (swi && d.rows == 16))
                 return fail(HB_ERR_UNSUPPORTED, "matvec_q4: 16, 32, 64 or 128 rows a wave (Out::Swiglu not 16)");
-            if (d.mv_waves > 16 || !pow2(d.mv_waves) || !pow2(d.split) || d.split > d.mv_waves || d.unroll > 4 ||
-                d.dbuf > 1)
-                return fail(HB_ERR_UNSUPPORTED,
-                            "matvec_q4: 1, 2, 4, 8 or 16 waves, split no more, unroll 1..4, dbuf 0 or 1");
+            if (d.mv_waves > 16 || !pow2(d.mv_waves) || !pow2(d.split) || d.split > d.mv_waves || d.unroll > 4)
+                return fail(HB_ERR_UNSUPPORTED, "matvec_q4: 1, 2, 4, 8 or 16 waves, split no more, unroll 1..4");
             if (experts && (!d.top_k || !d.experts || !d.tiles || !d.rows_max || d.mv_m != 16 ||
                             (d.out != HB_OUT_BF16 && !swi)))
                 return fail(HB_ERR_INVALID,
@@ -413,9 +424,9 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
                          d.top_k, d.experts, d.tiles, d.rows_max);
                 rows = name;
             }
-            snprintf(name, sizeof name, "matvec_q4_%ux%u_g%u%s_r%u_k%u_w%u_u%u_d%u_m%u%s", d.k, d.n, d.bk,
+            snprintf(name, sizeof name, "matvec_q4_%ux%u_g%u%s_r%u_k%u_w%u_u%u_m%u%s", d.k, d.n, d.bk,
                      d.out == HB_OUT_F32 ? "_f32" : d.out == HB_OUT_RESIDUAL ? "_res" : swi ? "_sw" : "", d.rows,
-                     d.split, d.mv_waves, d.unroll, d.dbuf, d.mv_m, rows.c_str());
+                     d.split, d.mv_waves, d.unroll, d.mv_m, rows.c_str());
             e->name = name;
             e->source = "matvec_q4.hip";
             e->threads = 64 * d.mv_waves;
@@ -423,7 +434,6 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             e->defines = {D("HB_K", d.k),          D("HB_N", d.n),         D("HB_GROUP", d.bk),
                           D("HB_OUT", d.out),      D("HB_MV_M", d.mv_m),   D("HB_RT", d.rows / 16),
                           D("HB_SPLIT", d.split),  D("HB_WAVES", d.mv_waves), D("HB_UNROLL", d.unroll),
-                          D("HB_STAGES", d.dbuf + 1),
                           D("HB_ROWS", d.rows_of), D("HB_TOPK", experts ? d.top_k : 1),
                           D("HB_E", experts ? d.experts : 1)};
             return HB_OK;

@@ -1242,6 +1242,21 @@ static std::vector<hb_desc> mv_q4_candidates(uint32_t k, uint32_t n, uint32_t ou
     d.bk = group;
     d.mv_m = mv_m;
     std::vector<hb_desc> v = {with_defaults(d)};
+    // Row blocks that leave no CU without one (or the least there are), each
+    // with its waves sharing K four, eight or sixteen ways.
+    const uint32_t nt = (n + 15) / 16, kt = (k + 127) / 128;
+    for (uint32_t rows : {16u, 32u, 64u, 128u})
+        for (uint32_t split : {4u, 8u, 16u})
+            for (uint32_t unroll : {1u, 2u}) {
+                if ((rows == 16 && out == HB_OUT_SWIGLU) || split > kt || rows * unroll > 128 || rows * split > 1024) continue;
+                if (rows > (out == HB_OUT_SWIGLU ? 32u : 16u) && nt * 16 / rows < 128) continue;
+                hb_desc c = v[0];
+                c.rows = rows;
+                c.split = split;
+                c.mv_waves = split;
+                c.unroll = unroll;
+                if (memcmp(&c, &v[0], sizeof c)) v.push_back(c);
+            }
     return v;
 }
 

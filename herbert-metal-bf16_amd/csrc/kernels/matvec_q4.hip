@@ -26,8 +26,8 @@ constexpr u32 OT = SWI ? RT / 2 : RT;                    // output tiles of a wa
 constexpr u32 ONT = SWI ? NT / 2 : NT;                   // output tiles
 constexpr u32 NBLK = (ONT + OT - 1) / OT, GPW = WAVES / SPLIT;
 constexpr u32 NWG = (NBLK + GPW - 1) / GPW;
-// Every wave's tiles of K fill its stages.
-constexpr bool WHOLE = KT % (SPLIT * U * HB_STAGES) == 0;
+// Every wave's tiles of K are whole rounds of U.
+constexpr bool WHOLE = KT % (SPLIT * U) == 0;
 static_assert(K % 8 == 0 && (!SWI || (RT % 2 == 0 && N % 32 == 0)), "shape");
 static_assert(WAVES % SPLIT == 0 && MV >= 1 && MV <= 16, "waves");
 
@@ -80,6 +80,13 @@ HB_DEV void store(void* yv, u64 row, u32 n, float v) {
     }
 }
 
+// LDS bytes of a wave: its x tile, then its parts of the sums (rows_of_w).
+template <u32 M>
+struct Lds {
+    static constexpr u32 REP = M <= 4 ? 4 : M <= 8 ? 2 : 1, TG = RT < REP ? RT : REP, C = 16 / TG;
+    static constexpr u32 X = C * 256, P = SPLIT > 1 || SWI ? RT * M * 64 : 0, BYTES = X > P ? X : P;
+};
+
 // Workgroup `wg` of a matrix: `cols` <= M columns, column c from x row
 // xrow(c) into y row yrow(c).
 //
@@ -88,18 +95,29 @@ HB_DEV void store(void* yv, u64 row, u32 n, float v) {
 // one of TG tiles: a set of TG tiles takes one load of scales and one
 // register of sums for each of a lane's x rows.
 template <u32 M, typename XRow, typename YRow>
-HB_DEV void rows_of_w(const unsigned char* __restrict__ W, const u16* __restrict__ x, void* yv, float* part, u32 wg,
+HB_DEV void rows_of_w(const unsigned char* __restrict__ W, const u16* __restrict__ x, void* yv, unsigned char* lds, u32 wg,
                       u32 cols, XRow xrow, YRow yrow) {
-    constexpr u32 REP = M <= 4 ? 4 : M <= 8 ? 2 : 1, TG = RT < REP ? RT : REP, SETS = RT / TG;
-    constexpr u32 C = 16 / TG, AR = M < 4 ? M : 4;
+    constexpr u32 TG = Lds<M>::TG, SETS = RT / TG, C = Lds<M>::C, AR = M < 4 ? M : 4;
+    constexpr u32 XI = ((M < C ? M : C) + 3) / 4;  // loads of four x rows
     static_assert(RT % TG == 0 && M <= C, "tiles in whole sets");
     const u32 tid = threadIdx.x, lane = tid & 63u, col = lane & 15u, quad = lane >> 4;
     const u32 wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const u32 sp = wave % SPLIT, gi = wave / SPLIT;
     const u32 mine = quad * TG / 4;     // the lane's tile of a set
     const u32 row0 = (4 * quad) % C;    // its x rows: row0 .. + AR - 1
+    // x comes in whole 256-byte lines of a row, four rows a load, and turns
+    // into the MFMA's operand through a tile of the wave's own in LDS, its
+    // 16-byte chunks at chunk ^ row, so that reads of one chunk of 16 rows
+    // meet no bank twice.  (Loaded as the operand, 64 bytes of 16 rows at a
+    // time, x took most of the time at 16 rows: 17408 to 5120 21 us.)
     // Columns past the rows repeat the last one and are never stored.
-    const u16* xp = x + xrow(col % C < cols ? col % C : cols - 1) * K;
+    u32x4* const xt = (u32x4*)(lds + wave * Lds<M>::BYTES);
+    const u16* xp[XI];
+#pragma unroll
+    for (u32 i = 0; i < XI; i++) {
+        const u32 c = 4 * i + quad;
+        xp[i] = x + xrow(c < cols ? c : cols - 1) * K;
+    }
     const u16* scales = (const u16*)(W + CODES);
     const u32 blk = wg * GPW + gi;
     // Tile r of the wave; past the last they repeat it and are never stored.
@@ -126,37 +144,54 @@ HB_DEV void rows_of_w(const unsigned char* __restrict__ W, const u16* __restrict
 #pragma unroll
         for (u32 i = 0; i < AR; i++) acc[g][i] = 0.0f;
 
-    // U tiles of K in flight as registers (tiles past kt1 repeat the last).
+    // U tiles of K in flight as registers; past kt1 the last one's codes again
+    // with zeros for x and the scales.
+    auto inside = [&](u32 kt, u32 u) HB_INLINE2 { return WHOLE || u == 0 || kt + u < kt1; };
     struct Stage {
-        u32x4 w[U][RT], xf[U][4];
+        u32x4 w[U][RT], x[U][XI];
         scales_t s[U][SETS];
     };
     auto load = [&](Stage& t, u32 kt) HB_INLINE2 {
 #pragma unroll
         for (u32 u = 0; u < U; u++) {
-            const u32 q = WHOLE && HB_STAGES == 1 ? kt + u : kt + u < kt1 ? kt + u : kt1 - 1;
+            const u32 q = inside(kt, u) ? kt + u : kt1 - 1;
 #pragma unroll
             for (u32 r = 0; r < RT; r++)
                 t.w[u][r] = __builtin_nontemporal_load((const u32x4*)(W + (u64)(tn[r] + q) * 1024) + lane);
 #pragma unroll
             for (u32 g = 0; g < SETS; g++) t.s[u][g] = sn[g][(u64)q * 64];
 #pragma unroll
-            for (u32 j = 0; j < 4; j++) {
-                const u32 k = q * 128 + 32 * j + 8 * quad;
-                t.xf[u][j] = u32x4{0, 0, 0, 0};
-                if (K % 128 == 0 || k < K) t.xf[u][j] = *(const chunk_t*)(xp + k);
+            for (u32 i = 0; i < XI; i++) {
+                const u32 k = q * 128 + 8 * col;
+                t.x[u][i] = *(const chunk_t*)(xp[i] + (K % 128 == 0 || k < K ? k : 0));
             }
         }
     };
     auto add = [&](const Stage& t, u32 kt) HB_INLINE2 {
 #pragma unroll
         for (u32 u = 0; u < U; u++) {
-            if (!WHOLE && kt + u >= kt1) break;
+            // The wave's own tile: its LDS accesses run in program order.
+            const bool in = inside(kt, u), in_k = in && (K % 128 == 0 || (kt + u) * 128 + 8 * col < K);
+            u32x4 xf[4];
+#pragma unroll
+            for (u32 i = 0; i < XI; i++) {
+                const u32 c = 4 * i + quad;
+                if (C >= 4 || quad < C) xt[c * 16 + (col ^ c)] = in_k ? t.x[u][i] : u32x4{0, 0, 0, 0};
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (u32 j = 0; j < 4; j++) {
+                const u32 c = col % C < 4 * XI ? col % C : 0;
+                xf[j] = xt[c * 16 + ((4 * j + quad) ^ c)];
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (u32 g = 0; g < GPT; g++) {
                 f32x4 base = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (u32 j = g * SPG; j < (g + 1) * SPG; j++) base = mfma(t.xf[u][j], b24, base);
+                for (u32 j = g * SPG; j < (g + 1) * SPG; j++) base = mfma(xf[j], b24, base);
 #pragma unroll
                 for (u32 e = 0; e < SETS; e++) {
                     f32x4 c[TG];
@@ -165,9 +200,9 @@ HB_DEV void rows_of_w(const unsigned char* __restrict__ W, const u16* __restrict
                         c[r] = base;
 #pragma unroll
                         for (u32 j = g * SPG; j < (g + 1) * SPG; j++)
-                            c[r] = mfma(t.xf[u][j], codes(t.w[u][e * TG + r][j], mask, one), c[r]);
+                            c[r] = mfma(xf[j], codes(t.w[u][e * TG + r][j], mask, one), c[r]);
                     }
-                    const float sc = scale_of(t.s[u][e], g);
+                    const float sc = in ? scale_of(t.s[u][e], g) : 0.0f;
 #pragma unroll
                     for (u32 i = 0; i < AR; i++) {
                         float v = c[0][i];
@@ -179,25 +214,10 @@ HB_DEV void rows_of_w(const unsigned char* __restrict__ W, const u16* __restrict
             }
         }
     };
-    if constexpr (HB_STAGES == 1) {
-        for (u32 kt = kt0; kt < kt1; kt += U) {
-            Stage a;
-            load(a, kt);
-            add(a, kt);
-        }
-    } else {
-        Stage a, b;
-        load(a, kt0);
-        for (u32 kt = kt0; kt < kt1; kt += 2 * U) {
-            load(b, kt + U);
-            __builtin_amdgcn_sched_barrier(0);
-            add(a, kt);
-            __builtin_amdgcn_sched_barrier(0);
-            load(a, kt + 2 * U);
-            __builtin_amdgcn_sched_barrier(0);
-            add(b, kt + U);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+    for (u32 kt = kt0; kt < kt1; kt += U) {
+        Stage a;
+        load(a, kt);
+        add(a, kt);
     }
 
     // A lane holds W row `col` of tile `mine` of each set for x rows row0 ..
@@ -218,8 +238,8 @@ HB_DEV void rows_of_w(const unsigned char* __restrict__ W, const u16* __restrict
             for (u32 i = 0; i < AR; i++) put(g * TG + mine, row0 + i, col, acc[g][i], 0.0f);
     } else {
         // A split's parts, and the gate and up rows, meet in LDS; the parts
-        // are added in wave order.  part[wave][tile][x row][W row].
-        auto at = [&](u32 w, u32 r, u32 c) HB_INLINE2 -> float& { return part[(w * RT + r) * M * 16 + c]; };
+        // are added in wave order: [wave][tile][x row][W row].
+        auto at = [&](u32 w, u32 r, u32 c) HB_INLINE2 -> float& { return ((float*)(lds + w * Lds<M>::BYTES))[r * M * 16 + c]; };
 #pragma unroll
         for (u32 g = 0; g < SETS; g++)
 #pragma unroll
@@ -244,15 +264,16 @@ HB_DEV void rows_of_w(const unsigned char* __restrict__ W, const u16* __restrict
 extern "C" __global__ __launch_bounds__(64 * WAVES) HB_VGPR_FORM void HB_NAME(const unsigned char* __restrict__ W,
                                                                                 const u16* __restrict__ x, void* yv,
                                                                                 u32 rows) {
-    __shared__ float part[SPLIT > 1 || SWI ? WAVES * RT * MV * 16 : 1];
-    rows_of_w<MV>(W, x, yv, part, blockIdx.x, rows < MV ? rows : MV, [](u32 c) -> u64 { return c; },
+    __shared__ u32x4 lds[WAVES * Lds<MV>::BYTES / 16];
+    rows_of_w<MV>(W, x, yv, (unsigned char*)lds, blockIdx.x, rows < MV ? rows : MV, [](u32 c) -> u64 { return c; },
                   [](u32 c) -> u64 { return c; });
 }
 #else
 extern "C" __global__ __launch_bounds__(64 * WAVES) HB_VGPR_FORM void HB_NAME(
     const u32* __restrict__ state, const unsigned char* __restrict__ W, const u16* __restrict__ x, void* yv,
     const u32* __restrict__ list, const u32* __restrict__ tiles, u32 m_launch) {
-    __shared__ float part[SPLIT > 1 || SWI ? WAVES * RT * MV * 16 : 1];
+    constexpr u32 BYTES = Lds<4>::BYTES > Lds<MV>::BYTES ? Lds<4>::BYTES : Lds<MV>::BYTES;
+    __shared__ u32x4 lds[WAVES * BYTES / 16];
     const u32 m = rows_of_state(state, m_launch), pairs = m * TOPK, t = blockIdx.x / NWG;
     if (t >= tiles[0]) return;
     const u32 expert = tiles[1 + 3 * t], first = tiles[2 + 3 * t];
@@ -273,8 +294,8 @@ extern "C" __global__ __launch_bounds__(64 * WAVES) HB_VGPR_FORM void HB_NAME(
     };
     // Most tiles of a decode batch have few rows.
     if (cols <= 4)
-        rows_of_w<4>(W + expert * BLOB, x, yv, part, blockIdx.x % NWG, cols, xrow, yrow);
+        rows_of_w<4>(W + expert * BLOB, x, yv, (unsigned char*)lds, blockIdx.x % NWG, cols, xrow, yrow);
     else
-        rows_of_w<MV>(W + expert * BLOB, x, yv, part, blockIdx.x % NWG, cols, xrow, yrow);
+        rows_of_w<MV>(W + expert * BLOB, x, yv, (unsigned char*)lds, blockIdx.x % NWG, cols, xrow, yrow);
 }
 #endif

@@ -350,18 +350,18 @@ def q4_dequantize(kdim, n, group=32):
     return Desc(kind=Kind.Q4_DEQUANTIZE, k=kdim, n=n, bk=group)
 
 
-def matvec_q4(kdim, n, out, group=32, mv_m=1, rows=0, split=0, waves=0, unroll=0, dbuf=0):
+def matvec_q4(kdim, n, out, group=32, mv_m=1, rows=0, split=0, waves=0, unroll=0):
     """y[m][n] = x[m][kdim].W^T over a packed 4-bit matrix for m <= mv_m <= 16 (bindings q4, x, y);
     zeros: the shape's defaults.  out Residual adds with one rounding, Swiglu as matvec's."""
     return Desc(kind=Kind.MATVEC_Q4, k=kdim, n=n, out=out, bk=group, mv_m=mv_m, rows=rows, split=split,
-                mv_waves=waves, unroll=unroll, dbuf=dbuf)
+                mv_waves=waves, unroll=unroll)
 
 
-def experts_q4(kdim, n, out, group, rows_of, top_k, experts, rows_max, rows=0, split=0, waves=0, unroll=0, dbuf=0):
+def experts_q4(kdim, n, out, group, rows_of, top_k, experts, rows_max, rows=0, split=0, waves=0, unroll=0):
     """matvec_q4 over the routed experts of a block of up to rows_max rows, tiles of moe_sort with
     bm = 16 (bindings state, q4 of every expert, X, Y, list, tiles)."""
     return Desc(kind=Kind.MATVEC_Q4, k=kdim, n=n, out=out, bk=group, mv_m=16, rows=rows, split=split, mv_waves=waves,
-                unroll=unroll, dbuf=dbuf, rows_of=rows_of, top_k=top_k, experts=experts, rows_max=rows_max,
+                unroll=unroll, rows_of=rows_of, top_k=top_k, experts=experts, rows_max=rows_max,
                 tiles=moe_tiles(rows_max, top_k, experts, 16))
 
 
