@@ -58,6 +58,20 @@ static void q4_defaults(hb_desc* d) {
     if (!d->mv_m) d->mv_m = d->rows_of == HB_ROWS_DENSE ? 1 : 16;
     const uint32_t nt = cdiv(d->n, 16), kt = cdiv(d->k, 128);
     const bool swi = d->out == HB_OUT_SWIGLU;
+    if (d->rows_of != HB_ROWS_DENSE) {
+        // The experts: 64 rows a wave once the largest block's pairs make
+        // 8192 workgroups of 32 (64 tokens of 8 experts, 2048 to 1024: 43.6 us
+        // against 46), below that 32 with all of a wave's K in flight (8
+        // tokens 13.7 against 14.5, 1 token 3.8 against 4.8).
+        const uint64_t wgs = (uint64_t)d->rows_max * d->top_k * (swi ? nt / 2 : nt / 2 + nt % 2);
+        if (!d->rows) d->rows = wgs >= 8192 ? 64 : 32;
+        if (!d->split) d->split = kt >= 4 ? 4 : kt >= 2 ? 2 : 1;
+        if (d->mv_waves && d->split > d->mv_waves) d->split = d->mv_waves;
+        if (!d->mv_waves) d->mv_waves = 4;
+        const uint32_t per = cdiv(kt, d->split);
+        if (!d->unroll) d->unroll = d->rows >= 64 ? 1 : per >= 3 ? 4 : per;
+        return;
+    }
     if (!d->rows) d->rows = nt > 4096 ? (d->mv_m > 8 ? 128 : 64) : nt > 256 || swi ? 32 : 16;
     if (!d->split) {
         d->split = d->rows == 16 ? 16 : 8;
@@ -447,8 +461,10 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
                      post ? "_post" : "", pre ? "_pre" : "", scales ? "_sc" : "", gate);
             e->name = name;
             e->source = "block_norm.hip";
-            // A 16-byte chunk of the row a thread, up to 1024 threads.
-            e->threads = cells < 1024 ? cdiv(cells, 64) * 64 : 1024;
+            // A 16-byte chunk of the row a thread, two past 512 (2048 rows of
+            // 5120: 18.5 us, one each 19.9; 2560: one each 10.6, two 10.9),
+            // up to 1024 threads.
+            e->threads = cdiv(cells <= 512 ? cells : cells <= 2048 ? cdiv(cells, 2) : 1024, 64) * 64;
             e->nbind = 3 + (post ? 1 : 0) + (pre ? 2 : 0) + (scales ? 1 : 0) + (gate ? 1 : 0);
             e->defines = {D("HB_D", d.n),       D("HB_THREADS", e->threads), D("HB_EPS", d.eps_bits),
                           D("HB_PLUS1", d.plus_one ? 1 : 0), D("HB_POST", post), D("HB_PRE", pre),

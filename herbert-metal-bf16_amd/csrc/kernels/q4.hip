@@ -34,6 +34,47 @@ HB_DEV u32 word_at(u32 row, u32 ch) { return ((ch & 3u) * 16 + row) * 4 + (ch >>
 HB_DEV u64 scale_at(u32 n, u32 kt, u32 g) { return ((u64)(n / 64 * KT + kt) * 64 + n % 64) * GPT + g; }
 HB_DEV u32 rotl(u32 v, u32 s) { return __builtin_amdgcn_alignbit(v, v, 32 - s); }
 
+#if HB_OP == 1
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+HB_DEV u32 word(u32x4 v, u32 i) { return v[i]; }
+
+template <u32 ctrl>
+HB_DEV s16x2 lane_max(s16x2 v) {
+    const int b = __builtin_bit_cast(int, v);
+    return __builtin_elementwise_max(v, __builtin_bit_cast(s16x2, __builtin_amdgcn_update_dpp(b, b, ctrl, 0xf, 0xf, true)));
+}
+
+// The codes q + 8 of eight elements in their places, q = w / s to the nearest
+// whole number of -8..7, ties to even.
+HB_DEV u32 group_codes(u32x4 v, float s) {
+    u32 nw = 0;
+    if (!(__builtin_fabsf(s) > 0x1p-100f)) {
+        // A scale near the subnormals, or of zero, where all codes are 8.
+#pragma unroll 1
+        for (u32 e = 0; e < 8; e++) {
+            const u32 half = v[e / 2] >> (16 * (e & 1)) & 0xffffu;
+            const float q = s == 0.0f ? 0.0f : __builtin_rintf(__fdiv_rn(bf16_to_f32(half), s));
+            nw |= (u32)(int)(__builtin_amdgcn_fmed3f(q, -8.0f, 7.0f) + 8.0f) << (4 * (e / 2) + 16 * (e & 1));
+        }
+        return nw;
+    }
+    // The quotient to the last bit, by the reciprocal and one correction by
+    // the exact remainder (Markstein): ten instructions less than a division.
+    const float r = __fdiv_rn(1.0f, s);
+#pragma unroll
+    for (u32 e = 0; e < 8; e++) {
+        const float w = e & 1 ? bf16_hi(v[e / 2]) : bf16_lo(v[e / 2]);
+        float q = w * r;
+        q = __builtin_fmaf(__builtin_fmaf(-s, q, w), r, q);
+        // 2^23 + 8 added rounds to a whole number in the low bits, ties to
+        // even as 8 is even.
+        const float z = __builtin_amdgcn_fmed3f(q, -8.0f, 7.0f) + 8388616.0f;
+        nw |= (__builtin_bit_cast(u32, z) & 15u) << (4 * (e / 2) + 16 * (e & 1));
+    }
+    return nw;
+}
+#endif
+
 #if HB_OP == 1 || HB_OP == 2
 extern "C" __global__ __launch_bounds__(256) void HB_NAME(const u16* __restrict__ src,
 #if HB_OP == 2
@@ -49,44 +90,44 @@ extern "C" __global__ __launch_bounds__(256) void HB_NAME(const u16* __restrict_
     unsigned char* blob = dst + mat * BLOB;
     u16* sc = (u16*)(blob + CODES);
     const u32 ch = lane & 15u, k = kt * 128 + ch * 8;
+#if HB_OP == 1
+    // All four loads in flight at once; past N and K some element's instead.
+    u32x4 vs[4];
+#pragma unroll
+    for (u32 i = 0; i < 4; i++) {
+        const u32 n = nt * 16 + 4 * i + (lane >> 4);
+        vs[i] = *(const chunk_t*)(src + (mat * N + (n < N ? n : N - 1)) * K + (k < K ? k : 0));
+    }
+#endif
 #pragma unroll
     for (u32 i = 0; i < 4; i++) {
         const u32 row = 4 * i + (lane >> 4), n = nt * 16 + row;
         const bool in = live && n < N && k < K;
         u32 nw = 0x88888888u;
 #if HB_OP == 1
-        u32x4 v = {0, 0, 0, 0};
-        if (in) v = *(const chunk_t*)(src + (mat * N + n) * K + k);
-        // The group's largest and smallest element; a group with a NaN or an
-        // infinity stands for NaN.
-        float hi = 0.0f, lo = 0.0f;
-        u32 bad = 0;
-        float w[8];
+        const u32x4 v = in ? vs[i] : u32x4{0, 0, 0, 0};
+        // bf16 bits order as their values do, the positive ones as signed
+        // halves and all of them without their sign: the group's largest of
+        // both, in the low and the high half of one word.
+        s16x2 hi = {-32768, -32768}, size = {0, 0};
 #pragma unroll
-        for (u32 e = 0; e < 8; e++) {
-            w[e] = e & 1 ? bf16_hi(v[e / 2]) : bf16_lo(v[e / 2]);
-            hi = __builtin_fmaxf(hi, w[e]);
-            lo = __builtin_fminf(lo, w[e]);
-            bad |= !(__builtin_fabsf(w[e]) <= 3.4e38f);
+        for (u32 e = 0; e < 4; e++) {
+            hi = __builtin_elementwise_max(hi, __builtin_bit_cast(s16x2, word(v, e)));
+            size = __builtin_elementwise_max(size, __builtin_bit_cast(s16x2, word(v, e) & 0x7fff7fffu));
         }
-#pragma unroll
-        for (u32 o = 1; o < GROUP / 8; o *= 2) {
-            hi = __builtin_fmaxf(hi, __shfl_xor(hi, o, 64));
-            lo = __builtin_fminf(lo, __shfl_xor(lo, o, 64));
-            bad |= __shfl_xor(bad, o, 64);
-        }
+        s16x2 far = {hi.x > hi.y ? hi.x : hi.y, size.x > size.y ? size.x : size.y};
+        far = lane_max<0xB1>(far);  // quad_perm [1, 0, 3, 2], [2, 3, 0, 1]
+        far = lane_max<0x4E>(far);
+        if (GROUP >= 64) far = lane_max<0x141>(far);   // row_half_mirror
+        if (GROUP == 128) far = lane_max<0x140>(far);  // row_mirror
         // s = the element of largest size (the positive one of two) / -8,
-        // which loses bits only among the subnormals.
-        const u32 sb = bad ? 0x7fc0u : f32_to_bf16((hi >= -lo ? hi : lo) * -0.125f);
+        // which loses bits only among the subnormals; a group with a NaN or
+        // an infinity stands for NaN.
+        const u32 top = (u16)far.y;
+        const bool bad = top >= 0x7f80u;
+        const u32 sb = bad ? 0x7fc0u : f32_to_bf16(bf16_to_f32(far.x == far.y ? top : top | 0x8000u) * -0.125f);
         const float s = bf16_to_f32(sb);
-        if (!bad && s != 0.0f) {
-            nw = 0;
-#pragma unroll
-            for (u32 e = 0; e < 8; e++) {
-                const float q = __builtin_fminf(__builtin_fmaxf(__builtin_rintf(__fdiv_rn(w[e], s)), -8.0f), 7.0f);
-                nw |= (u32)(int)(q + 8.0f) << (4 * (e / 2) + 16 * (e & 1));
-            }
-        }
+        if (!bad && top != 0) nw = group_codes(v, s);
         if (live && ch % (GROUP / 8) == 0) sc[scale_at(n, kt, ch / (GROUP / 8))] = n < N && k < K ? (u16)sb : 0;
 #else
         // Row order: byte b of a row holds element 2 b in its low half.
