@@ -9,6 +9,7 @@
 //          MxKxNr     the same with Out::Residual (Y += ...)
 //          MxKxNf     the same with Out::F32
 //          mv:MxKxN   the decode matvec over M <= 16 rows
+//          q4:MxKxN   the same over W quantised to 4 bits, groups of 32
 //
 // Output per shape: shape, kernel, microseconds per launch, TFLOP/s (GEMM)
 // or GB/s of algorithmic bytes (matvec).  The reference's counterpart is
@@ -30,13 +31,14 @@ int die(const char* what) {
 }
 
 struct Shape {
-    bool matvec = false;
+    bool matvec = false, q4 = false;
     uint32_t m = 0, k = 0, n = 0, out = HB_OUT_BF16;
 };
 
 bool parse(const char* s, Shape* sh) {
-    if (!strncmp(s, "mv:", 3)) {
+    if (!strncmp(s, "mv:", 3) || !strncmp(s, "q4:", 3)) {
         sh->matvec = true;
+        sh->q4 = *s == 'q';
         s += 3;
     }
     char tail[8] = "";
@@ -77,14 +79,14 @@ int main(int argc, char** argv) {
         } else {
             Shape sh;
             if (!parse(argv[i], &sh)) {
-                fprintf(stderr, "hb_gemm: bad shape '%s' (MxKxN[r|f] or mv:MxKxN, M <= 16)\n", argv[i]);
+                fprintf(stderr, "hb_gemm: bad shape '%s' (MxKxN[r|f], mv:MxKxN or q4:MxKxN, M <= 16)\n", argv[i]);
                 return 2;
             }
             shapes.push_back(sh);
         }
     }
     if (shapes.empty() || !reps) {
-        fprintf(stderr, "usage: hb_gemm [--tune key=value,...] [--reps N] MxKxN[r|f] | mv:MxKxN ...\n");
+        fprintf(stderr, "usage: hb_gemm [--tune key=value,...] [--reps N] MxKxN[r|f] | mv:MxKxN | q4:MxKxN ...\n");
         return 2;
     }
     hb_gpu* g = nullptr;
@@ -106,7 +108,35 @@ int main(int argc, char** argv) {
         hb_op op;
         memset(&op, 0, sizeof op);
         op.m = s.m;
-        if (s.matvec) {
+        if (s.q4) {
+            // W's place is taken by its packed form.
+            const uint64_t bytes = hb_q4_bytes(s.k, s.n, 32);
+            hb_desc d;
+            memset(&d, 0, sizeof d);
+            d.kind = HB_KIND_Q4_QUANTIZE;
+            d.k = s.k;
+            d.n = s.n;
+            d.bk = 32;
+            hb_buf q = 0;
+            int32_t quant = -1;
+            if (hb_kernel_build(g, &d, &quant) || hb_alloc(g, bytes, &q)) {
+                status = die("q4");
+                continue;
+            }
+            const hb_range b[2] = {whole(w), whole(q)};
+            if (hb_launch(g, quant, b, 2, 1) || hb_sync(g)) return die("q4_quantize");
+            hb_free(g, w);
+            w = q;
+            const hb_range wr = whole(w);
+            if (hb_engine_matvec_q4(e, s.k, s.n, s.out, 32, s.m, &wr, 1, whole(x), whole(y), &kern)) {
+                status = die("hb_engine_matvec_q4");
+                continue;
+            }
+            op.nbind = 3;
+            op.bind[0] = whole(w);
+            op.bind[1] = whole(x);
+            op.bind[2] = whole(y);
+        } else if (s.matvec) {
             hb_range wr = whole(w);
             if (hb_engine_matvec(e, s.k, s.n, s.out, s.m, &wr, 1, whole(x), whole(y), &kern)) {
                 status = die("hb_engine_matvec");
@@ -134,9 +164,10 @@ int main(int argc, char** argv) {
         if (hb_time(g, &op, 1, 3, &secs) || hb_time(g, &op, 1, reps, &secs)) return die("hb_time");
         const double t = secs / reps;
         if (s.matvec) {
-            const double bytes = 2.0 * s.n * s.k + 2.0 * s.m * s.k +
+            const double weights = s.q4 ? (double)s.n * s.k * (0.5 + 2.0 / 32) : 2.0 * s.n * s.k;
+            const double bytes = weights + 2.0 * s.m * s.k +
                                  2.0 * s.m * s.n * (s.out == HB_OUT_RESIDUAL ? 2 : 1);
-            printf("mv:%ux%ux%u %s %.2f us %.1f GB/s\n", s.m, s.k, s.n, hb_kernel_name(g, kern), t * 1e6,
+            printf("%s:%ux%ux%u %s %.2f us %.1f GB/s\n", s.q4 ? "q4" : "mv", s.m, s.k, s.n, hb_kernel_name(g, kern), t * 1e6,
                    bytes / t / 1e9);
         } else {
             printf("%ux%ux%u%s %s %.2f us %.1f TFLOP/s\n", s.m, s.k, s.n,

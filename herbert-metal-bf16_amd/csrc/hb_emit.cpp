@@ -10,8 +10,6 @@
 #include <cstdlib>
 #include <cstdio>
 #include <cstring>
-#include <utility>
-#include <vector>
 
 #include "hb_internal.h"
 
@@ -43,8 +41,9 @@ static uint64_t q4_tiles(uint32_t k, uint32_t n) { return ((uint64_t)k + 127) / 
 static uint64_t q4_bytes(uint32_t k, uint32_t n, uint32_t group) {
     return q4_tiles(k, n) * 1024 + ((uint64_t)k + 127) / 128 * (((uint64_t)n + 63) / 64) * (16384 / group);
 }
+// k and n within what keeps every byte count of a launch in 64 bits.
 static bool q4_shape(uint32_t k, uint32_t n, uint32_t group) {
-    return k && n && k % 8 == 0 && (group == 32 || group == 64 || group == 128) && q4_tiles(k, n) < (1u << 30);
+    return k && n && k % 8 == 0 && k <= (1u << 20) && n <= (1u << 24) && (group == 32 || group == 64 || group == 128);
 }
 
 // The 4-bit matvec's form by its row tiles (16 W rows) and K tiles (128 K).
@@ -404,7 +403,7 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
         case HB_KIND_Q4_PACK:
         case HB_KIND_Q4_DEQUANTIZE: {
             if (!q4_shape(d.k, d.n, d.bk))
-                return fail(HB_ERR_UNSUPPORTED, "q4: K a multiple of 8, groups of 32, 64 or 128");
+                return fail(HB_ERR_UNSUPPORTED, "q4: K a multiple of 8 up to 2^20, N up to 2^24, groups of 32, 64 or 128");
             const uint32_t op = d.kind - HB_KIND_Q4_QUANTIZE + 1;
             snprintf(name, sizeof name, "q4_%s_%ux%u_g%u", op == 1 ? "quantize" : op == 2 ? "pack" : "dequantize",
                      d.k, d.n, d.bk);
@@ -420,7 +419,8 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             if (d.out > HB_OUT_SWIGLU || d.rows_of > HB_ROWS_SCATTER)
                 return fail(HB_ERR_INVALID, "matvec_q4: out / rows_of out of range");
             if (!q4_shape(d.k, d.n, d.bk))
-                return fail(HB_ERR_UNSUPPORTED, "matvec_q4: K a multiple of 8, groups of 32, 64 or 128");
+                return fail(HB_ERR_UNSUPPORTED,
+                            "matvec_q4: K a multiple of 8 up to 2^20, N up to 2^24, groups of 32, 64 or 128");
             if (swi && d.n % 32)
                 return fail(HB_ERR_UNSUPPORTED, "matvec_q4 Out::Swiglu: gate and up rows each a multiple of 16");
             if (d.mv_m > 16) return fail(HB_ERR_UNSUPPORTED, "matvec_q4: m <= 16");
@@ -428,10 +428,11 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
                 return fail(HB_ERR_UNSUPPORTED, "matvec_q4: 16, 32, 64 or 128 rows a wave (Out::Swiglu not 16)");
             if (d.mv_waves > 16 || !pow2(d.mv_waves) || !pow2(d.split) || d.split > d.mv_waves || d.unroll > 4)
                 return fail(HB_ERR_UNSUPPORTED, "matvec_q4: 1, 2, 4, 8 or 16 waves, split no more, unroll 1..4");
-            if (experts && (!d.top_k || !d.experts || !d.tiles || !d.rows_max || d.mv_m != 16 ||
+            if (experts && (!d.top_k || d.top_k > d.experts || d.experts > 1024 || !d.tiles || !d.rows_max ||
+                            (uint64_t)d.rows_max * d.top_k >= (1u << 28) || d.mv_m != 16 ||
                             (d.out != HB_OUT_BF16 && !swi)))
-                return fail(HB_ERR_INVALID,
-                            "matvec_q4 over experts: top_k, experts, tiles and rows_max, tiles of 16 rows, bf16 out");
+                return fail(HB_ERR_INVALID, "matvec_q4 over experts: top_k, experts (<= 1024), tiles and rows_max "
+                                            "(below 2^28 pairs), tiles of 16 rows, bf16 out");
             std::string rows;
             if (experts) {
                 snprintf(name, sizeof name, "_%s_k%u_e%u_t%u_r%u", d.rows_of == HB_ROWS_GATHER ? "gather" : "scatter",
@@ -581,49 +582,73 @@ struct Access {
     bool write, rows;
 };
 
-static std::vector<Access> accesses(const hb_desc& d, uint32_t m) {
-    const uint64_t mm = m, k = d.k, n = d.n;
-    std::vector<Access> a;
-    if (d.kind == HB_KIND_Q4_QUANTIZE || d.kind == HB_KIND_Q4_DEQUANTIZE) {
-        const bool to = d.kind == HB_KIND_Q4_QUANTIZE;
-        a = {{"W", mm * n * k * 2, 2, !to, false}, {"q4", mm * q4_bytes(d.k, d.n, d.bk), 16, to, false}};
-        if (!to) std::swap(a[0], a[1]);
-    } else if (d.kind == HB_KIND_Q4_PACK) {
-        a = {{"codes", mm * n * k / 2, 2, false, false},
-             {"scales", mm * n * cdiv(d.k, d.bk) * 2, 2, false, false},
-             {"q4", mm * q4_bytes(d.k, d.n, d.bk), 16, true, false}};
-    } else if (d.kind == HB_KIND_MATVEC_Q4) {
-        const uint64_t nout = d.out == HB_OUT_SWIGLU ? n / 2 : n;
-        const uint32_t size = out_bytes(d.out);
-        if (d.rows_of == HB_ROWS_DENSE)
-            return {{"q4", q4_bytes(d.k, d.n, d.bk), 16, false, false},
-                    {"x", mm * k * 2, 2, false, false},
-                    {"y", mm * nout * size, size, true, false}};
-        const uint64_t pairs = mm * d.top_k;
-        a = {{"state", 16, 4, false, false},
-             {"q4", d.experts * q4_bytes(d.k, d.n, d.bk), 16, false, false},
-             {"X", (d.rows_of == HB_ROWS_GATHER ? mm : pairs) * k * 2, 2, false, false},
-             {"Y", pairs * nout * size, size, true, false},
-             {"list", pairs * 4, 4, false, false},
-             {"tiles", (1 + 3ull * d.tiles) * 4, 4, false, false}};
-    } else if (d.kind == HB_KIND_BLOCK_NORM) {
-        const uint64_t all = mm * n * 2;
-        a = {{"x", all, 2, false, true}, {"y", all, 2, false, true}, {"xo", all, 2, true, true}};
-        if (d.form & HB_NORM_PRE) a.push_back({"h", all, 2, true, true});
-        if (d.form & HB_NORM_POST) a.push_back({"w_post", n * 2, 2, false, false});
-        const uint32_t gate = d.form & HB_NORM_GATE_CHANNELS;
-        if (gate == HB_NORM_GATE_ROWS) a.push_back({"gate", mm * 2, 2, false, false});
-        if (gate == HB_NORM_GATE_ELEMENTS) a.push_back({"gate", all, 2, false, true});
-        if (gate == HB_NORM_GATE_CHANNELS) a.push_back({"gate", n * 2, 2, false, false});
-        if (d.form & HB_NORM_SCALES) a.push_back({"scales", 8, 4, false, false});
-        if (d.form & HB_NORM_PRE) a.push_back({"w_pre", n * 2, 2, false, false});
+struct AccessList {
+    Access a[8];
+    uint32_t n = 0;
+    void add(const char* what, uint64_t bytes, uint32_t align, bool write, bool rows = false) {
+        a[n++] = {what, bytes, align, write, rows};
     }
-    return a;
+};
+
+static AccessList accesses(const hb_desc& d, uint32_t m) {
+    const uint64_t mm = m, k = d.k, n = d.n;
+    AccessList l;
+    switch (d.kind) {
+        case HB_KIND_Q4_QUANTIZE:
+            l.add("W", mm * n * k * 2, 2, false);
+            l.add("q4", mm * q4_bytes(d.k, d.n, d.bk), 16, true);
+            break;
+        case HB_KIND_Q4_DEQUANTIZE:
+            l.add("q4", mm * q4_bytes(d.k, d.n, d.bk), 16, false);
+            l.add("W", mm * n * k * 2, 2, true);
+            break;
+        case HB_KIND_Q4_PACK:
+            l.add("codes", mm * n * k / 2, 2, false);
+            l.add("scales", mm * n * cdiv(d.k, d.bk) * 2, 2, false);
+            l.add("q4", mm * q4_bytes(d.k, d.n, d.bk), 16, true);
+            break;
+        case HB_KIND_MATVEC_Q4: {
+            const uint64_t nout = d.out == HB_OUT_SWIGLU ? n / 2 : n, q4 = q4_bytes(d.k, d.n, d.bk), pairs = mm * d.top_k;
+            const uint32_t size = out_bytes(d.out);
+            if (d.rows_of == HB_ROWS_DENSE) {
+                l.add("q4", q4, 16, false);
+                l.add("x", mm * k * 2, 2, false);
+                l.add("y", mm * nout * size, size, true);
+                break;
+            }
+            l.add("state", 16, 4, false);
+            l.add("q4", d.experts * q4, 16, false);
+            l.add("X", (d.rows_of == HB_ROWS_GATHER ? mm : pairs) * k * 2, 2, false);
+            l.add("Y", pairs * nout * size, size, true);
+            l.add("list", pairs * 4, 4, false);
+            l.add("tiles", (1 + 3ull * d.tiles) * 4, 4, false);
+            break;
+        }
+        case HB_KIND_BLOCK_NORM: {
+            const uint64_t all = mm * n * 2;
+            const uint32_t gate = d.form & HB_NORM_GATE_CHANNELS;
+            l.add("x", all, 2, false, true);
+            l.add("y", all, 2, false, true);
+            l.add("xo", all, 2, true, true);
+            if (d.form & HB_NORM_PRE) l.add("h", all, 2, true, true);
+            if (d.form & HB_NORM_POST) l.add("w_post", n * 2, 2, false);
+            if (gate == HB_NORM_GATE_ROWS) l.add("gate", mm * 2, 2, false);
+            if (gate == HB_NORM_GATE_ELEMENTS) l.add("gate", all, 2, false, true);
+            if (gate == HB_NORM_GATE_CHANNELS) l.add("gate", n * 2, 2, false);
+            if (d.form & HB_NORM_SCALES) l.add("scales", 8, 4, false);
+            if (d.form & HB_NORM_PRE) l.add("w_pre", n * 2, 2, false);
+            break;
+        }
+        default:
+            break;
+    }
+    return l;
 }
 
 int check_addresses(const hb_desc& d, void* const* ptrs, uint32_t nbind, uint32_t m) {
-    const std::vector<Access> a = accesses(d, m);
-    for (uint32_t i = 0; i < a.size() && i < nbind; i++) {
+    const AccessList l = accesses(d, m);
+    const Access* const a = l.a;
+    for (uint32_t i = 0; i < l.n && i < nbind; i++) {
         const uintptr_t pi = (uintptr_t)ptrs[i];
         if (pi % a[i].align)
             return fail(HB_ERR_INVALID, std::string("binding ") + std::to_string(i) + " (" + a[i].what +
@@ -682,16 +707,19 @@ int check_bindings(const hb_desc& d, const uint64_t* s, uint32_t nbind, uint32_t
         return HB_OK;
     }
     if (m == 0) return fail(HB_ERR_INVALID, "0 rows");
-    const std::vector<Access> acc = accesses(d, m);
-    if (!acc.empty()) {
-        if (d.kind == HB_KIND_MATVEC_Q4 && d.rows_of == HB_ROWS_DENSE && m > d.mv_m)
-            return fail(HB_ERR_INVALID, "matvec_q4 of " + std::to_string(m) + " rows: 1.." + std::to_string(d.mv_m));
-        if (d.kind == HB_KIND_MATVEC_Q4 && d.rows_of != HB_ROWS_DENSE && m > d.rows_max)
-            return fail(HB_ERR_INVALID, "m beyond the kernel's rows_max");
-        if (d.kind < HB_KIND_MATVEC_Q4 && m * q4_tiles(d.k, d.n) >= (1ull << 32))
+    if (d.kind >= HB_KIND_Q4_QUANTIZE && d.kind <= HB_KIND_BLOCK_NORM) {
+        // First what keeps the byte counts and the grid within range.
+        if (d.kind == HB_KIND_MATVEC_Q4) {
+            const bool dense = d.rows_of == HB_ROWS_DENSE;
+            if (dense && m > d.mv_m)
+                return fail(HB_ERR_INVALID, "matvec_q4 of " + std::to_string(m) + " rows: 1.." + std::to_string(d.mv_m));
+            if (!dense && m > d.rows_max) return fail(HB_ERR_INVALID, "m beyond the kernel's rows_max");
+        } else if (d.kind != HB_KIND_BLOCK_NORM && m * q4_tiles(d.k, d.n) >= (1u << 26)) {
             return fail(HB_ERR_UNSUPPORTED, "q4: too many matrices in one launch");
-        for (uint32_t i = 0; i < acc.size(); i++)
-            if ((rc = need(s, i, acc[i].bytes, acc[i].what))) return rc;
+        }
+        const AccessList l = accesses(d, m);
+        for (uint32_t i = 0; i < l.n; i++)
+            if ((rc = need(s, i, l.a[i].bytes, l.a[i].what))) return rc;
         return HB_OK;
     }
     uint64_t mm = m, k2 = 2ull * d.top_k;

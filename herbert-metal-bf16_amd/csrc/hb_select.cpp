@@ -1272,6 +1272,7 @@ int hb_engine_matvec_q4(hb_engine* e, uint32_t k, uint32_t n, uint32_t out, uint
                         const hb_range* ws, uint32_t nws, hb_range x, hb_range y, int32_t* kernel) {
     if (!e->g) return fail(HB_ERR_INVALID, "matvec_q4: an engine without a context");
     if (!nws) return fail(HB_ERR_INVALID, "matvec_q4: no weights");
+    if (!mv_m || !group) return fail(HB_ERR_INVALID, "matvec_q4: 0 rows, or a group of 0");
     const auto list = mv_q4_candidates(k, n, out, group, mv_m);
     if (!e->t["mv.auto"]) return e->build(list[0], kernel);
     const std::string key = q4_key(list[0]);

@@ -798,10 +798,11 @@ class MoeBlock:
     `w`: device buffers {"post_norm": [h], "router": [E][h], "w_gate_up":
     [E*2*inter][h], "w_down": [E*h][inter], "s_gate_up": [2*si][h], "s_down":
     [h][si], "shared_gate": [h]}.  `x` (host [rows][h]) is the residual
-    stream the selection runs on; the block updates buf["x"] in place."""
+    stream the selection runs on; the block updates buf["x"] in place.
+    q4_group: w_gate_up and w_down in 4 bits, as MoeLayer takes them."""
 
     def __init__(self, gpu, engine, experts, top_k, hidden, inter, shared_inter, rows, w, x,
-                 eps=1e-6, plus_one=True):
+                 eps=1e-6, plus_one=True, q4_group=0):
         g, h, si = gpu, hidden, shared_inter
         self.gpu, self.rows, self.h, self.si, self.w = gpu, rows, h, si, w
         self.buf = {"state": g.alloc_with(np.array([0, 0, 0, rows], np.uint32)),
@@ -825,7 +826,7 @@ class MoeBlock:
         g.free(xn_t)
         g.free(sc_t)
         self.layer = MoeLayer(g, engine, experts, top_k, h, inter, rows, w["w_gate_up"], w["w_down"],
-                              scores=scores, x=xn)
+                              scores=scores, x=xn, q4_group=q4_group)
         L = self.layer.buf
         self.s_gu_k, self.s_sw_k = engine.gate_up(h, si, r(b["state"]), r(w["s_gate_up"]), r(L["x"]),
                                                   r(b["s_gu"]), r(b["s_h"]), rows)
@@ -919,6 +920,25 @@ class Checkpoint:
         check(lib.hb_ckpt_upload(gpu.h, self.h, keys, lens, len(parts), ctypes.byref(b)))
         gpu._sizes[b.value] = 2 * sum(int(n) for _, n in parts)
         return b.value
+
+    def upload_q4(self, gpu, parts, kdim, n, group=32, count=1):
+        """upload, then quantised on the GPU: `count` packed 4-bit matrices of
+        n rows of kdim, the bf16 weights given back."""
+        if sum(int(c) for _, c in parts) != count * n * kdim:
+            raise HerbertError(HB_ERR_INVALID, "upload_q4: the parts hold no %d matrices of %dx%d" % (count, n, kdim))
+        q = gpu.alloc(count * q4_bytes(kdim, n, group))
+        w = None
+        try:
+            w = self.upload(gpu, parts)
+            gpu.launch(gpu.pipeline(q4_quantize(kdim, n, group)), [r(w), r(q)], count)
+            gpu.sync()
+        except Exception:
+            gpu.free(q)
+            raise
+        finally:
+            if w is not None:
+                gpu.free(w)
+        return q
 
 
 _BLOCK_IN = ctypes.CFUNCTYPE(ctypes.c_int, _P, _u32, _u32, ctypes.POINTER(ctypes.c_double))
@@ -1158,19 +1178,23 @@ def route_probe_rows(ckpt, block, hidden):
     return emb[np.array(probe_ids(block), dtype=np.int64) % vocab]
 
 
-def moe_weights_from_checkpoint(gpu, ckpt, layer, experts, hidden, inter, shared_inter):
+def moe_weights_from_checkpoint(gpu, ckpt, layer, experts, hidden, inter, shared_inter, q4_group=0):
     """The device weights of a qwen3_5_moe layer's sparse MLP as
     QwenEngine::load uploads them (qwen.rs:788-801): the post norm, the
     router (mlp.gate), the experts' [gate | up] rows and down rows
     (mlp.experts.gate_up_proj [E][2 inter][h], down_proj [E][h][inter]),
     the shared expert stacked [gate | up], its down and its gate; the dict
-    MoeBlock takes."""
+    MoeBlock takes.  q4_group: the experts quantised to 4 bits in groups of it."""
+    def experts_w(key, kdim, n):
+        parts = [(p(key), e * n * kdim)]
+        return ckpt.upload_q4(gpu, parts, kdim, n, q4_group, e) if q4_group else ckpt.upload(gpu, parts)
+
     p = lambda f: "%d.%s" % (layer, f)  # noqa: E731
     h, e, mi, si = hidden, experts, inter, shared_inter
     return {"post_norm": ckpt.upload(gpu, [(p("post_attention_layernorm.weight"), h)]),
             "router": ckpt.upload(gpu, [(p("mlp.gate.weight"), e * h)]),
-            "w_gate_up": ckpt.upload(gpu, [(p("mlp.experts.gate_up_proj"), e * 2 * mi * h)]),
-            "w_down": ckpt.upload(gpu, [(p("mlp.experts.down_proj"), e * h * mi)]),
+            "w_gate_up": experts_w("mlp.experts.gate_up_proj", h, 2 * mi),
+            "w_down": experts_w("mlp.experts.down_proj", mi, h),
             "s_gate_up": ckpt.upload(gpu, [(p("mlp.shared_expert.gate_proj.weight"), si * h),
                                            (p("mlp.shared_expert.up_proj.weight"), si * h)]),
             "s_down": ckpt.upload(gpu, [(p("mlp.shared_expert.down_proj.weight"), h * si)]),

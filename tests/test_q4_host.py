@@ -47,6 +47,10 @@ def test_q4_bytes(hb):
     (lambda hb: hb.experts_q4(128, 64, hb.Out.F32, 32, hb.Rows.Gather, 8, 64, 4), "bf16 out"),
     (lambda hb: hb.experts_q4(128, 64, hb.Out.Bf16, 32, hb.Rows.Sorted, 8, 64, 4), "rows_of"),
     (lambda hb: hb.experts_q4(128, 64, hb.Out.Bf16, 32, hb.Rows.Gather, 8, 64, 4).replace(tiles=0), "tiles"),
+    (lambda hb: hb.experts_q4(128, 64, hb.Out.Bf16, 32, hb.Rows.Gather, 8, 2048, 4), "experts"),
+    (lambda hb: hb.experts_q4(128, 64, hb.Out.Bf16, 32, hb.Rows.Gather, 8, 64, 1 << 26), "pairs"),
+    (lambda hb: hb.matvec_q4((1 << 20) + 8, 16, hb.Out.Bf16), "K a multiple of 8 up to"),
+    (lambda hb: hb.matvec_q4(128, (1 << 24) + 1, hb.Out.Bf16), "N up to"),
     (lambda hb: hb.q4_quantize(4, 16), "K a multiple of 8"),
     (lambda hb: hb.q4_pack(8, 16, 31), "groups"),
     (lambda hb: hb.q4_dequantize(8, 0), "q4"),
@@ -129,7 +133,7 @@ def test_refused_quantize_launches(hb, gpu):
     w, q = gpu.alloc(2 * 64 * 16), gpu.alloc(hb.q4_bytes(64, 16))
     for ranges, m, match in [([hb.r(w, 0, 2046), hb.r(q)], 1, "W"), ([hb.r(w), hb.r(q, 0, 1000)], 1, "q4"),
                              ([hb.r(w), hb.r(q)], 2, "binding"), ([hb.r(w), hb.r(q)], 0, "0 rows"),
-                             ([hb.r(w), hb.r(w)], 1, "overlap|holds")]:
+                             ([hb.r(w), hb.r(w)], 1, "overlap|holds"), ([hb.r(w), hb.r(q)], 1 << 31, "too many")]:
         with pytest.raises(hb.HerbertError, match=match):
             gpu.launch(k, ranges, m)
 
@@ -149,6 +153,13 @@ def test_engine_choice_and_pins(hb, gpu):
             e.mv_q4(128, 32, hb.Out.Bf16, 32, 2, [], hb.r(x), hb.r(y))
         with pytest.raises(hb.HerbertError, match="m <= 16"):
             e.mv_q4(128, 32, hb.Out.Bf16, 32, 17, [hb.r(w)], hb.r(x), hb.r(y))
+        with pytest.raises(hb.HerbertError, match="0 rows"):
+            e.mv_q4(128, 32, hb.Out.Bf16, 32, 0, [hb.r(w)], hb.r(x), hb.r(y))
+        with pytest.raises(hb.HerbertError, match="group"):
+            e.mv_q4(128, 32, hb.Out.Bf16, 0, 2, [hb.r(w)], hb.r(x), hb.r(y))
+    with hb.Engine(None) as e:
+        with pytest.raises(hb.HerbertError, match="without a context"):
+            e.mv_q4(*args)
     with hb.Engine(gpu, "") as e:
         e.pin(text)
         assert e.mv_q4(*args) == k and e.picks() == text
@@ -160,6 +171,7 @@ def test_engine_choice_and_pins(hb, gpu):
 @pytest.mark.parametrize("desc", [
     herbert_hip.matvec_q4(8, 1, herbert_hip.Out.Bf16),
     herbert_hip.matvec_q4(17408, 5120, herbert_hip.Out.F32, 32, 16, 64, 16, 16, 4),
+    herbert_hip.matvec_q4(17408, 5120, herbert_hip.Out.Swiglu, 32, 16, 128, 16, 16, 1),
     herbert_hip.experts_q4(2048, 1024, herbert_hip.Out.Swiglu, 128, herbert_hip.Rows.Gather, 8, 256, 64),
     herbert_hip.q4_quantize(72, 3, 128), herbert_hip.q4_pack(72, 3, 64), herbert_hip.q4_dequantize(72, 3, 32),
     herbert_hip.block_norm(1, 1e-6), herbert_hip.block_norm(32768, 1e-6, True, True, True, herbert_hip.Gate.Elements, True),
