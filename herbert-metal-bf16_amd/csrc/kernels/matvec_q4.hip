@@ -11,7 +11,8 @@
 // products, and starts from the sum of -24 x, an MFMA with a constant operand
 // that the row tiles of a wave share.  The group's scale then multiplies the
 // f32 sum of 16 rows x 16 columns.  Sums are f32 throughout; Out rounds once.
-// (24 x has to be finite: an x beyond 2^123 or an infinity gives NaN.)
+// (The sums pass through 24 x and 31 x: an infinite x, or a group's sum of
+// those past f32's range, gives NaN.)
 //
 // Bound by the codes' bytes: K N / 2 and 2 K N / GROUP for the scales.
 #include "hb_common.h"

@@ -161,7 +161,13 @@ typedef struct hb_desc {
      * through a per-wave LDS tile (unroll 4, 8 or 16; rows 32: two 16-row
      * MFMA tiles sharing each x fragment), 4 v_mfma_f32_4x4x4_16b_bf16 with
      * 4 W rows per wave, its 16 blocks slices of K, W loaded straight into
-     * the operand (m <= 8, K/split a multiple of 128, no fusions). */
+     * the operand (m <= 8, K/split a multiple of 128, no fusions).
+     * MATVEC_Q4: mv_m rows of x (1..16; 16 over experts), rows = W rows per
+     * wave (16, 32, 64 or 128; Out::Swiglu not 16), split waves sharing their K of
+     * mv_waves (1, 2, 4, 8 or 16), unroll tiles of 128 K in flight (1..4); 0
+     * = what the shape calls for.  bk = the weights' group, 0 = 32.  These
+     * fix the order of a row's sums, which depends neither on the launch's
+     * rows nor on the other rows. */
     uint32_t mv_m, split, persist, rows, form;
     /* MoE: slots per row (top_k), experts, the tile table's capacity
      * (moe_tiles, prefill.rs:832-835), rows of the largest block. */
@@ -265,8 +271,8 @@ double hb_compile_seconds(hb_gpu *gpu);
  * f32 and u32 4, q4 16), and what a launch writes overlaps nothing else it
  * binds: both are checked.  Of MATVEC_Q4: HB_OUT_BF16, _F32, _RESIDUAL
  * (y = rne(y + sum), one rounding) and _SWIGLU (n / 2 a multiple of 16, h =
- * rne(g * sigmoid(g) * u) of the f32 sums).  x beyond 2^123 or infinite
- * gives NaN.  Over experts (rows_of HB_ROWS_GATHER: x rows through the list,
+ * rne(g * sigmoid(g) * u) of the f32 sums).  The sums go through
+ * 31 |x|: an infinite x, or 128 of them past 2^116, give NaN.  Over experts (rows_of HB_ROWS_GATHER: x rows through the list,
  * y rows in sorted order; HB_ROWS_SCATTER: the other way round) the table is
  * one of tiles of up to 16 rows; y rows of no tile are left as they are.
  * `m` is the rows of the block (the kernels read state[3], never beyond m).

@@ -273,3 +273,46 @@ def test_experts_rows_of_state(gpu):
     finally:
         for b in bufs + [wd]:
             gpu.free(b)
+
+
+def test_rows_stand_alone(gpu):
+    """A row's bits depend neither on the launch's rows nor on the others: in
+    the matvec, and for a token of the experts alone and in a batch."""
+    k, n = 1032, 80
+    rng = np.random.default_rng(11)
+    codes, scales = q4.random_codes(rng, n, k, 64)
+    x = hb.normal_bf16(8, 1.0, (16, k))
+    full = matvec(gpu, codes, scales, x, k, n, 64, hb.Out.F32, mv_m=16)
+    for rows in (slice(0, 1), slice(3, 8), slice(5, 16)):
+        assert np.array_equal(matvec(gpu, codes, scales, x[rows], k, n, 64, hb.Out.F32, mv_m=16), full[rows])
+    t, top_k, experts, h = 30, 2, 16, 96
+    dn, ds = q4.random_codes(rng, experts * h, k, 64)
+    w = q4.pack(gpu, dn, ds, k, h, 64, experts)
+    hx = hb.normal_bf16(9, 1.0, (t * top_k, k))
+    kern = hb.experts_q4(k, h, hb.Out.Bf16, 64, hb.Rows.Scatter, top_k, experts, t)
+
+    def down(pairs_x, expert_of):
+        """y rows of sorted pairs whose experts are given in order."""
+        table = []
+        for e in np.unique(expert_of):
+            at = np.flatnonzero(expert_of == e)
+            table += [(e, at[0] + o, min(16, len(at) - o)) for o in range(0, len(at), 16)]
+        tiles = np.zeros(1 + 3 * hb.moe_tiles(t, top_k, experts, 16), np.uint32)
+        tiles[0] = len(table)
+        tiles[1:1 + 3 * len(table)] = np.array(table, np.uint32).reshape(-1)
+        m = len(pairs_x) // top_k
+        bufs = [gpu.alloc_with(a) for a in (np.array([0, 0, 0, m], np.uint32), pairs_x, np.zeros(len(pairs_x) * h, np.uint16),
+                                            np.arange(len(pairs_x), dtype=np.uint32), tiles)]
+        try:
+            st, xb, yb, lb, tb = bufs
+            run(gpu, kern, [hb.r(st), hb.r(w), hb.r(xb), hb.r(yb), hb.r(lb), hb.r(tb)], m)
+            return gpu.download(yb, np.uint16, len(pairs_x) * h).reshape(-1, h)
+        finally:
+            for b in bufs:
+                gpu.free(b)
+
+    batch = down(hx, np.repeat([2, 9, 15], 20))
+    for i in (0, 19, 23, 58):
+        alone = down(np.concatenate([hx[i:i + 1], hx[i:i + 1]]), np.array([[2, 9, 15][i // 20]] * 2))
+        assert np.array_equal(alone[0], batch[i]) and np.array_equal(alone[1], batch[i]), i
+    gpu.free(w)
