@@ -28,6 +28,14 @@ static_assert(GROUP == 32 || GROUP == 64 || GROUP == 128, "groups of 32, 64 or 1
 // Tensors may start at any element.
 typedef u32x4 chunk_t __attribute__((aligned(2)));
 
+typedef u32 word_t __attribute__((aligned(2)));
+// The low halves of a word's bytes, side by side.
+HB_DEV u32 halves(u32 b) {
+    b &= 0x0f0f0f0fu;
+    b = (b | b >> 4) & 0x00ff00ffu;
+    return (b | b >> 8) & 0xffffu;
+}
+
 // Word of chunk ch (8 elements) of row `row` within a tile's 256 words.
 HB_DEV u32 word_at(u32 row, u32 ch) { return ((ch & 3u) * 16 + row) * 4 + (ch >> 2); }
 // Scale of group g of row n in the K tile kt.
@@ -58,18 +66,23 @@ HB_DEV u32 group_codes(u32x4 v, float s) {
         }
         return nw;
     }
-    // The quotient to the last bit, by the reciprocal and one correction by
-    // the exact remainder (Markstein): ten instructions less than a division.
-    const float r = __fdiv_rn(1.0f, s);
+    // w / s by the reciprocal, corrected once by its exact remainder.  w and s
+    // have 8 bits each, so a quotient that is no half lies 2^-11 or more from
+    // the next one, and where it is one the correction gives it exactly.
+    // Adding 2^23 + 8 rounds to a whole number in the low bits, ties to even as
+    // 8 is even; the words' other bits sum to a constant.
+    const float r = __builtin_amdgcn_rcpf(s);
+    constexpr u32 MAGIC = 0x4B000000u;
+    nw = 0;
+#pragma unroll
+    for (u32 e = 0; e < 8; e++) nw -= MAGIC << (4 * (e / 2) + 16 * (e & 1));
 #pragma unroll
     for (u32 e = 0; e < 8; e++) {
         const float w = e & 1 ? bf16_hi(v[e / 2]) : bf16_lo(v[e / 2]);
         float q = w * r;
         q = __builtin_fmaf(__builtin_fmaf(-s, q, w), r, q);
-        // 2^23 + 8 added rounds to a whole number in the low bits, ties to
-        // even as 8 is even.
         const float z = __builtin_amdgcn_fmed3f(q, -8.0f, 7.0f) + 8388616.0f;
-        nw |= (__builtin_bit_cast(u32, z) & 15u) << (4 * (e / 2) + 16 * (e & 1));
+        nw += __builtin_bit_cast(u32, z) << (4 * (e / 2) + 16 * (e & 1));
     }
     return nw;
 }
@@ -90,15 +103,23 @@ extern "C" __global__ __launch_bounds__(256) void HB_NAME(const u16* __restrict_
     unsigned char* blob = dst + mat * BLOB;
     u16* sc = (u16*)(blob + CODES);
     const u32 ch = lane & 15u, k = kt * 128 + ch * 8;
+    // All loads in flight at once; past N and K some element's instead.
 #if HB_OP == 1
-    // All four loads in flight at once; past N and K some element's instead.
     u32x4 vs[4];
+#else
+    u32 vs[4], ss[4];
+#endif
 #pragma unroll
     for (u32 i = 0; i < 4; i++) {
         const u32 n = nt * 16 + 4 * i + (lane >> 4);
-        vs[i] = *(const chunk_t*)(src + (mat * N + (n < N ? n : N - 1)) * K + (k < K ? k : 0));
-    }
+        const u64 row = mat * N + (n < N ? n : N - 1);
+#if HB_OP == 1
+        vs[i] = *(const chunk_t*)(src + row * K + (k < K ? k : 0));
+#else
+        vs[i] = *(const word_t*)(src + (row * K + (k < K ? k : 0)) / 4);
+        ss[i] = scales[row * GROUPS + (k < K ? k : 0) / GROUP];
 #endif
+    }
 #pragma unroll
     for (u32 i = 0; i < 4; i++) {
         const u32 row = 4 * i + (lane >> 4), n = nt * 16 + row;
@@ -125,21 +146,15 @@ extern "C" __global__ __launch_bounds__(256) void HB_NAME(const u16* __restrict_
         // an infinity stands for NaN.
         const u32 top = (u16)far.y;
         const bool bad = top >= 0x7f80u;
-        const u32 sb = bad ? 0x7fc0u : f32_to_bf16(bf16_to_f32(far.x == far.y ? top : top | 0x8000u) * -0.125f);
+        const float eighth = bf16_to_f32(far.x == far.y ? top : top | 0x8000u) * -0.125f;
+        const u32 sb = bad ? 0x7fc0u : pack_bf16x2(eighth, 0.0f);
         const float s = bf16_to_f32(sb);
         if (!bad && top != 0) nw = group_codes(v, s);
         if (live && ch % (GROUP / 8) == 0) sc[scale_at(n, kt, ch / (GROUP / 8))] = n < N && k < K ? (u16)sb : 0;
 #else
         // Row order: byte b of a row holds element 2 b in its low half.
-        if (in) {
-            const u16* p = src + ((mat * N + n) * K + k) / 4;
-            const u32 b = p[0] | (u32)p[1] << 16;
-            nw = 0;
-#pragma unroll
-            for (u32 e = 0; e < 8; e++) nw |= (b >> (4 * e) & 15u) << (4 * (e / 2) + 16 * (e & 1));
-        }
-        if (live && ch % (GROUP / 8) == 0)
-            sc[scale_at(n, kt, ch / (GROUP / 8))] = n < N && k < K ? scales[(mat * N + n) * GROUPS + k / GROUP] : 0;
+        if (in) nw = halves(vs[i]) | halves(vs[i] >> 4) << 16;
+        if (live && ch % (GROUP / 8) == 0) sc[scale_at(n, kt, ch / (GROUP / 8))] = in ? (u16)ss[i] : 0;
 #endif
         words[wave][word_at(row, ch)] = rotl(nw, 3);
     }
