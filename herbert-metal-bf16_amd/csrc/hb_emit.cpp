@@ -52,7 +52,9 @@ static bool q4_shape(uint32_t k, uint32_t n, uint32_t group) {
 // 2560 at 1 row: 3.5 us, 32 rows 4.9), 32 up to 4096 tiles (2560 to 18432 with
 // the SwiGLU: 7.4 us, 64 rows 8.1), then 64, whose x and scales serve four
 // tiles a load (2560 to 151936 at 4 rows: 36.8 us, 32 rows 41); past 8 x rows
-// 128 (39.9 at 16 rows, 64 rows 42.9).
+// 128 (39.9 at 16 rows, 64 rows 42.9).  Eight waves share K, sixteen where
+// few row blocks have a long one (17408 to 5120 at 1 row: 11.3 us, 15.5 with
+// eight; at 16 rows 18.9 and 18.3).
 static void q4_defaults(hb_desc* d) {
     if (!d->mv_m) d->mv_m = d->rows_of == HB_ROWS_DENSE ? 1 : 16;
     const uint32_t nt = cdiv(d->n, 16), kt = cdiv(d->k, 128);
@@ -73,7 +75,7 @@ static void q4_defaults(hb_desc* d) {
     }
     if (!d->rows) d->rows = nt > 4096 ? (d->mv_m > 8 ? 128 : 64) : nt > 256 || swi ? 32 : 16;
     if (!d->split) {
-        d->split = d->rows == 16 ? 16 : 8;
+        d->split = d->rows == 16 || (kt >= 64 && nt <= 512) ? 16 : 8;
         while (d->split > kt || (d->mv_waves && d->split > d->mv_waves)) d->split /= 2;
         if (!d->split) d->split = 1;
     }
