@@ -116,6 +116,14 @@ hb_desc with_defaults(const hb_desc& in) {
     return d;
 }
 
+// block_norm's threads: a 16-byte chunk of the row each, two past 512 (2048
+// rows of 5120: 18.5 us, one each 19.9; 2560: one each 10.6, two 10.9), up to
+// 1024 threads.
+static uint32_t norm_threads(uint32_t n) {
+    const uint32_t cells = cdiv(n, 8);
+    return cdiv(cells <= 512 ? cells : cells <= 2048 ? cdiv(cells, 2) : 1024, 64) * 64;
+}
+
 static int emit_kind(const hb_desc& d, Emitted* e) {
     char name[256];
     e->defines.clear();
@@ -456,7 +464,7 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             return HB_OK;
         }
         case HB_KIND_BLOCK_NORM: {
-            const uint32_t gate = d.form >> 4, cells = cdiv(d.n, 8);
+            const uint32_t gate = d.form >> 4;
             if (!d.n || d.n > 32768) return fail(HB_ERR_UNSUPPORTED, "block_norm: rows of 1 to 32768");
             if (d.form & ~0x37u) return fail(HB_ERR_INVALID, "block_norm: parts out of range");
             const bool post = d.form & HB_NORM_POST, pre = d.form & HB_NORM_PRE, scales = d.form & HB_NORM_SCALES;
@@ -464,10 +472,7 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
                      post ? "_post" : "", pre ? "_pre" : "", scales ? "_sc" : "", gate);
             e->name = name;
             e->source = "block_norm.hip";
-            // A 16-byte chunk of the row a thread, two past 512 (2048 rows of
-            // 5120: 18.5 us, one each 19.9; 2560: one each 10.6, two 10.9),
-            // up to 1024 threads.
-            e->threads = cdiv(cells <= 512 ? cells : cells <= 2048 ? cdiv(cells, 2) : 1024, 64) * 64;
+            e->threads = norm_threads(d.n);
             e->nbind = 3 + (post ? 1 : 0) + (pre ? 2 : 0) + (scales ? 1 : 0) + (gate ? 1 : 0);
             e->defines = {D("HB_D", d.n),       D("HB_THREADS", e->threads), D("HB_EPS", d.eps_bits),
                           D("HB_PLUS1", d.plus_one ? 1 : 0), D("HB_POST", post), D("HB_PRE", pre),
@@ -556,7 +561,8 @@ uint32_t groups_of(const hb_desc& d, uint32_t m) {
             if (d.rows_of == HB_ROWS_DENSE) return wgs;
             // Tiles with rows: no more than pairs, nor than the table holds.
             const uint64_t pairs = (uint64_t)m * d.top_k;
-            return (uint32_t)((pairs < d.tiles ? pairs : d.tiles) * wgs);
+            const uint64_t groups = (pairs < d.tiles ? pairs : d.tiles) * wgs;
+            return groups < 0xffffffffu ? (uint32_t)groups : 0xffffffffu;
         }
         case HB_KIND_MOE_OUT:
         case HB_KIND_RMSNORM:
@@ -710,13 +716,19 @@ int check_bindings(const hb_desc& d, const uint64_t* s, uint32_t nbind, uint32_t
     }
     if (m == 0) return fail(HB_ERR_INVALID, "0 rows");
     if (d.kind >= HB_KIND_Q4_QUANTIZE && d.kind <= HB_KIND_BLOCK_NORM) {
-        // First what keeps the byte counts and the grid within range.
+        // First what keeps the byte counts and the grid (fewer than 2^32
+        // threads) within range.
         if (d.kind == HB_KIND_MATVEC_Q4) {
             const bool dense = d.rows_of == HB_ROWS_DENSE;
             if (dense && m > d.mv_m)
                 return fail(HB_ERR_INVALID, "matvec_q4 of " + std::to_string(m) + " rows: 1.." + std::to_string(d.mv_m));
             if (!dense && m > d.rows_max) return fail(HB_ERR_INVALID, "m beyond the kernel's rows_max");
-        } else if (d.kind != HB_KIND_BLOCK_NORM && m * q4_tiles(d.k, d.n) >= (1u << 26)) {
+            if ((uint64_t)groups_of(d, m) * 64 * d.mv_waves >> 32)
+                return fail(HB_ERR_UNSUPPORTED, "matvec_q4: too many workgroups in one launch");
+        } else if (d.kind == HB_KIND_BLOCK_NORM) {
+            if ((uint64_t)m * norm_threads(d.n) >> 32)
+                return fail(HB_ERR_UNSUPPORTED, "block_norm: too many rows in one launch");
+        } else if (m * q4_tiles(d.k, d.n) >= (1u << 26)) {
             return fail(HB_ERR_UNSUPPORTED, "q4: too many matrices in one launch");
         }
         const AccessList l = accesses(d, m);

@@ -28,7 +28,7 @@ namespace {
 // Every key of the reference's --tune, with its default, in the order of
 // Tune::summary.  The keys of this path act (prefill.block, gemm.*, moe.*,
 // mv.*, auto.heat, pf.fswi); the others are accepted and echoed, as the
-// reference's subsystems they name (attention, DeltaNet, decode fusions, Q4)
+// reference's subsystems they name (attention, DeltaNet, decode fusions, q4.fuse)
 // are not part of this library.
 struct Key {
     const char* name;

@@ -15,6 +15,7 @@ argument meaning:
                    2119), moe_sort / moe_sort_atomic / moe_gather
                    (prefill.rs:1315, 1450, 579): here they return a Desc,
                    which Gpu.pipeline compiles (hiprtc, gfx950).
+                   4-bit weights (q4_*, matvec_q4, experts_q4) and block_norm.
   - Engine         the kernel-selection part of QwenEngine (qwen.rs): gemm,
                    mv_full, expert_pipes, Tune.
 

@@ -2,7 +2,8 @@
  * herbert_hip.h -- C ABI of the MI355X (gfx950) bf16 matrix-multiplication
  * path of herbert-metal-bf16: the prefill block GEMM, the decode matvec and
  * the MoE expert grouped GEMM with its route, sort, gather, SwiGLU and
- * combine.  Plain pointers, sizes and integer status codes; no C++ or torch
+ * combine; the decode matvec and the experts over weights of 4 bits; the
+ * norms around a block.  Plain pointers, sizes and integer status codes; no C++ or torch
  * types cross it.  One context per device; a context is used by one host
  * thread at a time (the reference's `Gpu` is not Send either), and work is
  * ordered on the context's one HIP stream.

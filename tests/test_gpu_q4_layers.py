@@ -230,6 +230,41 @@ def test_moe_layer(gpu, rows, group):
             gpu.free(b)
 
 
+def test_moe_run_with_the_swiglu_apart(gpu):
+    """A gate|up that writes its sums (Out::Bf16), then swiglu_slots: h from
+    the rounded sums, everything else as in the fused run."""
+    E, K, H, MI, rows, group = 64, 4, 256, 128, 21, 64
+    rng = np.random.default_rng(12)
+    gu, gs = q4.random_codes(rng, E * 2 * MI, H, group)
+    dn, ds = q4.random_codes(rng, E * H, MI, group)
+    wg, wd = q4.pack(gpu, gu, gs, H, 2 * MI, group, E), q4.pack(gpu, dn, ds, MI, H, group, E)
+    with hb.Engine(gpu, "") as e:
+        layer = hb.MoeLayer(gpu, e, E, K, H, MI, rows, wg, wd, scores=hb.normal_bf16(1, 1.0, (rows, E)),
+                            x=hb.normal_bf16(2, 1.0, (rows, H)), q4_group=group)
+    b, pairs = layer.buf, rows * K
+    try:
+        layer.kernels[1] = gpu.pipeline(hb.experts_q4(H, 2 * MI, hb.Out.Bf16, group, hb.Rows.Gather, K, E, rows))
+        layer.run()
+        gpu.sync()
+        egu = gpu.download(b["egu"], np.uint16, pairs * 2 * MI).reshape(pairs, 2 * MI)
+        hh = gpu.download(b["ehb"], np.uint16, pairs * MI).reshape(pairs, MI)
+        assert np.array_equal(hh, orc.swiglu(egu, MI))
+        route = gpu.download(b["route"], np.uint32, rows * 2 * K).reshape(rows, 2 * K)
+        lst = gpu.download(b["list"], np.uint32, pairs)
+        x, ey = gpu.download(b["x"], np.uint16, rows * H).reshape(rows, H), gpu.download(b["ey"], np.uint16, pairs * H).reshape(pairs, H)
+        e = route[:, :K].reshape(-1)[lst]
+        for ex in np.unique(e):
+            p = np.flatnonzero(e == ex)
+            for got, xf, c, s in ((egu[p], f64(x[lst[p] // K]), gu[ex * 2 * MI:][:2 * MI], gs[ex * 2 * MI:][:2 * MI]),
+                                  (ey[lst[p]], f64(hh[p]), dn[ex * H:][:H], ds[ex * H:][:H])):
+                q4.close(got, xf @ q4.values(c, s, group).T, q4.sum_bound(xf, c, s, group), "expert %d" % ex)
+        assert np.array_equal(gpu.download(b["out"], np.uint16, rows * H).reshape(rows, H), orc.combine(ey, route, K, H))
+    finally:
+        layer.free()
+        gpu.free(wg)
+        gpu.free(wd)
+
+
 def test_moe_run_refuses(gpu):
     """Kernels that do not belong together: a sort of other tiles, the gate|up
     and down rows swapped, one bf16 and one 4-bit kernel, a gather kernel."""

@@ -126,6 +126,11 @@ def test_refused_norm_launches(hb, gpu):
             gpu.launch(k, [bad.get(i, v) for i, v in enumerate(good)], m)
     with pytest.raises(hb.HerbertError, match="0 rows"):
         gpu.launch(k, good, 0)
+    with pytest.raises(hb.HerbertError, match="too many rows"):
+        gpu.launch(k, good, 1 << 26)
+    many = gpu.pipeline(hb.experts_q4(8, 1 << 24, hb.Out.Bf16, 32, hb.Rows.Gather, 8, 64, 1 << 20))
+    with pytest.raises(hb.HerbertError, match="too many workgroups"):
+        gpu.launch(many, [R(x)] * 6, 1 << 20)
 
 
 def test_refused_quantize_launches(hb, gpu):
