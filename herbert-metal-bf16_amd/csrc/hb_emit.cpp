@@ -41,9 +41,11 @@ static uint64_t q4_tiles(uint32_t k, uint32_t n) { return ((uint64_t)k + 127) / 
 static uint64_t q4_bytes(uint32_t k, uint32_t n, uint32_t group) {
     return q4_tiles(k, n) * 1024 + ((uint64_t)k + 127) / 128 * (((uint64_t)n + 63) / 64) * (16384 / group);
 }
-// k and n within what keeps every byte count of a launch in 64 bits.
+// k and n within what keeps every byte count of a launch in 64 bits and the
+// kernels' tile numbers in 32.
 static bool q4_shape(uint32_t k, uint32_t n, uint32_t group) {
-    return k && n && k % 8 == 0 && k <= (1u << 20) && n <= (1u << 24) && (group == 32 || group == 64 || group == 128);
+    return k && n && k % 8 == 0 && k <= (1u << 20) && n <= (1u << 24) && q4_tiles(k, n) < (1u << 30) &&
+           (group == 32 || group == 64 || group == 128);
 }
 
 // The 4-bit matvec's form by its row tiles (16 W rows) and K tiles (128 K).
@@ -413,7 +415,7 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
         case HB_KIND_Q4_PACK:
         case HB_KIND_Q4_DEQUANTIZE: {
             if (!q4_shape(d.k, d.n, d.bk))
-                return fail(HB_ERR_UNSUPPORTED, "q4: K a multiple of 8 up to 2^20, N up to 2^24, groups of 32, 64 or 128");
+                return fail(HB_ERR_UNSUPPORTED, "q4: K a multiple of 8 up to 2^20, N up to 2^24, K N below 2^41, groups of 32, 64 or 128");
             const uint32_t op = d.kind - HB_KIND_Q4_QUANTIZE + 1;
             snprintf(name, sizeof name, "q4_%s_%ux%u_g%u", op == 1 ? "quantize" : op == 2 ? "pack" : "dequantize",
                      d.k, d.n, d.bk);
@@ -430,7 +432,7 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
                 return fail(HB_ERR_INVALID, "matvec_q4: out / rows_of out of range");
             if (!q4_shape(d.k, d.n, d.bk))
                 return fail(HB_ERR_UNSUPPORTED,
-                            "matvec_q4: K a multiple of 8 up to 2^20, N up to 2^24, groups of 32, 64 or 128");
+                            "matvec_q4: K a multiple of 8 up to 2^20, N up to 2^24, K N below 2^41, groups of 32, 64 or 128");
             if (swi && d.n % 32)
                 return fail(HB_ERR_UNSUPPORTED, "matvec_q4 Out::Swiglu: gate and up rows each a multiple of 16");
             if (d.mv_m > 16) return fail(HB_ERR_UNSUPPORTED, "matvec_q4: m <= 16");

@@ -187,7 +187,7 @@ HB_DEV void rows_of_w(const unsigned char* __restrict__ W, const u16* __restrict
 #pragma unroll
             for (u32 i = 0; i < XI; i++) {
                 const u32 c = 4 * i + quad;
-                if (C >= 4 || quad < C) xt[c * 16 + (col ^ c)] = in_k ? t.x[u][i] : u32x4{0, 0, 0, 0};
+                xt[c * 16 + (col ^ c)] = in_k ? t.x[u][i] : u32x4{0, 0, 0, 0};
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();

@@ -51,6 +51,8 @@ def test_q4_bytes(hb):
     (lambda hb: hb.experts_q4(128, 64, hb.Out.Bf16, 32, hb.Rows.Gather, 8, 64, 1 << 26), "pairs"),
     (lambda hb: hb.matvec_q4((1 << 20) + 8, 16, hb.Out.Bf16), "K a multiple of 8 up to"),
     (lambda hb: hb.matvec_q4(128, (1 << 24) + 1, hb.Out.Bf16), "N up to"),
+    (lambda hb: hb.matvec_q4(1 << 20, 1 << 24, hb.Out.Bf16), "K N below"),
+    (lambda hb: hb.q4_quantize(1 << 20, 1 << 24), "K N below"),
     (lambda hb: hb.q4_quantize(4, 16), "K a multiple of 8"),
     (lambda hb: hb.q4_pack(8, 16, 31), "groups"),
     (lambda hb: hb.q4_dequantize(8, 0), "q4"),
