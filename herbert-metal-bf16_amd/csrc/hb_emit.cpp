@@ -68,9 +68,11 @@ static void q4_defaults(hb_desc* d) {
         // tokens 13.7 against 14.5, 1 token 3.8 against 4.8).
         const uint64_t wgs = (uint64_t)d->rows_max * d->top_k * (swi ? nt / 2 : nt / 2 + nt % 2);
         if (!d->rows) d->rows = wgs >= 8192 ? 64 : 32;
-        if (!d->split) d->split = kt >= 4 ? 4 : kt >= 2 ? 2 : 1;
-        if (d->mv_waves && d->split > d->mv_waves) d->split = d->mv_waves;
-        if (!d->mv_waves) d->mv_waves = 4;
+        if (!d->split) {
+            d->split = kt >= 4 ? 4 : kt >= 2 ? 2 : 1;
+            if (d->mv_waves && d->split > d->mv_waves) d->split = d->mv_waves;
+        }
+        if (!d->mv_waves) d->mv_waves = d->split < 4 ? 4 : d->split;
         const uint32_t per = cdiv(kt, d->split);
         if (!d->unroll) d->unroll = d->rows >= 64 ? 1 : per >= 3 ? 4 : per;
         return;
