@@ -1680,7 +1680,8 @@ int hb_engine_pin(hb_engine* e, const char* text) {
         } else if (f[0] == "mv") {
             int32_t k;
             if ((rc = kernel_at(2, &k))) return rc;
-            if (k < 0) return bad("no matvec kernel");
+            // A 4-bit matvec takes as many bindings, and would read W as codes.
+            if (k < 0 || kernel_desc(e->g, k)->kind != HB_KIND_MATVEC) return bad("no matvec kernel");
             e->mv_pick[f[1]] = *kernel_desc(e->g, k);
         } else if (f[0] == "mv_q4") {
             int32_t k;
@@ -1696,6 +1697,12 @@ int hb_engine_pin(hb_engine* e, const char* text) {
             if (!Tune::parse_u32(f[2], &ep.bm, &err)) return bad("rows " + f[2]);
             for (int i = 0; i < 4; i++)
                 if ((rc = kernel_at(3 + 2 * i, &ep.kernels[i]))) return rc;
+            // The experts' 4-bit kernels bind what the grouped GEMMs bind.
+            for (int i = 1; i < 3; i++) {
+                const hb_desc* d = kernel_desc(e->g, ep.kernels[i]);
+                if (!d || (d->kind != HB_KIND_GEMM && (i == 2 || d->kind != HB_KIND_GEMM_SWIGLU)))
+                    return bad("no grouped GEMM of bf16 weights");
+            }
             e->experts_pick[f[1]] = ep;
         } else {
             return bad("unknown kind " + f[0]);

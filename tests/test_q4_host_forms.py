@@ -51,3 +51,35 @@ def test_experts_splits_compile(monkeypatch, rows, split):
     monkeypatch.setenv("HB_CACHE_DIR", "")
     d = experts(herbert_hip, rows=rows, split=split, unroll=1)
     herbert_hip.check(herbert_hip.lib.hb_kernel_precompile(ctypes.byref(d)))
+
+
+def pin_text(hb, gpu, desc):
+    return "%s\t%s" % (gpu.kernel_name(gpu.pipeline(desc)), " ".join(str(getattr(desc, f)) for f in hb._DESC_FIELDS))
+
+
+def test_pins_of_bf16_choices_take_no_4bit_kernel(hb, gpu):
+    """A 4-bit kernel binds as much as its bf16 counterpart, so only the pin can
+    tell that it would read bf16 weights as codes."""
+    mv = hb.matvec(2048, 64, hb.Out.Bf16)
+    mv_q4 = hb.matvec_q4(2048, 64, hb.Out.Bf16)
+    sort = hb.Desc(kind=hb.Kind.SORT, experts=64, top_k=8, bm=16, rows_max=4)
+    tile = dict(top_k=8, experts=64, bm=16, tiles=hb.moe_tiles(4, 8, 64, 16), wm=1, wn=4, bn=128, bk=64, rows_max=4)
+    gu = hb.gemm_mma_rows(2048, 1024, hb.Out.Bf16, rows_of=hb.Rows.Gather, **tile)
+    dn = hb.gemm_mma_rows(512, 2048, hb.Out.Bf16, rows_of=hb.Rows.Scatter, **tile)
+    gu_q4 = hb.experts_q4(2048, 1024, hb.Out.Swiglu, 32, hb.Rows.Gather, 8, 64, 4)
+    dn_q4 = hb.experts_q4(512, 2048, hb.Out.Bf16, 32, hb.Rows.Scatter, 8, 64, 4)
+
+    def line(*descs):
+        return "experts\tkey\t16\t%s\t-\t-\n" % "\t".join(pin_text(hb, gpu, d) for d in descs)
+
+    with hb.Engine(gpu, "") as e:
+        good = "mv\t2048x64 Bf16 m1\t%s\n" % pin_text(hb, gpu, mv) + line(sort, gu, dn)
+        e.pin(good)
+        text = e.picks()
+        assert [gpu.kernel_name(gpu.pipeline(d)) in text for d in (mv, sort, gu, dn)] == [True] * 4
+        with pytest.raises(hb.HerbertError, match="no matvec kernel"):
+            e.pin("mv\t2048x64 Bf16 m1\t%s\n" % pin_text(hb, gpu, mv_q4))
+        for descs in ((sort, gu_q4, dn_q4), (sort, gu_q4, dn), (sort, gu, dn_q4)):
+            with pytest.raises(hb.HerbertError, match="no grouped GEMM"):
+                e.pin(line(*descs))
+        assert e.picks() == text
