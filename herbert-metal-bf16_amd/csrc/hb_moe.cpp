@@ -28,6 +28,8 @@ int moe_experts_run(hb_gpu* g, const int32_t kernels[4], int32_t swiglu, int32_t
     if (q4 && (sd->bm != 16 || gd->rows_of != HB_ROWS_GATHER || dd->rows_of != HB_ROWS_SCATTER || gather >= 0))
         return fail(HB_ERR_INVALID, "moe experts in 4 bits: a sort of 16-row tiles, gathered gate|up rows, "
                                     "scattered down rows, no gather kernel");
+    // Its rows would be half as long as the combine reads them.
+    if (writes_swiglu(*dd)) return fail(HB_ERR_INVALID, "moe experts: a down kernel that writes a SwiGLU");
     const bool fused = writes_swiglu(*gd);
     if (!fused && !kernel_desc(g, swiglu))
         return fail(HB_ERR_INVALID, "moe experts: the gate|up GEMM needs the swiglu_slots kernel");

@@ -83,3 +83,19 @@ def test_pins_of_bf16_choices_take_no_4bit_kernel(hb, gpu):
             with pytest.raises(hb.HerbertError, match="no grouped GEMM"):
                 e.pin(line(*descs))
         assert e.picks() == text
+
+
+def test_experts_run_takes_no_swiglu_down(hb, gpu):
+    """A down kernel of Out::Swiglu writes rows of half its W rows."""
+    E, K, H, MI, rows = 64, 4, 256, 128, 8
+    wg, wd = gpu.alloc(E * hb.q4_bytes(H, 2 * MI)), gpu.alloc(E * hb.q4_bytes(MI, H))
+    with hb.Engine(gpu, "") as e:
+        layer = hb.MoeLayer(gpu, e, E, K, H, MI, rows, wg, wd, q4_group=32)
+
+    def run():
+        return hb.lib.hb_moe_experts_run(gpu.h, (ctypes.c_int32 * 4)(*layer.kernels), layer.swiglu_k, layer.combine_k,
+                                         ctypes.byref(layer.io), hb.r(layer.buf["out"]), rows)
+
+    assert run() == 0, hb.last_error()
+    layer.kernels[2] = gpu.pipeline(hb.experts_q4(MI, H, hb.Out.Swiglu, 32, hb.Rows.Scatter, K, E, rows))
+    assert run() == hb.ERR_INVALID and "down" in hb.last_error()
