@@ -42,7 +42,7 @@ int resolve(hb_gpu* g, const hb_range& r, char** ptr, uint64_t* size) {
     if (r.buf >= g->bufs.size() || !g->bufs[r.buf].live)
         return fail(HB_ERR_INVALID, "range on buffer " + std::to_string(r.buf) + ": no such buffer");
     const Buffer& b = g->bufs[r.buf];
-    if (r.offset > b.size || (r.size && r.offset + r.size > b.size))
+    if (r.offset > b.size || r.size > b.size - r.offset)
         return fail(HB_ERR_INVALID, "range [" + std::to_string(r.offset) + ", +" +
                                         std::to_string(r.size) + ") outside buffer " +
                                         std::to_string(r.buf) + " of " + std::to_string(b.size) +

@@ -99,3 +99,14 @@ def test_experts_run_takes_no_swiglu_down(hb, gpu):
     assert run() == 0, hb.last_error()
     layer.kernels[2] = gpu.pipeline(hb.experts_q4(MI, H, hb.Out.Swiglu, 32, hb.Rows.Scatter, K, E, rows))
     assert run() == hb.ERR_INVALID and "down" in hb.last_error()
+
+
+def test_a_range_past_64_bits_is_refused(hb, gpu):
+    """An offset and a size whose sum wraps lie outside the buffer, however
+    small the sum is."""
+    k = gpu.pipeline(hb.matvec_q4(128, 32, hb.Out.F32, mv_m=1))
+    w, x, y = gpu.alloc(hb.q4_bytes(128, 32)), gpu.alloc(256), gpu.alloc(128)
+    gpu.launch(k, [hb.r(w), hb.r(x), hb.r(y)], 1)
+    for bad in (hb.r(y, 4, 2 ** 64 - 4), hb.r(y, 64, 2 ** 64 - 32), hb.r(y, 0, 129), hb.r(y, 129)):
+        with pytest.raises(hb.HerbertError, match="outside buffer"):
+            gpu.launch(k, [hb.r(w), hb.r(x), bad], 1)
