@@ -85,7 +85,8 @@ uint64_t workspace_of(const hb_desc& d, uint32_t m);
 
 struct hb_gpu {
     int device = 0;
-    hipStream_t stream = nullptr;
+    // The stream all work goes to, and the context's own one (hb_set_stream).
+    hipStream_t stream = nullptr, own = nullptr;
     hipEvent_t ev0 = nullptr, ev1 = nullptr;
     std::vector<hb::Buffer> bufs;
     std::vector<hb::Kernel> kernels;

@@ -52,6 +52,10 @@ int resolve(hb_gpu* g, const hb_range& r, char** ptr, uint64_t* size) {
     return HB_OK;
 }
 
+// HIP's null stream is the current device's: the context's, where its work
+// goes there.
+static hipError_t here(hb_gpu* g) { return g->stream ? hipSuccess : hipSetDevice(g->device); }
+
 static const char* source_text(const std::string& name) {
     for (const auto& s : kSources)
         if (name == s.name) return s.text;
@@ -272,6 +276,7 @@ static int launch_one(hb_gpu* g, const Kernel& k, void** ptrs, uint32_t nptr, ui
     void* args[12];
     for (uint32_t i = 0; i < nptr; i++) args[i] = &ptrs[i];
     args[nptr] = &m;
+    HB_HIP(here(g));
     HB_HIP(hipModuleLaunchKernel(k.fn, groups, 1, 1, k.em.threads, 1, 1, 0, g->stream, args,
                                  nullptr));
     return HB_OK;
@@ -403,11 +408,12 @@ int hb_open(int device, hb_gpu** out) {
              p.multiProcessorCount, p.totalGlobalMem / 1073741824.0, p.gcnArchName,
              (size_t)p.sharedMemPerBlock / 1024);
     g->summary = buf;
-    if ((e = hipStreamCreateWithFlags(&g->stream, hipStreamNonBlocking)) != hipSuccess ||
+    if ((e = hipStreamCreateWithFlags(&g->own, hipStreamNonBlocking)) != hipSuccess ||
         (e = hipEventCreate(&g->ev0)) != hipSuccess || (e = hipEventCreate(&g->ev1)) != hipSuccess) {
         delete g;
         return hip_fail(e, "stream/event");
     }
+    g->stream = g->own;
     // The static scratch of hb_moe_experts_run_static on this device (the
     // device is current): its address, once per device.
     int rc = static_scratch(device, &g->scratch);
@@ -431,7 +437,7 @@ void hb_close(hb_gpu* g) {
     if (g->ws) hipFree(g->ws);
     hipEventDestroy(g->ev0);
     hipEventDestroy(g->ev1);
-    hipStreamDestroy(g->stream);
+    hipStreamDestroy(g->own);
     delete g;
 }
 
@@ -454,6 +460,7 @@ int hb_alloc(hb_gpu* g, uint64_t bytes, hb_buf* out) {
 int hb_free(hb_gpu* g, hb_buf buf) {
     if (buf >= g->bufs.size() || !g->bufs[buf].live)
         return fail(HB_ERR_INVALID, "hb_free: no buffer " + std::to_string(buf));
+    HB_HIP(here(g));
     HB_HIP(hipStreamSynchronize(g->stream));
     HB_HIP(hipFree(g->bufs[buf].ptr));
     g->bufs[buf].live = false;
@@ -475,6 +482,7 @@ int hb_upload(hb_gpu* g, hb_buf buf, uint64_t offset, const void* src, uint64_t 
     uint64_t n;
     int rc = resolve(g, r, &p, &n);
     if (rc) return rc;
+    HB_HIP(here(g));
     HB_HIP(hipMemcpyAsync(p, src, bytes, hipMemcpyHostToDevice, g->stream));
     HB_HIP(hipStreamSynchronize(g->stream));
     return HB_OK;
@@ -486,6 +494,7 @@ int hb_download(hb_gpu* g, hb_buf buf, uint64_t offset, void* dst, uint64_t byte
     uint64_t n;
     int rc = resolve(g, r, &p, &n);
     if (rc) return rc;
+    HB_HIP(here(g));
     HB_HIP(hipMemcpyAsync(dst, p, bytes, hipMemcpyDeviceToHost, g->stream));
     HB_HIP(hipStreamSynchronize(g->stream));
     return HB_OK;
@@ -498,6 +507,7 @@ int hb_copy(hb_gpu* g, hb_range dst, hb_range src) {
     if (rc || (rc = resolve(g, src, &ps, &ns))) return rc;
     if (nd != ns) return fail(HB_ERR_INVALID, "hb_copy: ranges of different sizes");
     if ((pd < ps + ns) && (ps < pd + nd) && nd) return fail(HB_ERR_INVALID, "hb_copy: ranges overlap");
+    HB_HIP(here(g));
     HB_HIP(hipMemcpyAsync(pd, ps, nd, hipMemcpyDeviceToDevice, g->stream));
     return HB_OK;
 }
@@ -523,6 +533,7 @@ int hb_zero(hb_gpu* g, hb_buf buf, uint64_t offset, uint64_t bytes) {
         if (groups > 0x7fffffffull) return fail(HB_ERR_INVALID, "hb_zero: too large");
         void* ptr = p;
         void* args[2] = {&ptr, &n};
+        HB_HIP(here(g));
         HB_HIP(hipModuleLaunchKernel(g->zero_kernel.fn, (uint32_t)groups, 1, 1, 256, 1, 1, 0,
                                      g->stream, args, nullptr));
     }
@@ -660,6 +671,7 @@ int hb_time_each(hb_gpu* g, const hb_op* ops, uint32_t nops, uint32_t reps, doub
     std::vector<Ready> ready;
     int prc = prepare(g, ops, nops, &ready);
     if (prc) return prc;
+    HB_HIP(here(g));
     if (!op_seconds) {
         HB_HIP(hipEventRecord(g->ev0, g->stream));
         for (uint32_t r = 0; r < reps; r++)
@@ -727,11 +739,16 @@ int hb_graph_record(hb_gpu* g, const hb_op* ops, uint32_t nops, hb_graph** out) 
     int rc = prepare(g, ops, nops, &ready);  // sizes the split-K workspace before the capture
     if (rc) return rc;
     HB_HIP(hipSetDevice(g->device));
-    HB_HIP(hipStreamBeginCapture(g->stream, hipStreamCaptureModeThreadLocal));
+    // On the context's own stream, whichever its work goes to: the null stream
+    // cannot be captured, and a caller's may be under a capture of its own.
+    HB_HIP(hipStreamBeginCapture(g->own, hipStreamCaptureModeThreadLocal));
+    const hipStream_t to = g->stream;
+    g->stream = g->own;
     for (auto& x : ready)
         if ((rc = launch_raw(g, *x.k, x.ptrs, x.n, x.m, x.groups))) break;
+    g->stream = to;
     hipGraph_t graph = nullptr;
-    hipError_t he = hipStreamEndCapture(g->stream, &graph);
+    hipError_t he = hipStreamEndCapture(g->own, &graph);
     if (rc || he != hipSuccess) {
         if (graph) hipGraphDestroy(graph);
         return rc ? rc : hip_fail(he, "hipStreamEndCapture");
@@ -751,12 +768,14 @@ int hb_graph_record(hb_gpu* g, const hb_op* ops, uint32_t nops, hb_graph** out) 
 }
 
 int hb_graph_launch(hb_graph* gr, uint32_t reps) {
+    HB_HIP(here(gr->g));
     for (uint32_t i = 0; i < reps; i++) HB_HIP(hipGraphLaunch(gr->exec, gr->g->stream));
     return HB_OK;
 }
 
 int hb_graph_time(hb_graph* gr, uint32_t reps, double* seconds) {
     hb_gpu* g = gr->g;
+    HB_HIP(here(g));
     HB_HIP(hipEventRecord(g->ev0, g->stream));
     for (uint32_t i = 0; i < reps; i++) HB_HIP(hipGraphLaunch(gr->exec, g->stream));
     HB_HIP(hipEventRecord(g->ev1, g->stream));
@@ -769,6 +788,7 @@ int hb_graph_time(hb_graph* gr, uint32_t reps, double* seconds) {
 
 void hb_graph_free(hb_graph* gr) {
     if (!gr) return;
+    (void)here(gr->g);
     hipStreamSynchronize(gr->g->stream);
     if (gr->exec) hipGraphExecDestroy(gr->exec);
     if (gr->graph) hipGraphDestroy(gr->graph);
@@ -777,8 +797,29 @@ void hb_graph_free(hb_graph* gr) {
 }
 
 int hb_sync(hb_gpu* g) {
+    HB_HIP(here(g));
     HB_HIP(hipStreamSynchronize(g->stream));
     return HB_OK;
 }
+
+}  // extern "C"
+
+// All work from here on to `to`.  What is queued is waited for, so that the
+// buffers and the workspace have one order of use; the event's record fails
+// for a stream that is none of this device's.
+static int change_stream(hb_gpu* g, hipStream_t to) {
+    if (to == g->stream) return HB_OK;
+    HB_HIP(hipSetDevice(g->device));
+    HB_HIP(hipEventRecord(g->ev0, to));
+    HB_HIP(hipStreamSynchronize(g->stream));
+    g->stream = to;
+    return HB_OK;
+}
+
+extern "C" {
+
+int hb_set_stream(hb_gpu* g, void* stream) { return change_stream(g, (hipStream_t)stream); }
+
+int hb_own_stream(hb_gpu* g) { return change_stream(g, g->own); }
 
 }  // extern "C"

@@ -182,6 +182,8 @@ lib.hb_download.argtypes = [_P, _u32, _u64, _P, _u64]
 lib.hb_zero.argtypes = [_P, _u32, _u64, _u64]
 lib.hb_copy.argtypes = [_P, Range, Range]
 lib.hb_buffer_ptr.argtypes = [_P, _u32, ctypes.POINTER(_P)]
+lib.hb_set_stream.argtypes = [_P, _P]
+lib.hb_own_stream.argtypes = [_P]
 lib.hb_kernel_build.argtypes = [_P, ctypes.POINTER(Desc), ctypes.POINTER(_i32)]
 lib.hb_kernel_name.argtypes = [_P, _i32]
 lib.hb_kernel_name.restype = ctypes.c_char_p
@@ -374,6 +376,12 @@ def block_norm(d, eps, plus_one=False, post=False, pre=True, gate=Gate.Off, scal
                 form=(1 if post else 0) | (2 if pre else 0) | (4 if scales else 0) | int(gate))
 
 
+def _hip_runtimes():
+    """The files of the HIP runtimes that this process has loaded."""
+    with open("/proc/self/maps") as f:
+        return {line.split(None, 5)[5].strip() for line in f if "libamdhip64" in line}
+
+
 class Gpu:
     """Gpu (src/metal/gpu.rs): one HIP device, its stream, buffers and kernels."""
 
@@ -400,6 +408,19 @@ class Gpu:
 
     def summary(self):
         return lib.hb_device_summary(self.h).decode()
+
+    def set_stream(self, stream=None):
+        """The stream of all work from here on (hb_set_stream): a hipStream_t as a
+        number, 0 for HIP's null stream, as torch's Stream.cuda_stream gives it;
+        None for the context's own.  Tensors over the context's buffers are in
+        order with its launches where both are on one stream; on the context's
+        own, sync() comes before they are read.  A process that imports torch
+        imports it before this package, or the two bring a HIP runtime each,
+        whose streams mean nothing to the other: refused."""
+        if stream is not None and len(_hip_runtimes()) > 1:
+            raise HerbertError(HB_ERR_INVALID, "set_stream: two HIP runtimes in this process (%s): import torch before "
+                               "herbert_hip" % ", ".join(sorted(_hip_runtimes())))
+        check(lib.hb_own_stream(self.h) if stream is None else lib.hb_set_stream(self.h, _P(int(stream))))
 
     # memory
     def alloc(self, nbytes):

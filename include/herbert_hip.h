@@ -6,7 +6,8 @@
  * norms around a block.  Plain pointers, sizes and integer status codes; no C++ or torch
  * types cross it.  One context per device; a context is used by one host
  * thread at a time (the reference's `Gpu` is not Send either), and work is
- * ordered on the context's one HIP stream.
+ * ordered on the context's one HIP stream, its own or a caller's
+ * (hb_set_stream).
  *
  * Every entry point cites the reference interface it replaces, as
  * path:line under src/ of xigh/herbert-metal-bf16.
@@ -43,6 +44,22 @@ void hb_close(hb_gpu *gpu);
 /* Gpu::summary (metal/gpu.rs:108): "name, CUs, memory, arch". */
 const char *hb_device_summary(hb_gpu *gpu);
 
+/* The stream that the context's work goes to from here on: a hipStream_t of
+ * the context's device, NULL for HIP's null stream; hb_own_stream: the
+ * context's own again.  The context opens on its own stream, which waits for
+ * no other and which no other waits for: a caller that reads or writes the
+ * buffers' memory (hb_buffer_ptr) by other means either runs the context on
+ * the stream of those, in whose order launches, copies and replays then stand,
+ * or calls hb_sync before it reads and waits for its own writes before it
+ * launches.  A change waits for the work queued before it; it is made while
+ * neither stream is being captured.  Launches on a stream under capture are
+ * captured with it (the calls that wait, hb_upload, hb_download, hb_free,
+ * hb_time and hb_sync, are not for that).  The stream must live until the
+ * context is changed to another or closed.  No counterpart in the reference,
+ * whose buffers the CPU shares. */
+int hb_set_stream(hb_gpu *gpu, void *stream);
+int hb_own_stream(hb_gpu *gpu);
+
 /* ---- memory: Gpu::alloc / alloc_with, Buffer, Range (metal/gpu.rs:59-67,
  * 150-157).  The context owns every buffer until hb_free or hb_close. ---- */
 typedef uint32_t hb_buf;
@@ -65,7 +82,8 @@ int hb_zero(hb_gpu *gpu, hb_buf buf, uint64_t offset, uint64_t bytes);
  * whose buffers are shared with the CPU; for callers that stage device
  * buffers, and the plain copy that calibrates the traffic counters. */
 int hb_copy(hb_gpu *gpu, hb_range dst, hb_range src);
-/* Device address of a buffer (for callers that bring their own kernels). */
+/* Device address of a buffer (for callers that bring their own kernels;
+ * hb_set_stream says in which order those stand to the context's). */
 int hb_buffer_ptr(hb_gpu *gpu, hb_buf buf, void **ptr);
 
 /* ---- kernel descriptors: the emitter functions of the reference
