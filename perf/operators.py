@@ -227,6 +227,10 @@ def prepare(case, seed):
 
 def _prepare_own(case, v):
     hb, gpu, eng = _open()
+    # One stream for torch and the library, as a program that holds tensors
+    # over the library's buffers has it: what run gives is in order with what
+    # torch does before and after.
+    gpu.set_stream(torch.cuda.current_stream().cuda_stream)
     op = case["op"]
     bufs, out = {}, {}
     if op == "matvec":
