@@ -165,8 +165,8 @@ int main(int argc, char** argv) {
         const double t = secs / reps;
         if (s.matvec) {
             const double weights = s.q4 ? (double)s.n * s.k * (0.5 + 2.0 / 32) : 2.0 * s.n * s.k;
-            const double bytes = weights + 2.0 * s.m * s.k +
-                                 2.0 * s.m * s.n * (s.out == HB_OUT_RESIDUAL ? 2 : 1);
+            // Residual reads y too, F32 writes twice the bytes.
+            const double bytes = weights + 2.0 * s.m * s.k + 2.0 * s.m * s.n * (s.out == HB_OUT_BF16 ? 1 : 2);
             printf("%s:%ux%ux%u %s %.2f us %.1f GB/s\n", s.q4 ? "q4" : "mv", s.m, s.k, s.n, hb_kernel_name(g, kern), t * 1e6,
                    bytes / t / 1e9);
         } else {

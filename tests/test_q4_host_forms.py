@@ -2,6 +2,8 @@
 memory: the fields a descriptor names are kept, kernels that do not belong
 together are refused."""
 import ctypes
+import os
+import subprocess
 
 import pytest
 
@@ -110,3 +112,18 @@ def test_a_range_past_64_bits_is_refused(hb, gpu):
     for bad in (hb.r(y, 4, 2 ** 64 - 4), hb.r(y, 64, 2 ** 64 - 32), hb.r(y, 0, 129), hb.r(y, 129)):
         with pytest.raises(hb.HerbertError, match="outside buffer"):
             gpu.launch(k, [hb.r(w), hb.r(x), bad], 1)
+
+
+def test_native_host_counts_its_bytes(hb, tmp_path):
+    """hb_gemm over the host runtime, whose launches take 10 us each: GB/s of
+    weights, x and y in each Out, four bytes an f32."""
+    lib = os.path.dirname(hb.LIB_PATH)
+    exe = str(tmp_path / "hb_gemm")
+    subprocess.run(["g++", "-O1", "-std=c++17", os.path.join(host_gpu.PKG, "csrc", "hb_cli.cpp"), "-I", os.path.join(host_gpu.ROOT, "include"),
+                    "-L", lib, "-lherbert_hip", "-Wl,-rpath," + lib, "-o", exe], check=True)
+    r = subprocess.run([exe, "--reps", "2", "mv:16x64x4096", "mv:16x64x4096f", "mv:16x64x4096r"],
+                       capture_output=True, text=True, timeout=60, env=dict(os.environ, HB_CACHE_DIR=""))
+    assert r.returncode == 0, r.stderr
+    y, x, w = 16 * 4096, 2 * 16 * 64, 2 * 64 * 4096
+    want = [w + x + 2 * y, w + x + 4 * y, w + x + 4 * y]
+    assert [line.split()[-2] for line in r.stdout.splitlines()] == ["%.1f" % (b / 1e4) for b in want], r.stdout
