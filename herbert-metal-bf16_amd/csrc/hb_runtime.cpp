@@ -805,8 +805,9 @@ int hb_sync(hb_gpu* g) {
 }  // extern "C"
 
 // All work from here on to `to`.  What is queued is waited for, so that the
-// buffers and the workspace have one order of use; the event's record fails
-// for a stream that is none of this device's.
+// buffers and the workspace have one order of use.  An event of this device is
+// recorded on `to` first: a stream that HIP does not take for it changes
+// nothing.
 static int change_stream(hb_gpu* g, hipStream_t to) {
     if (to == g->stream) return HB_OK;
     HB_HIP(hipSetDevice(g->device));

@@ -18,13 +18,15 @@
 // Measured against them at the 7.0 TB/s that a streaming read reaches (a
 // launch's own 2.4 us in both): 2560 to 151936 in groups of 32 at 1 row 34.4
 // us of 33.7, at 4 rows 36.8; 17408 to 5120 in groups of 128 at 1 row 11.3 of
-// 9.0, at 16 rows 18.3, where each CU reads all of x (557 KB) for its 143 KB
-// of codes and the lines in flight in its L1 are the limit; 4096 to 2560 at 1
-// row 3.5 of 3.2.  A second stage of loads in registers changed nothing (the
-// waves of a CU cover each other's latency), nor did parts of K in several
-// workgroups at 16 rows (13.9 us before the parts are added, in a launch of
-// their own).  Half of the VALU's issue is in use at 4 rows: 28 of some 60
-// instructions a tile make the codes bf16.
+// 9.0, at 16 rows 18.3; 4096 to 2560 at 1 row 3.5 of 3.2.  The case at 16 rows
+// runs 160 workgroups of 32 W rows: 96 of the 256 CUs have none, and each of
+// the others reads all of x (557 KB) for 287 KB of codes and scales.  16 W rows
+// a wave (320 workgroups) take 28 us there, 64 (80 workgroups) 26.  K in four
+// parts over four times the workgroups took 13.9 us before the 2.5 or more of a
+// second launch that adds the parts: some 2 us less in all, for a workspace;
+// not built.  A second stage of loads in registers changed nothing (the waves
+// of a CU cover each other's latency).  Half of the VALU's issue is in use at
+// 4 rows: 28 of some 60 instructions a tile make the codes bf16.
 #include "hb_common.h"
 
 constexpr u32 K = HB_K, N = HB_N, GROUP = HB_GROUP, OUT = HB_OUT, MV = HB_MV_M;

@@ -355,7 +355,8 @@ def q4_dequantize(kdim, n, group=32):
 
 def matvec_q4(kdim, n, out, group=32, mv_m=1, rows=0, split=0, waves=0, unroll=0):
     """y[m][n] = x[m][kdim].W^T over a packed 4-bit matrix for m <= mv_m <= 16 (bindings q4, x, y);
-    zeros: the shape's defaults.  out Residual adds with one rounding, Swiglu as matvec's."""
+    zeros: the shape's defaults.  out Residual adds with one rounding, Swiglu as matvec's.  More
+    rows in launches of 16, or through q4_dequantize and a GEMM."""
     return Desc(kind=Kind.MATVEC_Q4, k=kdim, n=n, out=out, bk=group, mv_m=mv_m, rows=rows, split=split,
                 mv_waves=waves, unroll=unroll)
 
@@ -712,7 +713,11 @@ class MoeLayer:
     q4_group: w_gate_up and w_down are packed 4-bit matrices of all experts
     (q4_quantize / q4_pack over [2 inter][hidden] and [hidden][inter], in
     groups of q4_group), read by experts_q4 over tiles of 16 rows; the
-    engine times nothing then."""
+    engine times nothing then.  Any rows, but a decode batch's kernels: an
+    expert's codes are read again for every 16 of its rows.  256 experts of
+    2048 / 512 with top 8, the whole layer: 33 us of 8 rows (bf16 66), 87 of 64
+    (212), 158 of 512 (277), 239 of 1024 (304), and behind bf16 at 2048, 395
+    (346)."""
 
     def __init__(self, gpu, engine, experts, top_k, hidden, inter, rows, w_gate_up, w_down,
                  scores=None, x=None, q4_group=0):
