@@ -391,6 +391,7 @@ class Gpu:
         check(lib.hb_open(int(device), ctypes.byref(h)))
         self.h = h
         self._sizes = {}
+        self._stream = None  # its own
 
     @classmethod
     def open(cls, device=0):
@@ -418,10 +419,14 @@ class Gpu:
         own, sync() comes before they are read.  A process that imports torch
         imports it before this package, or the two bring a HIP runtime each,
         whose streams mean nothing to the other: refused."""
+        stream = None if stream is None else int(stream)
+        if stream == self._stream:
+            return
         if stream is not None and len(_hip_runtimes()) > 1:
             raise HerbertError(HB_ERR_INVALID, "set_stream: two HIP runtimes in this process (%s): import torch before "
                                "herbert_hip" % ", ".join(sorted(_hip_runtimes())))
-        check(lib.hb_own_stream(self.h) if stream is None else lib.hb_set_stream(self.h, _P(int(stream))))
+        check(lib.hb_own_stream(self.h) if stream is None else lib.hb_set_stream(self.h, _P(stream)))
+        self._stream = stream
 
     # memory
     def alloc(self, nbytes):

@@ -95,7 +95,7 @@ import herbert_hip as hb
 many = len(hb._hip_runtimes())
 assert many == (1 if sys.argv[1] == "torch" else 2), hb._hip_runtimes()
 g = object.__new__(hb.Gpu)
-g.h = None
+g.h = g._stream = None
 hb.lib = type("lib", (), {"hb_set_stream": staticmethod(lambda h, s: 0), "hb_own_stream": staticmethod(lambda h: 0)})
 g.set_stream()
 try:
