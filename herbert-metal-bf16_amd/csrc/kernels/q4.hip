@@ -16,9 +16,9 @@
 // All three are bound by the bf16 side's bytes, read and written at what a
 // copy reaches (5.4 TB/s): 5120 x 34816 in groups of 32, 457 MB, quantised in
 // 86 us and read back in 83, each alone over several matrices; in turn, as the
-// case of both has them, 110 and 72, 176 for the pair (the quantising launch
-// starts while the read back's 356 MB of writes are still in the last-level
-// cache); 256 matrices of 2048 x 1024, 604 MB, laid out in 114.  A wave
+// case of both has them, 110 and 72, 176 for the pair (likely as part of the
+// read back's 356 MB of writes leave the last-level cache under the launch that
+// follows); 256 matrices of 2048 x 1024, 604 MB, laid out in 114.  A wave
 // handles a tile, 16 bytes of bf16 a lane in four passes of 4 rows x 256
 // bytes, their loads in flight at once (one after the other: 131); divisions
 // and float extremes cost more than the bytes (144), hence the reciprocal and
