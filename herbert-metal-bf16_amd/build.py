@@ -66,6 +66,31 @@ CHECKS = {
         "-DHB_K=512 -DHB_N=2048 -DHB_GROUP=32 -DHB_OUT=0 -DHB_MV_M=16 -DHB_RT=1 -DHB_SPLIT=1 -DHB_WAVES=4 -DHB_UNROLL=4 "
         "-DHB_ROWS=2 -DHB_TOPK=8 -DHB_E=256",
     ],
+    "f8.hip": ["-DHB_OP=%d -DHB_K=%d -DHB_N=%d" % (op, k, n) for op, k, n in ((1, 2560, 1), (2, 5008, 1000), (3, 16, 1), (4, 5008, 1000))],
+    "route_topk.hip": [
+        "-DHB_E=256 -DHB_TOPK=8 -DHB_SIGMOID=0 -DHB_BIAS=0 -DHB_GROUPS=1 -DHB_TOP_GROUPS=1 -DHB_GROUP_TOP=1 -DHB_RENORM=1 "
+        "-DHB_F32=0 -DHB_SCALE=0x3f800000",
+        "-DHB_E=160 -DHB_TOPK=6 -DHB_SIGMOID=1 -DHB_BIAS=1 -DHB_GROUPS=8 -DHB_TOP_GROUPS=3 -DHB_GROUP_TOP=2 -DHB_RENORM=0 "
+        "-DHB_F32=1 -DHB_SCALE=0x41800000",
+    ],
+    "matvec_f8.hip": [
+        "-DHB_K=2560 -DHB_N=151936 -DHB_OUT=1 -DHB_MV_M=4 -DHB_RT=2 -DHB_SPLIT=8 -DHB_WAVES=8 -DHB_UNROLL=1 -DHB_ROWS=0 "
+        "-DHB_TOPK=1 -DHB_E=1",
+        "-DHB_K=5008 -DHB_N=7001 -DHB_OUT=2 -DHB_MV_M=13 -DHB_RT=1 -DHB_SPLIT=1 -DHB_WAVES=4 -DHB_UNROLL=2 -DHB_ROWS=0 "
+        "-DHB_TOPK=1 -DHB_E=1",
+        "-DHB_K=2048 -DHB_N=1024 -DHB_OUT=3 -DHB_MV_M=16 -DHB_RT=4 -DHB_SPLIT=4 -DHB_WAVES=4 -DHB_UNROLL=1 -DHB_ROWS=1 "
+        "-DHB_TOPK=8 -DHB_E=256",
+    ],
+    "gemm_f8.hip": [
+        "-DHB_K=2560 -DHB_N=10240 -DHB_OUT=0 -DHB_ROWS=0 -DHB_TOPK=1 -DHB_E=1 -DHB_BM=128 -DHB_BN=128 -DHB_WM=2 -DHB_WN=2 "
+        "-DHB_STAGES=3 -DHB_BAND=4 -DHB_KSPLIT=1",
+        "-DHB_K=5008 -DHB_N=7001 -DHB_OUT=2 -DHB_ROWS=0 -DHB_TOPK=1 -DHB_E=1 -DHB_BM=64 -DHB_BN=192 -DHB_WM=1 -DHB_WN=4 "
+        "-DHB_STAGES=3 -DHB_BAND=4 -DHB_KSPLIT=1",
+        "-DHB_K=2048 -DHB_N=1024 -DHB_OUT=3 -DHB_ROWS=1 -DHB_TOPK=8 -DHB_E=256 -DHB_BM=64 -DHB_BN=256 -DHB_WM=1 -DHB_WN=4 "
+        "-DHB_STAGES=2 -DHB_BAND=4 -DHB_KSPLIT=1",
+        "-DHB_K=512 -DHB_N=2048 -DHB_OUT=0 -DHB_ROWS=2 -DHB_TOPK=8 -DHB_E=256 -DHB_BM=128 -DHB_BN=128 -DHB_WM=2 -DHB_WN=2 "
+        "-DHB_STAGES=3 -DHB_BAND=4 -DHB_KSPLIT=1",
+    ],
     "block_norm.hip": [
         "-DHB_D=2560 -DHB_THREADS=320 -DHB_EPS=0x358637bd -DHB_PLUS1=1 -DHB_POST=1 -DHB_PRE=1 -DHB_SCALES=1 -DHB_GATE=1",
         "-DHB_D=2565 -DHB_THREADS=384 -DHB_EPS=0x358637bd -DHB_PLUS1=0 -DHB_POST=0 -DHB_PRE=1 -DHB_SCALES=0 -DHB_GATE=2",

@@ -87,6 +87,48 @@ static void q4_defaults(hb_desc* d) {
     if (!d->unroll) d->unroll = d->rows == 16 ? 2 : 1;
 }
 
+// f8 rows and matrices (f8.h): a row's codes and its padded scales; a matrix's
+// codes and its blocks' scales.
+static uint64_t f8_row_bytes(uint64_t k) { return k + ((k + 127) / 128 + 3) / 4 * 16; }
+static uint64_t f8_matrix_bytes(uint64_t k, uint64_t n) {
+    return n * k + ((n + 127) / 128 * ((k + 127) / 128) + 3) / 4 * 16;
+}
+// k and n within what keeps every byte count of a launch in 64 bits.
+static bool f8_shape(uint32_t k, uint32_t n) { return k && n && k % 16 == 0 && k <= (1u << 20) && n <= (1u << 24); }
+static bool f8_rows_form(const hb_desc& d) { return d.form == HB_F8_ROWS; }
+
+// The 8-bit matvec's form by its row tiles (16 W rows) and K tiles (128 K).
+static void mv_f8_defaults(hb_desc* d) {
+    if (!d->mv_m) d->mv_m = d->rows_of == HB_ROWS_DENSE ? 1 : 16;
+    const uint32_t nt = cdiv(d->n, 16), kt = cdiv(d->k, 128);
+    const bool swi = d->out == HB_OUT_SWIGLU;
+    if (!d->rows) d->rows = d->rows_of != HB_ROWS_DENSE || nt > 256 || swi ? 32 : 16;
+    if (!d->split) {
+        d->split = d->rows_of != HB_ROWS_DENSE ? 4 : d->rows == 16 || (kt >= 64 && nt <= 512) ? 16 : 8;
+        while (d->split > kt || (d->mv_waves && d->split > d->mv_waves)) d->split /= 2;
+        if (!d->split) d->split = 1;
+    }
+    if (!d->mv_waves) d->mv_waves = d->split < 4 ? 4 : d->split;
+    if (!d->unroll) d->unroll = d->rows == 16 ? 2 : 1;
+}
+
+// The 8-bit GEMM's tile by the rows it is built for (rows_max).
+static void gemm_f8_defaults(hb_desc* d) {
+    const bool swi = d->out == HB_OUT_SWIGLU;
+    if (!d->bm) d->bm = d->rows_max && d->rows_max <= 32 ? 32 : d->rows_max && d->rows_max <= 64 ? 64 : 128;
+    if (!d->bn) d->bn = swi ? 256 : 128;
+    if (!d->wm) d->wm = d->bm >= 128 ? 2 : 1;
+    if (!d->wn) d->wn = swi || d->wm == 1 ? 4 : 2;
+    if (!d->dbuf) d->dbuf = d->bm + d->bn >= 384 ? 1 : 2;
+    if (!d->band) d->band = 4;
+}
+
+// What a GEMM_F8 workgroup holds in LDS.
+static uint64_t gemm_f8_lds(const hb_desc& d) {
+    const uint32_t blocks = d.out == HB_OUT_SWIGLU ? 2 : d.bn % 128 == 0 ? d.bn / 128 : cdiv(d.bn, 128) + (128 % d.bn != 0);
+    return (uint64_t)(d.dbuf + 1) * (d.bm + d.bn) * 128 + d.bm * 64 + (uint64_t)blocks * cdiv(d.k, 128) * 4;
+}
+
 hb_desc with_defaults(const hb_desc& in) {
     hb_desc d = in;
     if (d.ksplit == 1) d.ksplit = 0;  // one part: no split
@@ -116,6 +158,14 @@ hb_desc with_defaults(const hb_desc& in) {
     } else if (d.kind >= HB_KIND_Q4_QUANTIZE && d.kind <= HB_KIND_MATVEC_Q4) {
         if (!d.bk) d.bk = 32;
         if (d.kind == HB_KIND_MATVEC_Q4) q4_defaults(&d);
+    } else if (d.kind == HB_KIND_MATVEC_F8) {
+        mv_f8_defaults(&d);
+    } else if (d.kind == HB_KIND_GEMM_F8) {
+        gemm_f8_defaults(&d);
+    } else if (d.kind == HB_KIND_ROUTE_TOPK) {
+        if (!d.bm) d.bm = 1;
+        if (!d.bn) d.bn = d.bm;
+        if (!d.eps_bits) d.eps_bits = 0x3f800000u;
     }
     return d;
 }
@@ -483,6 +533,118 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
                           D("HB_SCALES", scales), D("HB_GATE", gate)};
             return HB_OK;
         }
+        case HB_KIND_ROUTE_TOPK: {
+            if (!d.experts || d.experts > 1024 || !d.top_k || d.top_k > 32)
+                return fail(HB_ERR_UNSUPPORTED, "route_topk: 1 to 1024 experts, top_k 1 to 32");
+            if (d.form & ~31u) return fail(HB_ERR_INVALID, "route_topk: parts out of range");
+            if (d.bm > 64 || d.experts % d.bm || !d.bn || d.bn > d.bm || d.top_k > d.experts / d.bm * d.bn)
+                return fail(HB_ERR_UNSUPPORTED, "route_topk: up to 64 groups of equal size, top_groups of them, top_k no more than their experts");
+            const uint32_t f = d.form;
+            snprintf(name, sizeof name, "route_topk_%u_k%u_g%ut%u_%s%s%s%s%s_x%08x", d.experts, d.top_k, d.bm, d.bn,
+                     f & HB_ROUTE_SIGMOID ? "sig" : "smx", f & HB_ROUTE_BIAS ? "_b" : "", f & HB_ROUTE_RENORM ? "_n" : "",
+                     f & HB_ROUTE_F32 ? "_f32" : "", f & HB_ROUTE_GROUP_TWO ? "_two" : "", d.eps_bits);
+            e->name = name;
+            e->source = "route_topk.hip";
+            e->threads = 256;
+            e->nbind = f & HB_ROUTE_BIAS ? 3 : 2;
+            e->defines = {D("HB_E", d.experts), D("HB_TOPK", d.top_k), D("HB_GROUPS", d.bm), D("HB_TOP_GROUPS", d.bn),
+                          D("HB_SIGMOID", f & HB_ROUTE_SIGMOID ? 1 : 0), D("HB_BIAS", f & HB_ROUTE_BIAS ? 1 : 0),
+                          D("HB_RENORM", f & HB_ROUTE_RENORM ? 1 : 0), D("HB_F32", f & HB_ROUTE_F32 ? 1 : 0),
+                          D("HB_GROUP_TOP", f & HB_ROUTE_GROUP_TWO ? 2 : 1), D("HB_SCALE", d.eps_bits)};
+            return HB_OK;
+        }
+        case HB_KIND_F8_QUANTIZE:
+        case HB_KIND_F8_DEQUANTIZE: {
+            if (d.form > HB_F8_ROWS) return fail(HB_ERR_INVALID, "f8: a matrix or rows");
+            const bool rows = f8_rows_form(d);
+            if (!f8_shape(d.k, rows ? 1 : d.n))
+                return fail(HB_ERR_UNSUPPORTED, "f8: K a multiple of 16 up to 2^20, N up to 2^24");
+            const uint32_t op = (d.kind == HB_KIND_F8_QUANTIZE ? 1 : 3) + (rows ? 0 : 1);
+            if (rows)
+                snprintf(name, sizeof name, "f8_%s_rows_%u", op == 1 ? "quantize" : "dequantize", d.k);
+            else
+                snprintf(name, sizeof name, "f8_%s_%ux%u", op == 2 ? "quantize" : "dequantize", d.k, d.n);
+            e->name = name;
+            e->source = "f8.hip";
+            e->threads = 256;
+            e->nbind = 2;
+            e->defines = {D("HB_OP", op), D("HB_K", d.k), D("HB_N", rows ? 1 : d.n)};
+            return HB_OK;
+        }
+        case HB_KIND_MATVEC_F8: {
+            const bool experts = d.rows_of != HB_ROWS_DENSE, swi = d.out == HB_OUT_SWIGLU;
+            if (d.out > HB_OUT_SWIGLU || d.rows_of > HB_ROWS_SCATTER)
+                return fail(HB_ERR_INVALID, "matvec_f8: out / rows_of out of range");
+            if (!f8_shape(d.k, d.n)) return fail(HB_ERR_UNSUPPORTED, "matvec_f8: K a multiple of 16 up to 2^20, N up to 2^24");
+            if (swi && d.n % 256)
+                return fail(HB_ERR_UNSUPPORTED, "matvec_f8 Out::Swiglu: gate and up rows each a multiple of 128");
+            if (d.mv_m > 16) return fail(HB_ERR_UNSUPPORTED, "matvec_f8: m <= 16");
+            if ((d.rows != 16 && d.rows != 32 && d.rows != 64) || (swi && d.rows == 16))
+                return fail(HB_ERR_UNSUPPORTED, "matvec_f8: 16, 32 or 64 rows a wave (Out::Swiglu not 16)");
+            if (d.mv_waves > 16 || !pow2(d.mv_waves) || !pow2(d.split) || d.split > d.mv_waves || d.unroll > 4)
+                return fail(HB_ERR_UNSUPPORTED, "matvec_f8: 1, 2, 4, 8 or 16 waves, split no more, unroll 1..4");
+            if (experts && (!d.top_k || d.top_k > d.experts || d.experts > 1024 || !d.tiles || !d.rows_max ||
+                            (uint64_t)d.rows_max * d.top_k >= (1u << 28) || d.mv_m != 16 || (d.out != HB_OUT_BF16 && !swi)))
+                return fail(HB_ERR_INVALID, "matvec_f8 over experts: top_k, experts (<= 1024), tiles and rows_max "
+                                            "(below 2^28 pairs), tiles of 16 rows, bf16 out");
+            std::string rows;
+            if (experts) {
+                snprintf(name, sizeof name, "_%s_k%u_e%u_t%u_r%u", d.rows_of == HB_ROWS_GATHER ? "gather" : "scatter",
+                         d.top_k, d.experts, d.tiles, d.rows_max);
+                rows = name;
+            }
+            snprintf(name, sizeof name, "matvec_f8_%ux%u%s_r%u_k%u_w%u_u%u_m%u%s", d.k, d.n,
+                     d.out == HB_OUT_F32 ? "_f32" : d.out == HB_OUT_RESIDUAL ? "_res" : swi ? "_sw" : "", d.rows, d.split,
+                     d.mv_waves, d.unroll, d.mv_m, rows.c_str());
+            e->name = name;
+            e->source = "matvec_f8.hip";
+            e->threads = 64 * d.mv_waves;
+            e->nbind = experts ? 6 : 3;
+            e->defines = {D("HB_K", d.k),           D("HB_N", d.n),            D("HB_OUT", d.out),
+                          D("HB_MV_M", d.mv_m),     D("HB_RT", d.rows / 16),   D("HB_SPLIT", d.split),
+                          D("HB_WAVES", d.mv_waves), D("HB_UNROLL", d.unroll), D("HB_ROWS", d.rows_of),
+                          D("HB_TOPK", experts ? d.top_k : 1), D("HB_E", experts ? d.experts : 1)};
+            return HB_OK;
+        }
+        case HB_KIND_GEMM_F8: {
+            const bool experts = d.rows_of != HB_ROWS_DENSE, swi = d.out == HB_OUT_SWIGLU;
+            if (d.out > HB_OUT_SWIGLU || d.rows_of > HB_ROWS_SCATTER)
+                return fail(HB_ERR_INVALID, "gemm_f8: out / rows_of out of range");
+            if (!f8_shape(d.k, d.n) || d.k > 65536 || (uint64_t)d.k * d.n > 0x7fffffffull)
+                return fail(HB_ERR_UNSUPPORTED, "gemm_f8: K a multiple of 16 up to 2^16, K N below 2^31");
+            if (swi && (d.n % 256 || d.rows_of == HB_ROWS_SCATTER))
+                return fail(HB_ERR_UNSUPPORTED, "gemm_f8 Out::Swiglu: gate and up rows each a multiple of 128, no scatter");
+            if (d.bm > 256 || !pow2(d.bm) || d.bm < 32 || d.bn > 256 || d.bn % 32 || !d.wm || !d.wn || d.wm * d.wn > 16 ||
+                d.bm % (d.wm * 16) || d.bn % (d.wn * 16) || (swi && (d.bn != 256 || d.bn / d.wn % 32)))
+                return fail(HB_ERR_UNSUPPORTED, "gemm_f8: tiles of 32 to 256 X rows (a power of 2) by up to 256 W rows (Out::Swiglu 256), "
+                                                "whole fragments of 16 a wave");
+            if (d.dbuf < 1 || d.dbuf > 3 || !d.band || gemm_f8_lds(d) > 160 * 1024)
+                return fail(HB_ERR_UNSUPPORTED, "gemm_f8: 2 to 4 stages within 160 KiB of LDS, a band");
+            if (d.ksplit > 16 || (d.ksplit > 1 && (experts || swi || d.n % 4 || d.ksplit > cdiv(d.k, 128))))
+                return fail(HB_ERR_UNSUPPORTED, "gemm_f8 split K: 2..16 parts of whole K tiles, dense rows, N a multiple of 4");
+            if (experts && (!d.top_k || d.top_k > d.experts || d.experts > 1024 || !d.tiles || !d.rows_max ||
+                            (uint64_t)d.rows_max * d.top_k >= (1u << 28) || (d.out != HB_OUT_BF16 && !swi)))
+                return fail(HB_ERR_INVALID, "gemm_f8 over experts: top_k, experts (<= 1024), tiles and rows_max (below 2^28 pairs), bf16 out");
+            std::string rows;
+            if (experts) {
+                snprintf(name, sizeof name, "_%s_k%u_e%u_t%u_r%u", d.rows_of == HB_ROWS_GATHER ? "gather" : "scatter", d.top_k,
+                         d.experts, d.tiles, d.rows_max);
+                rows = name;
+            } else if (d.ksplit > 1) {
+                rows = "_ks" + std::to_string(d.ksplit);
+            }
+            snprintf(name, sizeof name, "gemm_f8_%ux%u_%s_t%ux%u_w%ux%u_d%u_b%u%s", d.k, d.n, swi ? "sw" : out_tag(d.out), d.bn,
+                     d.bm, d.wn, d.wm, d.dbuf, d.band, rows.c_str());
+            e->name = name;
+            e->source = "gemm_f8.hip";
+            e->threads = 64 * d.wm * d.wn;
+            e->nbind = 6;
+            e->defines = {D("HB_K", d.k),   D("HB_N", d.n),   D("HB_OUT", d.ksplit > 1 ? (uint32_t)HB_OUT_F32 : d.out),
+                          D("HB_ROWS", d.rows_of), D("HB_TOPK", experts ? d.top_k : 1), D("HB_E", experts ? d.experts : 1),
+                          D("HB_BM", d.bm), D("HB_BN", d.bn), D("HB_WM", d.wm), D("HB_WN", d.wn),
+                          D("HB_STAGES", d.dbuf + 1), D("HB_BAND", d.band), D("HB_KSPLIT", d.ksplit > 1 ? d.ksplit : 1)};
+            return HB_OK;
+        }
         case HB_KIND_ROUND_PROBE:
             e->name = "round_probe_bf16";
             e->source = "probe.hip";
@@ -545,7 +707,21 @@ uint32_t groups_of(const hb_desc& d, uint32_t m) {
             return d.persist ? (d.persist < wgs ? d.persist : wgs) : wgs;
         }
         case HB_KIND_ROUTE:
+        case HB_KIND_ROUTE_TOPK:
             return cdiv(m, 4);  // a wavefront per row
+        case HB_KIND_F8_QUANTIZE:  // 16 lanes a group of a row; a workgroup a block
+            if (f8_rows_form(d)) return (uint32_t)(((uint64_t)m * cdiv(d.k, 128) + 15) / 16);
+            return (uint32_t)((uint64_t)m * cdiv(d.n, 128) * cdiv(d.k, 128));
+        case HB_KIND_F8_DEQUANTIZE:  // 16 elements a thread
+            return (uint32_t)(((uint64_t)m * (f8_rows_form(d) ? 1 : d.n) * (d.k / 16) + 255) / 256);
+        case HB_KIND_GEMM_F8: {
+            const uint32_t nt = d.out == HB_OUT_SWIGLU ? cdiv(d.n, 256) : cdiv(d.n, d.bn);
+            if (d.rows_of == HB_ROWS_DENSE) return (uint32_t)((uint64_t)cdiv(m, d.bm) * nt * (d.ksplit > 1 ? d.ksplit : 1));
+            // Tiles with rows: no more than pairs, nor than the table holds;
+            // whole rounds of the eight XCDs.
+            const uint64_t pairs = (uint64_t)m * d.top_k, all = (pairs < d.tiles ? pairs : d.tiles) * nt;
+            return (uint32_t)((all + 7) / 8 * 8);
+        }
         case HB_KIND_SORT:
         case HB_KIND_SORT_ATOMIC:
             return 1;
@@ -558,6 +734,7 @@ uint32_t groups_of(const hb_desc& d, uint32_t m) {
         case HB_KIND_Q4_PACK:
         case HB_KIND_Q4_DEQUANTIZE:  // a wave a tile
             return (uint32_t)((m * q4_tiles(d.k, d.n) + 3) / 4);
+        case HB_KIND_MATVEC_F8:
         case HB_KIND_MATVEC_Q4: {
             const uint32_t per = d.out == HB_OUT_SWIGLU ? d.rows / 32 : d.rows / 16;
             const uint32_t nt = d.out == HB_OUT_SWIGLU ? d.n / 32 : cdiv(d.n, 16);
@@ -580,7 +757,7 @@ uint32_t groups_of(const hb_desc& d, uint32_t m) {
 }
 
 uint64_t workspace_of(const hb_desc& d, uint32_t m) {
-    if (d.kind != HB_KIND_GEMM || d.ksplit < 2) return 0;
+    if (!splits_k(d)) return 0;
     return (uint64_t)d.ksplit * m * d.n * 4;
 }
 
@@ -632,6 +809,38 @@ static AccessList accesses(const hb_desc& d, uint32_t m) {
             l.add("q4", d.experts * q4, 16, false);
             l.add("X", (d.rows_of == HB_ROWS_GATHER ? mm : pairs) * k * 2, 2, false);
             l.add("Y", pairs * nout * size, size, true);
+            l.add("list", pairs * 4, 4, false);
+            l.add("tiles", (1 + 3ull * d.tiles) * 4, 4, false);
+            break;
+        }
+        case HB_KIND_ROUTE_TOPK: {
+            const uint32_t size = d.form & HB_ROUTE_F32 ? 4 : 2;
+            l.add("scores", mm * d.experts * size, size, false);
+            l.add("route", mm * 8 * d.top_k, 4, true);
+            if (d.form & HB_ROUTE_BIAS) l.add("bias", 4ull * d.experts, 4, false);
+            break;
+        }
+        case HB_KIND_F8_QUANTIZE:
+        case HB_KIND_F8_DEQUANTIZE: {
+            const bool rows = f8_rows_form(d), to = d.kind == HB_KIND_F8_QUANTIZE;
+            const uint64_t wide = mm * (rows ? 1 : n) * k * 2, f8 = mm * (rows ? f8_row_bytes(k) : f8_matrix_bytes(k, n));
+            if (to) l.add(rows ? "x" : "W", wide, 2, false);
+            l.add("f8", f8, 16, to);
+            if (!to) l.add(rows ? "x" : "W", wide, 2, true);
+            break;
+        }
+        case HB_KIND_MATVEC_F8:
+        case HB_KIND_GEMM_F8: {
+            const bool dense = d.rows_of == HB_ROWS_DENSE, mv = d.kind == HB_KIND_MATVEC_F8, swi = d.out == HB_OUT_SWIGLU;
+            const uint64_t w = f8_matrix_bytes(k, n), pairs = mm * d.top_k, xrow = mv ? k * 2 : f8_row_bytes(k);
+            const bool f8_out = swi && !mv;
+            const uint64_t yrow = f8_out ? f8_row_bytes(n / 2) : (swi ? n / 2 : n) * out_bytes(d.out);
+            const uint32_t xa = mv ? 2 : 16, ya = f8_out ? 16 : out_bytes(d.out);
+            if (!(mv && dense)) l.add("state", 16, 4, false);
+            l.add("W", (dense ? 1 : d.experts) * w, 16, false);
+            l.add("X", (dense || d.rows_of == HB_ROWS_GATHER ? mm : pairs) * xrow, xa, false);
+            l.add("Y", (dense ? mm : pairs) * yrow, ya, true);
+            if (dense) break;
             l.add("list", pairs * 4, 4, false);
             l.add("tiles", (1 + 3ull * d.tiles) * 4, 4, false);
             break;
@@ -719,16 +928,32 @@ int check_bindings(const hb_desc& d, const uint64_t* s, uint32_t nbind, uint32_t
         return HB_OK;
     }
     if (m == 0) return fail(HB_ERR_INVALID, "0 rows");
-    if (d.kind >= HB_KIND_Q4_QUANTIZE && d.kind <= HB_KIND_BLOCK_NORM) {
+    if (d.kind >= HB_KIND_Q4_QUANTIZE && d.kind <= HB_KIND_MATVEC_F8) {
         // First what keeps the byte counts and the grid (fewer than 2^32
         // threads) within range.
-        if (d.kind == HB_KIND_MATVEC_Q4) {
+        if (d.kind == HB_KIND_MATVEC_Q4 || d.kind == HB_KIND_MATVEC_F8) {
+            const std::string what = d.kind == HB_KIND_MATVEC_Q4 ? "matvec_q4" : "matvec_f8";
             const bool dense = d.rows_of == HB_ROWS_DENSE;
             if (dense && m > d.mv_m)
-                return fail(HB_ERR_INVALID, "matvec_q4 of " + std::to_string(m) + " rows: 1.." + std::to_string(d.mv_m));
+                return fail(HB_ERR_INVALID, what + " of " + std::to_string(m) + " rows: 1.." + std::to_string(d.mv_m));
             if (!dense && m > d.rows_max) return fail(HB_ERR_INVALID, "m beyond the kernel's rows_max");
             if ((uint64_t)groups_of(d, m) * 64 * d.mv_waves >> 32)
-                return fail(HB_ERR_UNSUPPORTED, "matvec_q4: too many workgroups in one launch");
+                return fail(HB_ERR_UNSUPPORTED, what + ": too many workgroups in one launch");
+        } else if (d.kind == HB_KIND_ROUTE_TOPK) {
+            if (m >= (1u << 26)) return fail(HB_ERR_UNSUPPORTED, "route_topk: too many rows in one launch");
+        } else if (d.kind == HB_KIND_F8_QUANTIZE || d.kind == HB_KIND_F8_DEQUANTIZE) {
+            // Rows of at most 2^20, matrices of at most 2^44 elements.
+            const uint64_t each = f8_rows_form(d) ? cdiv(d.k, 16) : (uint64_t)cdiv(d.n, 128) * 128 * (cdiv(d.k, 128) * 8);
+            if (each >> 32 || m * each >> 32) return fail(HB_ERR_UNSUPPORTED, "f8: too many elements in one launch");
+        } else if (d.kind == HB_KIND_GEMM_F8) {
+            const bool dense = d.rows_of == HB_ROWS_DENSE;
+            if (!dense && m > d.rows_max) return fail(HB_ERR_INVALID, "m beyond the kernel's rows_max");
+            // The kernel addresses X by 32 bits.
+            if ((d.rows_of == HB_ROWS_SCATTER ? (uint64_t)m * d.top_k : m) * f8_row_bytes(d.k) > 0x7fffffffull)
+                return fail(HB_ERR_UNSUPPORTED, "gemm_f8: X at most 2 GiB - 1 bytes");
+            const uint64_t nt = cdiv(d.n, d.bn);
+            const uint64_t groups = dense ? cdiv(m, d.bm) * nt * (d.ksplit > 1 ? d.ksplit : 1) : ((uint64_t)m * d.top_k < d.tiles ? (uint64_t)m * d.top_k : d.tiles) * nt + 8;
+            if (groups * 64 * d.wm * d.wn >> 32) return fail(HB_ERR_UNSUPPORTED, "gemm_f8: too many workgroups in one launch");
         } else if (d.kind == HB_KIND_BLOCK_NORM) {
             if ((uint64_t)m * norm_threads(d.n) >> 32)
                 return fail(HB_ERR_UNSUPPORTED, "block_norm: too many rows in one launch");
@@ -803,6 +1028,15 @@ int check_bindings(const hb_desc& d, const uint64_t* s, uint32_t nbind, uint32_t
 }
 
 }  // namespace hb
+
+extern "C" uint64_t hb_f8_bytes(uint32_t k, uint32_t n) { return hb::f8_shape(k, n) ? hb::f8_matrix_bytes(k, n) : 0; }
+
+extern "C" uint64_t hb_f8_row_bytes(uint32_t k) { return hb::f8_shape(k, 1) ? hb::f8_row_bytes(k) : 0; }
+
+extern "C" uint32_t hb_f8_tile_rows(uint32_t rows, uint32_t top_k, uint32_t experts) {
+    const uint64_t pairs = (uint64_t)rows * top_k;
+    return pairs <= 4ull * experts ? 16 : pairs <= 32ull * experts ? 32 : pairs <= 96ull * experts ? 64 : 128;
+}
 
 extern "C" uint64_t hb_q4_bytes(uint32_t k, uint32_t n, uint32_t group) {
     return hb::q4_shape(k, n, group) ? hb::q4_bytes(k, n, group) : 0;

@@ -48,8 +48,11 @@ int check_bindings(const hb_desc& d, const uint64_t* sizes, uint32_t nbind, uint
 int check_addresses(const hb_desc& d, void* const* ptrs, uint32_t nbind, uint32_t m);
 // A gate|up kernel that writes the SwiGLU of its sums itself.
 inline bool writes_swiglu(const hb_desc& d) {
-    return d.kind == HB_KIND_GEMM_SWIGLU || (d.kind == HB_KIND_MATVEC_Q4 && d.out == HB_OUT_SWIGLU);
+    return d.kind == HB_KIND_GEMM_SWIGLU ||
+           ((d.kind == HB_KIND_MATVEC_Q4 || d.kind == HB_KIND_MATVEC_F8 || d.kind == HB_KIND_GEMM_F8) && d.out == HB_OUT_SWIGLU);
 }
+// A GEMM in parts of K, whose launches are two kernels.
+inline bool splits_k(const hb_desc& d) { return (d.kind == HB_KIND_GEMM || d.kind == HB_KIND_GEMM_F8) && d.ksplit > 1; }
 // Fills defaults of the descriptor's zero fields (tile sizes, ...).
 hb_desc with_defaults(const hb_desc& d);
 

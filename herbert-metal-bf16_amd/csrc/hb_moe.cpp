@@ -21,13 +21,21 @@ int moe_experts_run(hb_gpu* g, const int32_t kernels[4], int32_t swiglu, int32_t
     // Grouped expert GEMMs only (never a dense split-K pair, whose
     // workspace the static entry point could not allocate).
     const hb_desc* dd = kernel_desc(g, dn);
-    const bool q4 = gd->kind == HB_KIND_MATVEC_Q4;
+    const bool q4 = gd->kind == HB_KIND_MATVEC_Q4, mv_f8 = gd->kind == HB_KIND_MATVEC_F8, f8 = gd->kind == HB_KIND_GEMM_F8;
     if (gd->rows_of == HB_ROWS_DENSE || dd->rows_of == HB_ROWS_DENSE ||
-        dd->kind != (q4 ? HB_KIND_MATVEC_Q4 : HB_KIND_GEMM))
+        dd->kind != (q4 || mv_f8 || f8 ? gd->kind : (uint32_t)HB_KIND_GEMM))
         return fail(HB_ERR_INVALID, "moe experts: kernels[1] and kernels[2] are grouped expert GEMMs");
-    if (q4 && (sd->bm != 16 || gd->rows_of != HB_ROWS_GATHER || dd->rows_of != HB_ROWS_SCATTER || gather >= 0))
-        return fail(HB_ERR_INVALID, "moe experts in 4 bits: a sort of 16-row tiles, gathered gate|up rows, "
-                                    "scattered down rows, no gather kernel");
+    if ((q4 || mv_f8) && (sd->bm != 16 || gd->rows_of != HB_ROWS_GATHER || dd->rows_of != HB_ROWS_SCATTER || gather >= 0))
+        return fail(HB_ERR_INVALID, std::string("moe experts in ") + (q4 ? "4" : "8") +
+                                        " bits: a sort of 16-row tiles, gathered gate|up rows, "
+                                        "scattered down rows, no gather kernel");
+    if (f8) {
+        const hb_desc* qd = kernel_desc(g, gather);
+        if (sd->bm != gd->bm || sd->bm != dd->bm || gd->rows_of != HB_ROWS_GATHER || dd->rows_of != HB_ROWS_SCATTER ||
+            gd->out != HB_OUT_SWIGLU || !qd || qd->kind != HB_KIND_F8_QUANTIZE || qd->form != HB_F8_ROWS || qd->k != gd->k)
+            return fail(HB_ERR_INVALID, "moe experts in 8 bits: a sort of the products' tiles, gathered gate|up rows with the "
+                                        "SwiGLU, scattered down rows, kernels[3] the quantise kernel of x's rows");
+    }
     // Its rows would be half as long as the combine reads them.
     if (writes_swiglu(*dd)) return fail(HB_ERR_INVALID, "moe experts: a down kernel that writes a SwiGLU");
     const bool fused = writes_swiglu(*gd);
@@ -48,7 +56,10 @@ int moe_experts_run(hb_gpu* g, const int32_t kernels[4], int32_t swiglu, int32_t
     };
     if ((rc = run(sort, {STATE, ROUTE, LIST, TILES}, m))) return rc;
     int xin = X;
-    if (gather >= 0) {
+    if (f8) {
+        if ((rc = run(gather, {X, XS}, m))) return rc;
+        xin = XS;
+    } else if (gather >= 0) {
         if ((rc = run(gather, {STATE, LIST, X, XS}, m))) return rc;
         xin = XS;
     }

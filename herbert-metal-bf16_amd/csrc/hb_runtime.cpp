@@ -547,7 +547,7 @@ int hb_kernel_precompile(const hb_desc* desc) {
     if (rc) return rc;
     std::string code;
     if ((rc = compile(em, "gfx950", &code))) return rc;
-    if (d.kind == HB_KIND_GEMM && d.ksplit > 1) {
+    if (splits_k(d)) {
         hb_desc rd{};
         rd.kind = KIND_SPLITK_REDUCE;
         rd.n = d.n;
@@ -571,7 +571,7 @@ int hb_kernel_build(hb_gpu* g, const hb_desc* desc, int32_t* kernel) {
     Kernel k;
     rc = load_kernel(g, d, &k);
     if (rc) return rc;
-    if (d.kind == HB_KIND_GEMM && d.ksplit > 1) {
+    if (splits_k(d)) {
         // Its second kernel, built (or found) first.
         hb_desc rd{};
         rd.kind = KIND_SPLITK_REDUCE;

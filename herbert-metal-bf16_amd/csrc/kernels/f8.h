@@ -1,0 +1,74 @@
+// f8.h -- 8-bit floating point operands (OCP e4m3, largest 448): codes q and
+// f32 scales s, an element q * s.  Of a group's bf16 elements x, with a =
+// max(|largest|, 2^-100):
+//
+//   s = a / 448 (f32),  q = the e4m3 nearest to 448 x / a, ties to even.
+//
+// A group with a NaN or an infinity stands for NaN.  "f8 rows" hold
+// activations: a row's k codes, then the f32 scales of its groups of 128, the
+// count of scales rounded up to a multiple of 4.  An "f8 matrix" holds weights:
+// the codes [n][k], then the f32 scales [ceil(n / 128)][ceil(k / 128)] of its
+// blocks of 128 x 128, in all a multiple of 16 bytes.  k is a multiple of 16.
+#pragma once
+#include "hb_common.h"
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef u16 u16x2 __attribute__((ext_vector_type(2)));
+
+constexpr u32 f8_blocks(u32 k) { return (k + 127) / 128; }
+constexpr u64 f8_row_bytes(u64 k) { return k + ((k + 127) / 128 + 3) / 4 * 16; }
+constexpr u64 f8_matrix_bytes(u64 k, u64 n) {
+    return n * k + ((n + 127) / 128 * ((k + 127) / 128) + 3) / 4 * 16;
+}
+
+// The larger halves of two words, as u16: bf16 without their signs stand in
+// the order of their sizes, infinities and NaNs last.
+HB_DEV u32 f8_max2(u32 a, u32 b) {
+    return __builtin_bit_cast(u32, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+// The largest sizes of 8 bf16, two of them in a word's halves.
+HB_DEV u32 f8_max8(u32x4 v) {
+    const u32 m = 0x7fff7fffu;
+    return f8_max2(f8_max2(v.x & m, v.y & m), f8_max2(v.z & m, v.w & m));
+}
+// Both halves of f8_max8's words over the 16 lanes of a row of lanes: the
+// largest one's bf16 bits, in every lane.
+HB_DEV u32 f8_max_lanes(u32 w) {
+#define HB_F8_DPP(ctrl) w = f8_max2(w, (u32)__builtin_amdgcn_update_dpp(0, (int)w, ctrl, 0xf, 0xf, true))
+    HB_F8_DPP(0x128);  // row_ror:8
+    HB_F8_DPP(0x124);  // row_ror:4
+    HB_F8_DPP(0x4E);   // quad_perm [2,3,0,1]
+    HB_F8_DPP(0xB1);   // quad_perm [1,0,3,2]
+#undef HB_F8_DPP
+    w = f8_max2(w, w >> 16);
+    return w & 0xffffu;
+}
+
+// s and 448 / a of a group whose largest size has the bf16 bits `top`.
+struct F8Scale {
+    float s, inv;
+};
+HB_DEV F8Scale f8_scale(u32 top) {
+    u32 b = top << 16;
+    b = b > 0x0d800000u ? b : 0x0d800000u;  // 2^-100; a NaN stays the larger
+    const float a = __builtin_bit_cast(float, b);
+    return {a / 448.0f, 448.0f / a};
+}
+
+// 448 x / a, near enough to round to e4m3: the product with the rounded
+// reciprocal is within 2^-22 of the quotient.  x and a have 8 bits each, so a
+// quotient that lies halfway between two codes does so exactly and any other at
+// least 2^-14 from halfway; rounding the product to 19 bits restores the first
+// kind and keeps the second on its side.
+HB_DEV float f8_quotient(float x, float inv) {
+    return __builtin_bit_cast(float, (__builtin_bit_cast(u32, x * inv) + 16u) & ~31u);
+}
+// The codes of two bf16 in a word, in the low or the high half of `old`.
+template <bool high>
+HB_DEV u32 f8_codes2(u32 w, float inv, u32 old) {
+    return (u32)__builtin_amdgcn_cvt_pk_fp8_f32(f8_quotient(bf16_lo(w), inv), f8_quotient(bf16_hi(w), inv), (int)old, high);
+}
+// Those of 8 bf16, in order.
+HB_DEV u32x2 f8_codes8(u32x4 v, float inv) {
+    return u32x2{f8_codes2<true>(v.y, inv, f8_codes2<false>(v.x, inv, 0)), f8_codes2<true>(v.w, inv, f8_codes2<false>(v.z, inv, 0))};
+}

@@ -95,6 +95,17 @@ class Kind(enum.IntEnum):
     Q4_DEQUANTIZE = 16
     MATVEC_Q4 = 17
     BLOCK_NORM = 18
+    ROUTE_TOPK = 19
+    F8_QUANTIZE = 20
+    F8_DEQUANTIZE = 21
+    GEMM_F8 = 22
+    MATVEC_F8 = 23
+
+
+class Score(enum.IntEnum):
+    """What route_topk makes of a score (enum hb_route_parts)."""
+    Softmax = 0
+    Sigmoid = 1
 
 
 class Gate(enum.IntEnum):
@@ -367,6 +378,101 @@ def experts_q4(kdim, n, out, group, rows_of, top_k, experts, rows_max, rows=0, s
     return Desc(kind=Kind.MATVEC_Q4, k=kdim, n=n, out=out, bk=group, mv_m=16, rows=rows, split=split, mv_waves=waves,
                 unroll=unroll, rows_of=rows_of, top_k=top_k, experts=experts, rows_max=rows_max,
                 tiles=moe_tiles(rows_max, top_k, experts, 16))
+
+
+lib.hb_f8_bytes.argtypes = [_u32, _u32]
+lib.hb_f8_bytes.restype = _u64
+lib.hb_f8_row_bytes.argtypes = [_u32]
+lib.hb_f8_row_bytes.restype = _u64
+lib.hb_f8_tile_rows.argtypes = [_u32, _u32, _u32]
+lib.hb_f8_tile_rows.restype = _u32
+
+
+def f8_bytes(kdim, n):
+    """Bytes of an f8 matrix (hb_f8_bytes): e4m3 codes [n][kdim], then f32 scales
+    [ceil(n / 128)][ceil(kdim / 128)]."""
+    b = lib.hb_f8_bytes(int(kdim), int(n))
+    if not b:
+        raise HerbertError(HB_ERR_UNSUPPORTED, "f8 %dx%d: K a multiple of 16" % (kdim, n))
+    return b
+
+
+def f8_row_bytes(kdim):
+    """Bytes of a row of f8 rows (hb_f8_row_bytes): kdim codes, then the f32 scales of its groups
+    of 128, their count rounded up to a multiple of 4."""
+    b = lib.hb_f8_row_bytes(int(kdim))
+    if not b:
+        raise HerbertError(HB_ERR_UNSUPPORTED, "f8 rows of %d: K a multiple of 16" % kdim)
+    return b
+
+
+def f8_tile_rows(rows, top_k, experts):
+    """The rows per expert tile that experts_f8 takes for blocks of up to `rows` rows (hb_f8_tile_rows)."""
+    return lib.hb_f8_tile_rows(int(rows), int(top_k), int(experts))
+
+
+def f8_quantize(kdim, n):
+    """W [n][kdim] bf16 -> the f8 matrix, a scale for each block of 128 x 128 (bindings W, f8;
+    launched over the count of matrices)."""
+    return Desc(kind=Kind.F8_QUANTIZE, k=kdim, n=n)
+
+
+def f8_quantize_rows(kdim):
+    """x [m][kdim] bf16 -> f8 rows, a scale for each 128 elements of a row (bindings x, f8)."""
+    return Desc(kind=Kind.F8_QUANTIZE, k=kdim, form=1)
+
+
+def f8_dequantize(kdim, n):
+    """The f8 matrix -> W [n][kdim] bf16, code * scale rounded once (bindings f8, W)."""
+    return Desc(kind=Kind.F8_DEQUANTIZE, k=kdim, n=n)
+
+
+def f8_dequantize_rows(kdim):
+    """f8 rows -> x [m][kdim] bf16 (bindings f8, x)."""
+    return Desc(kind=Kind.F8_DEQUANTIZE, k=kdim, form=1)
+
+
+def gemm_f8(kdim, n, out, rows=0, bm=0, bn=0, wm=0, wn=0, stages=0, band=0, ksplit=0):
+    """Y[m][n] = X.W^T of f8 rows X and an f8 matrix W (bindings state, W, X, Y, list, tiles, the
+    last two not read).  rows: those of a launch, which the defaults go by; any may be launched.
+    out Residual adds with one rounding; Swiglu: W [gate (n / 2) | up (n / 2)], h as f8 rows."""
+    return Desc(kind=Kind.GEMM_F8, k=kdim, n=n, out=out, rows_max=rows, bm=bm, bn=bn, wm=wm, wn=wn, dbuf=max(0, stages - 1),
+                band=band, ksplit=ksplit)
+
+
+def matvec_f8(kdim, n, out, mv_m=1, rows=0, split=0, waves=0, unroll=0):
+    """y[m][n] = x[m][kdim].W^T over an f8 matrix for m <= mv_m <= 16 rows of bf16 x, quantised as
+    f8_quantize_rows would (bindings W, x, y); zeros: the shape's defaults.  out Residual adds with
+    one rounding, Swiglu writes bf16."""
+    return Desc(kind=Kind.MATVEC_F8, k=kdim, n=n, out=out, mv_m=mv_m, rows=rows, split=split, mv_waves=waves, unroll=unroll)
+
+
+def experts_f8(kdim, n, out, rows_of, top_k, experts, rows_max, bm, **form):
+    """The routed experts' product over 8-bit matrices for blocks of up to rows_max rows, over tiles
+    of moe_sort with this bm (f8_tile_rows; bindings state, W of every expert, X, Y, list, tiles):
+    bm 16 matvec_f8's form, which takes bf16 rows and with out Swiglu writes them; 32 to 256
+    gemm_f8's, f8 rows."""
+    common = dict(k=kdim, n=n, out=out, rows_of=rows_of, top_k=top_k, experts=experts, rows_max=rows_max,
+                  tiles=moe_tiles(rows_max, top_k, experts, bm))
+    if bm == 16:
+        return Desc(kind=Kind.MATVEC_F8, mv_m=16, **common, **form)
+    return Desc(kind=Kind.GEMM_F8, bm=bm, **common, **form)
+
+
+def route_topk(experts, top_k, score=Score.Softmax, bias=False, groups=1, top_groups=None, group_top=1, renorm=True, scale=1.0,
+               f32=False):
+    """Routing to experts (HB_KIND_ROUTE_TOPK): the top_k of softmax or sigmoid scores (bf16, or f32),
+    plus a bias in the choice if any, among the top_groups groups of the largest best (group_top 1)
+    or two best summed (2); weights renormalised over the chosen if renorm, times scale (bindings
+    scores, route[, bias])."""
+    if group_top not in (1, 2):
+        raise HerbertError(HB_ERR_INVALID, "route_topk: a group's best one or two experts")
+    bits = struct.unpack("<I", struct.pack("<f", scale))[0]
+    if not bits:
+        raise HerbertError(HB_ERR_INVALID, "route_topk: a scale of 0")
+    form = int(score) | (2 if bias else 0) | (4 if renorm else 0) | (8 if f32 else 0) | (16 if group_top == 2 else 0)
+    return Desc(kind=Kind.ROUTE_TOPK, experts=experts, top_k=top_k, form=form, bm=groups, bn=groups if top_groups is None else top_groups,
+                eps_bits=bits)
 
 
 def block_norm(d, eps, plus_one=False, post=False, pre=True, gate=Gate.Off, scales=False):

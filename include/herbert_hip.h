@@ -114,8 +114,49 @@ enum hb_kind {
     HB_KIND_Q4_DEQUANTIZE = 16, /* q4 -> W [n][k] bf16, (q - 8) * s rounded once; m = matrices */
     HB_KIND_MATVEC_Q4 = 17,     /* matvec_q4: y[m][n] = x[m][k].W^T, m <= mv_m <= 16; or the
                                  * experts' over moe_sort's tiles of 16 rows (rows_of) */
-    HB_KIND_BLOCK_NORM = 18     /* a block's post norm, its gate, the residual add and the next
+    HB_KIND_BLOCK_NORM = 18,    /* a block's post norm, its gate, the residual add and the next
                                  * block's norm, rows of n (enum hb_norm_parts in `form`) */
+    HB_KIND_ROUTE_TOPK = 19,    /* routing to experts by softmax or sigmoid scores, with a bias,
+                                 * groups, renormalised weights (enum hb_route_parts in `form`) */
+    /* 8-bit floating point (OCP e4m3) with f32 scales, an element = code * scale.
+     * Of a group's bf16 elements, with a = max(|largest|, 2^-100): scale = a /
+     * 448, code = the e4m3 nearest to 448 x / a, ties to even; a group with a
+     * NaN or an infinity stands for NaN.  k a multiple of 16.
+     * "f8 rows" (activations): a row = its k codes, then the scales of its
+     * groups of 128 along k, their count rounded up to a multiple of 4
+     * (hb_f8_row_bytes).  "f8 matrix" (weights): the codes [n][k], then the
+     * scales [ceil(n/128)][ceil(k/128)] of its blocks of 128 x 128
+     * (hb_f8_bytes): what an 8-bit checkpoint holds, one after the other. */
+    HB_KIND_F8_QUANTIZE = 20,   /* form 0: W [n][k] bf16 -> f8 matrix, m = matrices; HB_F8_ROWS: x
+                                 * [m][k] bf16 -> f8 rows */
+    HB_KIND_F8_DEQUANTIZE = 21, /* the same back, code * scale rounded once to bf16 */
+    HB_KIND_GEMM_F8 = 22,       /* Y[m][n] = X.W^T of f8 rows X and an f8 matrix W, f32 sums; dense,
+                                 * or the experts' over moe_sort's tiles of bm rows (rows_of) */
+    HB_KIND_MATVEC_F8 = 23      /* the same for m <= mv_m <= 16 rows of bf16 x, quantised as they are
+                                 * loaded; or the experts' over tiles of 16 rows (rows_of) */
+};
+
+enum hb_f8_form { HB_F8_MATRIX = 0, HB_F8_ROWS = 1 };
+
+/* HB_KIND_ROUTE_TOPK: of the scores s [m][experts] (bf16, or f32), per row
+ *   p = softmax(s) or sigmoid(s),  c = p, or p + bias
+ *   groups (hb_desc.bm, 0 = 1) of consecutive experts: a group's score its
+ *     largest c, or the sum of its two largest; the `bn` (0 = all) groups of the
+ *     largest scores stay
+ *   the top_k experts of largest c in them; ties, of groups too, to the lowest index
+ *   w = p, or p over the sum of the chosen p, times the f32 in eps_bits (0 = 1)
+ * as ROUTE's rows: the experts in increasing order, then the f32 bits of their
+ * weights (not rounded to bf16).  An order that hangs on p is that of p in 64
+ * bits.  A score of NaN or -inf masks its expert: its p is 0 and, as those
+ * outside the groups that stay, it is chosen only where fewer than top_k others
+ * are left, the lowest index first, with weight 0.  Experts 1..1024, top_k
+ * 1..32, up to 64 groups. */
+enum hb_route_parts {
+    HB_ROUTE_SIGMOID = 1,
+    HB_ROUTE_BIAS = 2,      /* f32 [experts], a third binding */
+    HB_ROUTE_RENORM = 4,
+    HB_ROUTE_F32 = 8,       /* f32 scores */
+    HB_ROUTE_GROUP_TWO = 16 /* a group's score the sum of its two largest c */
 };
 
 /* HB_KIND_BLOCK_NORM's parts, in hb_desc.form.  Per row, in f32:
@@ -186,7 +227,7 @@ typedef struct hb_desc {
      * mv_waves (1, 2, 4, 8 or 16), unroll tiles of 128 K in flight (1..4); 0
      * = what the shape calls for.  bk = the weights' group, 0 = 32.  These
      * fix the order of a row's sums, which depends neither on the launch's
-     * rows nor on the other rows. */
+     * rows nor on the other rows.  MATVEC_F8: as MATVEC_Q4, rows 16, 32 or 64. */
     uint32_t mv_m, split, persist, rows, form;
     /* MoE: slots per row (top_k), experts, the tile table's capacity
      * (moe_tiles, prefill.rs:832-835), rows of the largest block. */
@@ -282,18 +323,27 @@ double hb_compile_seconds(hb_gpu *gpu);
  *   RMSNORM: x, w, y (eps_bits, plus_one of the descriptor)
  *   Q4_QUANTIZE: W, q4    Q4_PACK: codes, scales, q4    Q4_DEQUANTIZE: q4, W
  *   MATVEC_Q4: q4, x, y; over experts: state, q4 [experts], X, Y, list, tiles
+ *   ROUTE_TOPK: scores, route[, bias]
+ *   F8_QUANTIZE: W or x, f8    F8_DEQUANTIZE: f8, W or x
+ *   GEMM_F8: state, W, X, Y, list, tiles (dense: the last two not read)
+ *   MATVEC_F8: W, x, y; over experts: state, W [experts], X, Y, list, tiles
  *   BLOCK_NORM: x, y, xo, then those its parts name, in this order: h (PRE),
  *     w_post (POST), gate, scales (2 f32, SCALES), w_pre (PRE).  xo may be x
  *     or y, h may be y or x, or either an element gate, as a whole; no other
  *     overlap.
- * The bindings of these five start at a multiple of their element (2 bytes,
- * f32 and u32 4, q4 16), and what a launch writes overlaps nothing else it
+ * The bindings of these (ROUTE_TOPK, Q4_*, F8_*, GEMM_F8, MATVEC_Q4 and _F8,
+ * BLOCK_NORM) start at a multiple of their element (2 bytes,
+ * f32 and u32 4, q4, f8 matrices and f8 rows 16), and what a launch writes overlaps nothing else it
  * binds: both are checked.  Of MATVEC_Q4: HB_OUT_BF16, _F32, _RESIDUAL
  * (y = rne(y + sum), one rounding) and _SWIGLU (n / 2 a multiple of 16, h =
  * rne(g * sigmoid(g) * u) of the f32 sums).  The sums go through
  * 31 |x|: an infinite x, or 128 of them past 2^116, give NaN.  Over experts (rows_of HB_ROWS_GATHER: x rows through the list,
  * y rows in sorted order; HB_ROWS_SCATTER: the other way round) the table is
  * one of tiles of up to 16 rows; y rows of no tile are left as they are.
+ * Of MATVEC_F8 the same Outs, with n / 2 a multiple of 128 for _SWIGLU; of
+ * GEMM_F8 too, whose _SWIGLU (dense or gathered) writes h, rounded to bf16 and
+ * quantised, as f8 rows: the next GEMM_F8's X.  Its tiles' rows are bm, the
+ * sort's.  X and each W of a GEMM_F8 hold less than 2 GiB.
  * `m` is the rows of the block (the kernels read state[3], never beyond m).
  * A split-K GEMM (ksplit > 1) launched over more rows than any earlier
  * split launch on this context first grows the context's workspace: the
@@ -340,6 +390,16 @@ int hb_sync(hb_gpu *gpu);
  * multiple of 8, group 32, 64 or 128), 0 for a shape the kernels refuse.
  * Matrices of one shape stand one after the other at this distance. */
 uint64_t hb_q4_bytes(uint32_t k, uint32_t n, uint32_t group);
+
+/* Bytes of an f8 matrix of n rows of k (k a multiple of 16; matrices of one
+ * shape stand one after the other at this distance; the scales at n k) and of
+ * a row of f8 rows; 0 for a shape the kernels refuse. */
+uint64_t hb_f8_bytes(uint32_t k, uint32_t n);
+uint64_t hb_f8_row_bytes(uint32_t k);
+/* The rows per expert tile (moe_sort's bm) of the 8-bit experts for blocks of
+ * up to `rows` rows: 16 for MATVEC_F8, which takes and writes bf16 rows
+ * between the two products, else the bm of GEMM_F8, which takes f8 rows. */
+uint32_t hb_f8_tile_rows(uint32_t rows, uint32_t top_k, uint32_t experts);
 
 /* ---- synthetic inputs (host side, no GPU) ---- */
 /* n bf16 values ~ N(0, std^2): splitmix64(seed) -> two uniforms -> Box-Muller
@@ -473,7 +533,10 @@ int hb_engine_experts(hb_engine *engine, uint32_t experts, uint32_t top_k, uint3
  * [m][hidden] bf16.  Every launch's bindings are checked first.  Experts in
  * 4 bits: kernels[1] and [2] of kind HB_KIND_MATVEC_Q4 over a sort of
  * 16-row tiles, w_gate_up and w_down the packed matrices of all experts; a
- * gate|up with HB_OUT_SWIGLU writes EHB itself. */
+ * gate|up with HB_OUT_SWIGLU writes EHB itself.  Experts in 8 bits: as those
+ * in 4 with HB_KIND_MATVEC_F8; or kernels[1] (HB_OUT_SWIGLU) and [2] of kind
+ * HB_KIND_GEMM_F8 over a sort of their bm rows, kernels[3] the F8_QUANTIZE of
+ * x's rows, which writes them to xs [m]; ehb then holds f8 rows. */
 int hb_moe_experts_run(hb_gpu *gpu, const int32_t kernels[4], int32_t swiglu, int32_t combine,
                        const hb_moe_io *io, hb_range out, uint32_t m);
 
