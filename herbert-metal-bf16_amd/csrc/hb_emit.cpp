@@ -87,9 +87,9 @@ static void q4_defaults(hb_desc* d) {
     if (!d->unroll) d->unroll = d->rows == 16 ? 2 : 1;
 }
 
-// f8 rows and matrices (f8.h): a row's codes and its padded scales; a matrix's
+// f8 rows and matrices (f8.h): a row's codes and scales in whole lines; a matrix's
 // codes and its blocks' scales.
-static uint64_t f8_row_bytes(uint64_t k) { return k + ((k + 127) / 128 + 3) / 4 * 16; }
+static uint64_t f8_row_bytes(uint64_t k) { return (k + (k + 127) / 128 * 4 + 127) / 128 * 128; }
 static uint64_t f8_matrix_bytes(uint64_t k, uint64_t n) {
     return n * k + ((n + 127) / 128 * ((k + 127) / 128) + 3) / 4 * 16;
 }
@@ -121,12 +121,13 @@ static void gemm_f8_defaults(hb_desc* d) {
     if (!d->wn) d->wn = swi || d->wm == 1 ? 4 : 2;
     if (!d->dbuf) d->dbuf = d->bm + d->bn >= 384 ? 1 : 2;
     if (!d->band) d->band = 4;
+    if (!d->mfma) d->mfma = 16;
 }
 
 // What a GEMM_F8 workgroup holds in LDS.
 static uint64_t gemm_f8_lds(const hb_desc& d) {
     const uint32_t blocks = d.out == HB_OUT_SWIGLU ? 2 : d.bn % 128 == 0 ? d.bn / 128 : cdiv(d.bn, 128) + (128 % d.bn != 0);
-    return (uint64_t)(d.dbuf + 1) * (d.bm + d.bn) * 128 + d.bm * 64 + (uint64_t)blocks * cdiv(d.k, 128) * 4;
+    return (uint64_t)(d.dbuf + 1) * (d.bm + d.bn) * 128 + d.bm * 64 + (uint64_t)blocks * cdiv(cdiv(d.k, 128), 64) * 256;
 }
 
 hb_desc with_defaults(const hb_desc& in) {
@@ -615,7 +616,8 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             if (swi && (d.n % 256 || d.rows_of == HB_ROWS_SCATTER))
                 return fail(HB_ERR_UNSUPPORTED, "gemm_f8 Out::Swiglu: gate and up rows each a multiple of 128, no scatter");
             if (d.bm > 256 || !pow2(d.bm) || d.bm < 32 || d.bn > 256 || d.bn % 32 || !d.wm || !d.wn || d.wm * d.wn > 16 ||
-                d.bm % (d.wm * 16) || d.bn % (d.wn * 16) || (swi && (d.bn != 256 || d.bn / d.wn % 32)))
+                (d.mfma != 16 && d.mfma != 32) || d.bm % (d.wm * d.mfma) || d.bn % (d.wn * d.mfma) ||
+                (swi && (d.bn != 256 || d.bn / d.wn % (2 * d.mfma))))
                 return fail(HB_ERR_UNSUPPORTED, "gemm_f8: tiles of 32 to 256 X rows (a power of 2) by up to 256 W rows (Out::Swiglu 256), "
                                                 "whole fragments of 16 a wave");
             if (d.dbuf < 1 || d.dbuf > 3 || !d.band || gemm_f8_lds(d) > 160 * 1024)
@@ -633,8 +635,10 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             } else if (d.ksplit > 1) {
                 rows = "_ks" + std::to_string(d.ksplit);
             }
-            snprintf(name, sizeof name, "gemm_f8_%ux%u_%s_t%ux%u_w%ux%u_d%u_b%u%s", d.k, d.n, swi ? "sw" : out_tag(d.out), d.bn,
-                     d.bm, d.wn, d.wm, d.dbuf, d.band, rows.c_str());
+            if (d.sched > 1 || (d.sched && (d.dbuf != 1 || d.bn / d.wn < 4 * d.mfma)))
+                return fail(HB_ERR_UNSUPPORTED, "gemm_f8 (fragments ahead): two stages, four fragments of W a wave");
+            snprintf(name, sizeof name, "gemm_f8_%ux%u_%s_t%ux%u_w%ux%u_x%u_d%u_b%u%s%s", d.k, d.n, swi ? "sw" : out_tag(d.out), d.bn,
+                     d.bm, d.wn, d.wm, d.mfma, d.dbuf, d.band, d.sched ? "_fa" : "", rows.c_str());
             e->name = name;
             e->source = "gemm_f8.hip";
             e->threads = 64 * d.wm * d.wn;
@@ -642,7 +646,8 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             e->defines = {D("HB_K", d.k),   D("HB_N", d.n),   D("HB_OUT", d.ksplit > 1 ? (uint32_t)HB_OUT_F32 : d.out),
                           D("HB_ROWS", d.rows_of), D("HB_TOPK", experts ? d.top_k : 1), D("HB_E", experts ? d.experts : 1),
                           D("HB_BM", d.bm), D("HB_BN", d.bn), D("HB_WM", d.wm), D("HB_WN", d.wn),
-                          D("HB_STAGES", d.dbuf + 1), D("HB_BAND", d.band), D("HB_KSPLIT", d.ksplit > 1 ? d.ksplit : 1)};
+                          D("HB_STAGES", d.dbuf + 1), D("HB_BAND", d.band), D("HB_KSPLIT", d.ksplit > 1 ? d.ksplit : 1),
+                          D("HB_SCHED", d.sched), D("HB_MFMA", d.mfma)};
             return HB_OK;
         }
         case HB_KIND_ROUND_PROBE:

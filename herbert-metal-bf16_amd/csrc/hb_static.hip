@@ -67,14 +67,13 @@ extern "C" int hb_moe_experts_run_static(hb_gpu* g, const int32_t kernels[4], in
     // The table's capacity: what the sort and the GEMMs were built for.
     const uint64_t cap_sort = (sd->rows_max * (uint64_t)sd->top_k + sd->bm - 1) / sd->bm + sd->experts;
     const uint64_t cap = cap_sort > gd->tiles ? cap_sort : gd->tiles;
-    // (8-bit SwiGLU rows are no longer than bf16 ones.)
     // Layout: state, list, tiles, xs, egu, ehb, ey (each 256-byte aligned).
     const uint64_t sz[7] = {kStateBytes,
                             pairs * 4,
                             (1 + 3 * (cap > dd->tiles ? cap : dd->tiles)) * 4,
                             !gather ? 0 : gd->kind == HB_KIND_GEMM_F8 ? m * hb_f8_row_bytes(gd->k) : pairs * hidden * 2,
                             fused ? 0 : pairs * 2 * inter * 2,
-                            pairs * inter * 2,
+                            pairs * (gd->kind == HB_KIND_GEMM_F8 ? hb_f8_row_bytes((uint32_t)inter) : inter * 2),
                             pairs * hidden * 2};
     uint64_t off[7], total = 0;
     for (int i = 0; i < 7; i++) {

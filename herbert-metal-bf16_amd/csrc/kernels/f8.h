@@ -5,8 +5,8 @@
 //   s = a / 448 (f32),  q = the e4m3 nearest to 448 x / a, ties to even.
 //
 // A group with a NaN or an infinity stands for NaN.  "f8 rows" hold
-// activations: a row's k codes, then the f32 scales of its groups of 128, the
-// count of scales rounded up to a multiple of 4.  An "f8 matrix" holds weights:
+// activations: a row's k codes, then the f32 scales of its groups of 128, in
+// all whole lines of 128 bytes.  An "f8 matrix" holds weights:
 // the codes [n][k], then the f32 scales [ceil(n / 128)][ceil(k / 128)] of its
 // blocks of 128 x 128, in all a multiple of 16 bytes.  k is a multiple of 16.
 #pragma once
@@ -16,7 +16,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef u16 u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr u32 f8_blocks(u32 k) { return (k + 127) / 128; }
-constexpr u64 f8_row_bytes(u64 k) { return k + ((k + 127) / 128 + 3) / 4 * 16; }
+constexpr u64 f8_row_bytes(u64 k) { return (k + (k + 127) / 128 * 4 + 127) / 128 * 128; }
 constexpr u64 f8_matrix_bytes(u64 k, u64 n) {
     return n * k + ((n + 127) / 128 * ((k + 127) / 128) + 3) / 4 * 16;
 }

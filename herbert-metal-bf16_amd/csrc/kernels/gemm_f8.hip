@@ -36,9 +36,10 @@ constexpr u32 K = HB_K, N = HB_N;
 constexpr int OUT = HB_OUT, ROWS = HB_ROWS;
 constexpr u32 TOPK = HB_TOPK, BM = HB_BM, BN = HB_BN, WM = HB_WM, WN = HB_WN;
 constexpr u32 NWV = WM * WN, NTH = 64 * NWV, NS = HB_STAGES, KSP = HB_KSPLIT;
-constexpr u32 TM = BM / WM, TN = BN / WN, IM = TM / 16, IN = TN / 16;
+constexpr u32 FM = HB_MFMA, FR = FM * FM / 64, MK = FM / 16;  // a block of FM x FM: sums a lane, MFMAs
+constexpr u32 TM = BM / WM, TN = BN / WN, IM = TM / FM, IN = TN / FM;
 constexpr bool SWI = OUT == 3;
-constexpr u32 KB = f8_blocks(K), NB = f8_blocks(N), NOUT = SWI ? N / 2 : N, BF = SWI ? BN / 2 : BN;
+constexpr u32 KB = f8_blocks(K), KBP = (KB + 63) / 64 * 64, NB = f8_blocks(N), NOUT = SWI ? N / 2 : N, BF = SWI ? BN / 2 : BN;
 constexpr u32 NTILES = (NOUT + BF - 1) / BF;
 constexpr u64 XROW = f8_row_bytes(K), HROW = f8_row_bytes(NOUT), MATRIX = f8_matrix_bytes(K, N);
 constexpr u32 XST = BM * 8, WST = BN * 8;                 // 16-byte chunks of a stage
@@ -47,7 +48,26 @@ constexpr u32 XLMAX = (NXL + NWV - 1) / NWV, WLMAX = (NWL + NWV - 1) / NWV;
 constexpr u32 LMIN = NXL / NWV + NWL / NWV;               // loads a stage of every wave
 constexpr u32 NSL = BM / 32, SLMAX = (NSL + NWV - 1) / NWV;  // wave loads of eight K tiles' X scales
 constexpr u32 SWR = SWI ? 2 : BN % 128 == 0 ? BN / 128 : (BN + 127) / 128 + (128 % BN != 0);  // W's blocks of a tile
-static_assert(K % 16 == 0 && BM % 32 == 0 && BN % 16 == 0 && TM % 16 == 0 && TN % 16 == 0, "tile");
+constexpr u32 LDS = NS * (XST + WST) + BM * 4 + SWR * KBP / 4;  // 16-byte chunks: stages, scales
+// Outputs of two bytes whose rows are whole chunks leave through LDS, a row
+// (and a chunk between them, so that the rows' banks differ) at EPIROW bytes.
+constexpr u32 EPIROW = BN * 2 + 16;
+constexpr bool EPI_LDS = OUT == 0 && NOUT % 8 == 0 && BM * EPIROW <= 160 * 1024;
+constexpr u32 EPI = EPI_LDS ? BM * EPIROW / 16 : 0;
+constexpr u32 LROWS = NWV * 8;                            // rows between a wave's loads
+#ifndef HB_SCHED
+#define HB_SCHED 0
+#endif
+constexpr bool AHEAD = HB_SCHED == 1;
+// The W row of a tile's row r, from the tile's first column on: a wave's gate
+// rows stand before the up rows of the same features.
+constexpr u32 w_row(u32 r) {
+    return SWI ? (r % TN >= TN / 2 ? NOUT : 0) + r / TN * (TN / 2) + r % TN % (TN / 2) : r;
+}
+// Its rows LROWS apart lie as far from each other wherever they start.
+static_assert(!SWI || LROWS % TN == 0 || (TN / 2) % LROWS == 0, "SwiGLU rows of a wave's loads");
+static_assert(!AHEAD || (NS == 2 && IN >= 4), "fragments ahead: two stages, four fragments of W a wave");
+static_assert(K % 16 == 0 && BM % 32 == 0 && BN % 16 == 0 && TM % FM == 0 && TN % FM == 0, "tile");
 static_assert(!SWI || (BN == 256 && IN % 2 == 0 && N % 256 == 0 && KSP == 1 && ROWS != 2), "SwiGLU");
 static_assert(KSP == 1 || (OUT == 1 && ROWS == 0 && N % 4 == 0), "split K: f32 partial sums");
 static_assert(NS >= 2 && NS <= 4, "stages");
@@ -92,11 +112,11 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
                                                             const unsigned char* __restrict__ X, void* __restrict__ Yv,
                                                             const u32* __restrict__ list, const u32* __restrict__ tiles,
                                                             u32 m_launch) {
-    __shared__ u32x4 lds[NS * (XST + WST)];
-    __shared__ u32x4 sscale[2 * BM * 2];   // X's scales: [place][row][K tile of eight]
-    __shared__ float wscale[SWR * KB];
+    __shared__ u32x4 lds[LDS > EPI ? LDS : EPI];
     u32x4* const sXa = lds;
     u32x4* const sWa = lds + NS * XST;
+    u32x4* const sscale = sWa + NS * WST;                // X's scales: [place][row][K tile of eight]
+    float* const wscale = (float*)(sscale + 2 * BM * 2);
     const u32 tid = threadIdx.x, lane = tid & 63u;
     const u32 wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const u32 wm = wave % WM, wn = wave / WM;
@@ -146,7 +166,7 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
     }
     const u32 n0 = gn * BF;
 
-    // Row r of the tile in X, and the W row of its row r; past N the last one.
+    // Row r of an experts' tile in X.
     auto x_row = [&](u32 r) HB_INLINE -> u32 {
         if constexpr (ROWS == 1) {
             const u32 pr = list[row0 + r] / TOPK;
@@ -154,39 +174,34 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
         }
         return row0 + r;
     };
-    auto w_row = [&](u32 r) HB_INLINE -> u32 {
-        if constexpr (SWI) {
-            const u32 t = r % TN, i = t / 16, up = i >= IN / 2 ? 1u : 0u;
-            return up * NOUT + n0 + (r / TN) * (TN / 2) + (i - up * (IN / 2)) * 16 + t % 16;
-        }
-        return n0 + r < N ? n0 + r : N - 1;
-    };
     // W's block of 128 rows that fragment i of wave wn stands in, of the tile's.
     const u32 nb0 = n0 / 128;
     auto w_block = [&](u32 i) HB_INLINE -> u32 {
         if constexpr (SWI) return i >= IN / 2 ? 1u : 0u;
-        return (n0 + wn * TN + i * 16) / 128 - nb0;
+        if constexpr (BN % 128 == 0 && 128 % TN == 0) return wn * TN / 128;  // one for all i
+        return (n0 + wn * TN + i * FM) / 128 - nb0;
     };
 
-    // This wave's loads of a stage: LDS slot p of the operand's stage holds
-    // (row p / 8, chunk p % 8 ^ row >> 1).  Rows past the tile's at an offset
-    // past the resource's range: zeros without a memory access.
+    // This wave's loads of a stage, wave loads wave, wave + NWV, ..: LDS slot p
+    // of the operand's stage holds (row p / 8, chunk p % 8 ^ row >> 1), so that a
+    // lane's chunk is the same in each, and its rows LROWS apart: one address
+    // a lane and constants.  Rows past the operand's end lie past its
+    // resource's range, an experts' tile's rows past its own are put there:
+    // zeros without a memory access.  (The scalar offset, which the range
+    // check takes off the range, stays within a row.)
     constexpr u32 AWAY = 0x80000000u;
-    u32 xoff[XLMAX], woff[WLMAX], soff[SLMAX];
+    const u32 lr = wave * 8 + lane / 8, cc = (lane % 8) ^ ((lr >> 1) & 7u);
+    u32 xoff[ROWS == 0 ? 1 : XLMAX], soff[SLMAX];
 #pragma unroll
-    for (u32 i = 0; i < XLMAX; i++) {
-        const u32 p = (wave + NWV * i) * 64 + lane, r = p / 8, cc = (p % 8) ^ ((r >> 1) & 7u);
-        xoff[i] = r < rows ? (u32)(x_row(r) * XROW) + cc * 16 : AWAY;
+    for (u32 i = 0; i < (ROWS == 0 ? 1 : XLMAX); i++) {
+        const u32 r = lr + LROWS * i;
+        xoff[i] = ROWS == 0 ? (u32)((row0 + r) * XROW) + cc * 16 : r < rows ? (u32)(x_row(r) * XROW) + cc * 16 : AWAY;
     }
-#pragma unroll
-    for (u32 i = 0; i < WLMAX; i++) {
-        const u32 p = (wave + NWV * i) * 64 + lane, r = p / 8, cc = (p % 8) ^ ((r >> 1) & 7u);
-        woff[i] = r < BN ? w_row(r) * K + cc * 16 : AWAY;
-    }
+    const u32 woff = (w_row(lr) + n0) * K + cc * 16;
 #pragma unroll
     for (u32 i = 0; i < SLMAX; i++) {
-        const u32 p = (wave + NWV * i) * 64 + lane, r = p / 2;
-        soff[i] = r < rows ? (u32)(x_row(r) * XROW) + K + (p % 2) * 16 : AWAY;
+        const u32 r = (wave + NWV * i) * 32 + lane / 2;
+        soff[i] = ROWS == 0 || r < rows ? (u32)((ROWS == 0 ? row0 + r : x_row(r)) * XROW) + K + (lane % 2) * 16 : AWAY;
     }
     const u64 xbytes = (u64)(ROWS == 2 ? m_launch * TOPK : m_launch) * XROW;
     const __amdgpu_buffer_rsrc_t rX = __builtin_amdgcn_make_buffer_rsrc((void*)X, (short)0, (int)xbytes, 0x00020000);
@@ -195,9 +210,8 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
     typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
     auto lds_addr = [&](u32x4* p) HB_INLINE -> u32 { return (u32)(u64)(lds_u32x4*)p; };
     // The last K tile may be short: its chunks past K are zeros.
-    auto cut = [&](u32 kt, u32 i, u32 off) HB_INLINE -> u32 {
+    auto cut = [&](u32 kt, u32 off) HB_INLINE -> u32 {
         if constexpr (K % 128 == 0) return off;
-        const u32 p = (wave + NWV * i) * 64 + lane, r = p / 8, cc = (p % 8) ^ ((r >> 1) & 7u);
         return kt == KB - 1 && cc * 16 >= K % 128 ? AWAY : off;
     };
     const u32 kt0 = part * KB / KSP, kt1 = (part + 1) * KB / KSP;
@@ -210,115 +224,239 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
                             "s"(c * 32) : "memory");
         }
     };
-    auto load_tile = [&](u32 kt, u32 st) HB_INLINE {
+    auto load_x = [&](u32 kt, u32 st) HB_INLINE {
         // The scales first, so that they have landed when the tile has.
         if (kt % 8 == 0 || kt == kt0) load_scales(kt / 8);
+        const u32 xo = cut(kt, xoff[0]);
 #pragma unroll
         for (u32 i = 0; i < XLMAX; i++) {
             if (NXL % NWV && wave + NWV * i >= NXL) continue;
             asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                         :: "s"(lds_addr(&sXa[st * XST + (wave + NWV * i) * 64])), "v"(cut(kt, i, xoff[i])), "s"(rX),
-                            "s"(kt * 128) : "memory");
-        }
-#pragma unroll
-        for (u32 i = 0; i < WLMAX; i++) {
-            if (NWL % NWV && wave + NWV * i >= NWL) continue;
-            asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                         :: "s"(lds_addr(&sWa[st * WST + (wave + NWV * i) * 64])), "v"(cut(kt, i, woff[i])), "s"(rW),
+                         :: "s"(lds_addr(&sXa[st * XST + (wave + NWV * i) * 64])),
+                            "v"(ROWS == 0 ? xo + i * LROWS * (u32)XROW : cut(kt, xoff[ROWS == 0 ? 0 : i])), "s"(rX),
                             "s"(kt * 128) : "memory");
         }
     };
+    // W's loads first, first + step, ..
+    auto load_w = [&](u32 kt, u32 st, u32 first, u32 step) HB_INLINE {
+        const u32 wo = cut(kt, woff);
+#pragma unroll
+        for (u32 i = first; i < WLMAX; i += step) {
+            if (NWL % NWV && wave + NWV * i >= NWL) continue;
+            asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                         :: "s"(lds_addr(&sWa[st * WST + (wave + NWV * i) * 64])), "v"(wo + w_row(LROWS * i) * K), "s"(rW),
+                            "s"(kt * 128) : "memory");
+        }
+    };
+    auto load_tile = [&](u32 kt, u32 st) HB_INLINE {
+        load_x(kt, st);
+        load_w(kt, st, 0, 1);
+    };
 
-    f32x4 acc[IN][IM];
+    float acc[IN][IM][FR];
 #pragma unroll
     for (u32 i = 0; i < IN; i++)
 #pragma unroll
-        for (u32 j = 0; j < IM; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const u32 fr = lane & 15u, fc = lane >> 4, fsw = (fr >> 1) & 7u;
-    const u32 wbase = (wn * TN + fr) * 8, xbase = (wm * TM + fr) * 8;
-    auto fragment = [&](const u32x4* p) HB_INLINE -> i32x8 {
-        const u32x4 a = p[fc ^ fsw], b = p[(fc + 4) ^ fsw];
-        return i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
-    };
-
-    // Prologue: tiles 0 .. NS - 2 in flight, W's scales into LDS.
+        for (u32 j = 0; j < IM; j++)
 #pragma unroll
-    for (u32 t = 0; t + 1 < NS; t++)
-        if (kt0 + t < kt1) load_tile(kt0 + t, t);
-    {
-        const float* ws = (const float*)(W + expert * MATRIX + (u64)N * K);
-        for (u32 i = tid; i < SWR * KB; i += NTH) {
-            u32 b = SWI ? (i / KB) * (NOUT / 128) + nb0 : nb0 + i / KB;
-            b = b < NB ? b : NB - 1;
-            wscale[i] = ws[(u64)b * KB + i % KB];
+            for (u32 e = 0; e < FR; e++) acc[i][j][e] = 0.0f;
+    const u32 fr = lane % FM, fc = lane / FM, fsw = (fr >> 1) & 7u;
+    const u32 wbase = (wn * TN + fr) * 8, xbase = (wm * TM + fr) * 8;
+    struct Fragment {
+        i32x8 k[MK];
+    };
+    auto fragment = [&](const u32x4* p) HB_INLINE -> Fragment {
+        Fragment f;
+#pragma unroll
+        for (u32 q = 0; q < MK; q++) {
+            const u32x4 a = p[(fc + 4 * q) ^ fsw], b = p[(fc + 4 / MK + 4 * q) ^ fsw];
+            f.k[q] = i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
         }
-    }
-    WAIT_VM(0);
-    STAGE_BARRIER();
+        return f;
+    };
+    typedef float block_t __attribute__((ext_vector_type(FR)));
 
-    u32 st = 0;
-    for (u32 kt = kt0; kt < kt1; kt++) {
-        // Tile kt + NS - 1 into the stage that tile kt - 1 used: every wave
-        // has passed the barrier after its last read of it.
-        const bool more = kt + NS - 1 < kt1;
-        if (more) load_tile(kt + NS - 1, st == 0 ? NS - 1 : st - 1);
+    float sx[IM];
+    Fragment xf[IM];
+    auto read_x = [&](u32 kt, u32 st) HB_INLINE {
         const u32x4* sX = sXa + st * XST + xbase;
-        const u32x4* sW = sWa + st * WST + wbase;
         const float* sc = (const float*)(sscale + (kt / 8 & 1u) * BM * 2) + (wm * TM + fr) * 8 + (kt & 7u);
-        float sx[IM];
-        i32x8 b[IM];
 #pragma unroll
         for (u32 j = 0; j < IM; j++) {
-            b[j] = fragment(sX + j * 128);
-            sx[j] = sc[j * 128];
+            xf[j] = fragment(sX + j * FM * 8);
+            sx[j] = sc[j * FM * 8];
         }
+    };
+    float last_sw = 0.0f;
+    auto product_of = [&](const Fragment& w, const Fragment& x) HB_INLINE -> block_t {
+        block_t t = {};
 #pragma unroll
-        for (u32 i = 0; i < IN; i++) {
-            const i32x8 a = fragment(sW + i * 128);
-            const float sw = wscale[w_block(i) * KB + kt];
+        for (u32 q = 0; q < MK; q++) {
+#if HB_MFMA == 16
+            t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.k[q], x.k[q], t, 0, 0, 0, 0, 0, 0);
+#else
+            t = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w.k[q], x.k[q], t, 0, 0, 0, 0, 0, 0);
+#endif
+        }
+        return t;
+    };
+    auto add = [&](u32 i, u32 j, const block_t& t, float s) HB_INLINE {
+#pragma unroll
+        for (u32 e = 0; e < FR; e++) {
+            acc[i][j][e] = __builtin_fmaf(s, t[e], acc[i][j][e]);
+            // Here and not later: the compiler would let blocks wait in
+            // registers and add them behind the next barrier.
+            if (AHEAD) asm volatile("" : "+v"(acc[i][j][e]));
+        }
+    };
+    // W's scales of the tile's blocks, a row of them KBP places apart, the same
+    // way; past a row's end come the next one's or zeros.
+    const __amdgpu_buffer_rsrc_t rS = __builtin_amdgcn_make_buffer_rsrc((void*)(W + expert * MATRIX + (u64)N * K), (short)0,
+                                                                        (int)(NB * KB * 4), 0x00020000);
+    auto w_scales = [&]() HB_INLINE {
+#pragma unroll
+        for (u32 i = 0; i < (SWR * (KBP / 64) + NWV - 1) / NWV; i++) {
+            const u32 q = wave + NWV * i, r = q / (KBP / 64), part64 = q % (KBP / 64);
+            if (r >= SWR) continue;
+            u32 b = nb0 + (SWI ? r * (NOUT / 128) : r);
+            b = b < NB ? b : NB - 1;
+            asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                         :: "s"(lds_addr((u32x4*)(wscale + q * 64))), "v"((b * KB + part64 * 64 + lane) * 4), "s"(rS) : "memory");
+        }
+    };
+
+    if constexpr (AHEAD) {
+        // One barrier a K tile, before its last LAST fragments of W: by then a
+        // wave holds those, so that the tile's stage is free for tile kt + 2,
+        // and tile kt + 1 has landed, so that X's fragments of it and W's first
+        // one are read while the last MFMAs run.
+        constexpr u32 LAST = IN / 4;
+        w_scales();
+        load_tile(kt0, 0);
+        if (kt0 + 1 < kt1) {
+            load_tile(kt0 + 1, 1);
+            WAIT_VM(LMIN);
+        } else {
+            WAIT_VM(0);
+        }
+        STAGE_BARRIER();
+        Fragment xa[IM], xb[IM], first;
+        float sa[IM], sb[IM];
+        auto ready = [&](u32 kt, u32 st, Fragment (&x)[IM], float (&sc)[IM]) HB_INLINE {
+            const u32x4* sX = sXa + st * XST + xbase;
+            const float* c = (const float*)(sscale + (kt / 8 & 1u) * BM * 2) + (wm * TM + fr) * 8 + (kt & 7u);
+            first = fragment(sWa + st * WST + wbase);
 #pragma unroll
             for (u32 j = 0; j < IM; j++) {
-                const f32x4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b[j], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-                const float s = sx[j] * sw;
-#pragma unroll
-                for (u32 e = 0; e < 4; e++) acc[i][j][e] = __builtin_fmaf(s, t[e], acc[i][j][e]);
+                x[j] = fragment(sX + j * FM * 8);
+                sc[j] = c[j * FM * 8];
             }
+        };
+        auto step = [&](u32 kt, u32 st, Fragment (&x)[IM], float (&sc)[IM], Fragment (&xn)[IM], float (&sn)[IM]) HB_INLINE {
+            const u32x4* sW = sWa + st * WST + wbase;
+            Fragment w[IN];
+            w[0] = first;
+            float sw = wscale[w_block(0) * KBP + kt];
+            block_t t[2];
+#pragma unroll
+            for (u32 i = 0; i < IN; i++) {
+                if (i + 1 < IN - LAST) w[i + 1] = fragment(sW + (i + 1) * FM * 8);
+                if (i + 1 == IN - LAST) {
+#pragma unroll
+                    for (u32 q = IN - LAST; q < IN; q++) w[q] = fragment(sW + q * FM * 8);
+                }
+                if (i == IN - LAST) {
+                    WAIT_VM(0);
+                    STAGE_BARRIER();
+                    if (kt + 2 < kt1) load_tile(kt + 2, st);
+                    ready(kt + 1, 1 - st, xn, sn);  // past the last tile: of a stage that nobody uses
+                }
+                if (!(BN % 128 == 0 && 128 % TN == 0 && !SWI) && i) sw = wscale[w_block(i) * KBP + kt];
+#pragma unroll
+                for (u32 j = 0; j < IM; j++) {
+                    const u32 q = i * IM + j;
+                    t[q % 2] = product_of(w[i], x[j]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (q) {
+                        const u32 p = q - 1;
+                        add(p / IM, p % IM, t[p % 2], sc[p % IM] * (p / IM == i ? sw : last_sw));
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                last_sw = sw;
+            }
+            add(IN - 1, IM - 1, t[(IN * IM - 1) % 2], sc[IM - 1] * sw);
+        };
+        ready(kt0, 0, xa, sa);
+        u32 kt = kt0;
+#pragma unroll 1
+        for (; kt + 1 < kt1; kt += 2) {
+            step(kt, 0, xa, sa, xb, sb);
+            step(kt + 1, 1, xb, sb, xa, sa);
         }
-        // Tile kt + 1 landed: at most the loads of the tiles after it are in
-        // flight.
-        if (more) WAIT_VM((NS - 2) * LMIN);
+        if (kt < kt1) step(kt, 0, xa, sa, xb, sb);
+        STAGE_BARRIER();
+    } else {
+        // W's scales and tiles 0 .. NS - 2 in flight, the first landed.
+        w_scales();
+#pragma unroll
+        for (u32 t = 0; t + 1 < NS; t++)
+            if (kt0 + t < kt1) load_tile(kt0 + t, t);
+        if (kt0 + NS - 1 <= kt1) WAIT_VM((NS - 2) * LMIN);
         else WAIT_VM(0);
         STAGE_BARRIER();
-        st = st + 1 == NS ? 0 : st + 1;
+        u32 st = 0;
+        for (u32 kt = kt0; kt < kt1; kt++) {
+            // Tile kt + NS - 1 into the stage that tile kt - 1 used: every wave
+            // has passed the barrier after its last read of it.
+            const bool more = kt + NS - 1 < kt1;
+            if (more) load_tile(kt + NS - 1, st == 0 ? NS - 1 : st - 1);
+            const u32x4* sW = sWa + st * WST + wbase;
+            read_x(kt, st);
+#pragma unroll
+            for (u32 i = 0; i < IN; i++) {
+                const Fragment wf = fragment(sW + i * FM * 8);
+                const float sw = wscale[w_block(i) * KBP + kt];
+#pragma unroll
+                for (u32 j = 0; j < IM; j++) add(i, j, product_of(wf, xf[j]), sx[j] * sw);
+            }
+            // Tile kt + 1 landed: at most the loads of the tiles after it are in
+            // flight.
+            if (more) WAIT_VM((NS - 2) * LMIN);
+            else WAIT_VM(0);
+            STAGE_BARRIER();
+            st = st + 1 == NS ? 0 : st + 1;
+        }
     }
 
     if constexpr (KSP > 1) Yv = (float*)Yv + (u64)part * m_launch * N;  // this part's slab
     if constexpr (SWI) {
         // h of the lane's features, rounded; the largest of each row over the
         // lane's, its column's other quads, and the waves of WN.
+        constexpr u32 NR = FR / 4;  // runs of four features a block
         u32* const tops = (u32*)lds;
-        u32x2 h[IN > 1 ? IN / 2 : 1][IM];
+        u32x2 h[IN > 1 ? IN / 2 : 1][IM][NR];
 #pragma unroll
         for (u32 j = 0; j < IM; j++) {
             u32 top = 0;
 #pragma unroll
-            for (u32 i = 0; i < IN / 2; i++) {
-                float gr[4], ur[4], hr[4];
+            for (u32 i = 0; i < IN / 2; i++)
 #pragma unroll
-                for (u32 e = 0; e < 4; e++) gr[e] = acc[i][j][e], ur[e] = acc[i + IN / 2][j][e];
-                swiglu_n<4>(gr, ur, hr);
-                h[i][j] = u32x2{pack_bf16x2(hr[0], hr[1]), pack_bf16x2(hr[2], hr[3])};
-                top = f8_max2(top, f8_max2(h[i][j].x & 0x7fff7fffu, h[i][j].y & 0x7fff7fffu));
-            }
+                for (u32 q = 0; q < NR; q++) {
+                    float hr[4];
+                    swiglu_n<4>(&acc[i][j][4 * q], &acc[i + IN / 2][j][4 * q], hr);
+                    h[i][j][q] = u32x2{pack_bf16x2(hr[0], hr[1]), pack_bf16x2(hr[2], hr[3])};
+                    top = f8_max2(top, f8_max2(h[i][j][q].x & 0x7fff7fffu, h[i][j][q].y & 0x7fff7fffu));
+                }
 #pragma unroll
-            for (u32 x = 16; x < 64; x *= 2) top = f8_max2(top, (u32)__shfl_xor((int)top, x, 64));
+            for (u32 x = FM; x < 64; x *= 2) top = f8_max2(top, (u32)__shfl_xor((int)top, x, 64));
             top = f8_max2(top, top >> 16) & 0xffffu;
-            if (fc == 0) tops[wn * BM + wm * TM + j * 16 + fr] = top;
+            if (fc == 0) tops[wn * BM + wm * TM + j * FM + fr] = top;
         }
         STAGE_BARRIER();
 #pragma unroll
         for (u32 j = 0; j < IM; j++) {
-            const u32 ml = wm * TM + j * 16 + fr;
+            const u32 ml = wm * TM + j * FM + fr;
             u32 top = 0;
 #pragma unroll
             for (u32 q = 0; q < WN; q++) top = tops[q * BM + ml] > top ? tops[q * BM + ml] : top;
@@ -327,24 +465,54 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
             unsigned char* y = (unsigned char*)Yv + (u64)(row0 + ml) * HROW;
 #pragma unroll
             for (u32 i = 0; i < IN / 2; i++)
-                *(u32*)(y + n0 + wn * (TN / 2) + i * 16 + 4 * fc) = f8_codes2<true>(h[i][j].y, s.inv, f8_codes2<false>(h[i][j].x, s.inv, 0));
+#pragma unroll
+                for (u32 q = 0; q < NR; q++)
+                    *(u32*)(y + n0 + wn * (TN / 2) + i * FM + q * 8 + 4 * fc) =
+                        f8_codes2<true>(h[i][j][q].y, s.inv, f8_codes2<false>(h[i][j][q].x, s.inv, 0));
             if (wn == 0 && fc == 0) *(float*)(y + NOUT + 4 * gn) = s.s;
+        }
+        return;
+    }
+    auto y_row = [&](u32 r) HB_INLINE -> u32 {
+        if constexpr (ROWS == 2) {
+            const u32 p = list[row0 + r];
+            return p < pairs ? p : pairs - 1;
+        }
+        return row0 + r;
+    };
+    if constexpr (EPI_LDS) {
+        // Past the barrier behind the last tile.
+        unsigned char* const t = (unsigned char*)lds;
+#pragma unroll
+        for (u32 j = 0; j < IM; j++)
+#pragma unroll
+            for (u32 i = 0; i < IN; i++)
+#pragma unroll
+                for (u32 q = 0; q < FR / 4; q++)
+                    *(u32x2*)(t + (wm * TM + j * FM + fr) * EPIROW + (wn * TN + i * FM + q * 8 + 4 * fc) * 2) =
+                        u32x2{pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])};
+        STAGE_BARRIER();
+        constexpr u32 CPR = BN / 8;
+        for (u32 c = tid; c < BM * CPR; c += NTH) {
+            const u32 r = c / CPR, n = n0 + c % CPR * 8;
+            if (r >= rows || n >= NOUT) continue;
+            const u32x4 v = *(const u32x4*)(t + r * EPIROW + c % CPR * 16);
+            __builtin_nontemporal_store(v, (u32x4*)((u16*)Yv + (u64)y_row(r) * NOUT + n));
         }
         return;
     }
 #pragma unroll
     for (u32 j = 0; j < IM; j++) {
-        const u32 ml = wm * TM + j * 16 + fr;
+        const u32 ml = wm * TM + j * FM + fr;
         if (ml >= rows) continue;
-        u32 yrow = row0 + ml;
-        if constexpr (ROWS == 2) {
-            const u32 s = list[row0 + ml];
-            yrow = s < pairs ? s : pairs - 1;
-        }
+        const u32 yrow = y_row(ml);
 #pragma unroll
-        for (u32 i = 0; i < IN; i++) {
-            const u32 n = n0 + wn * TN + i * 16 + 4 * fc;
-            if (n < NOUT) store4(Yv, yrow, n, acc[i][j]);
-        }
+        for (u32 i = 0; i < IN; i++)
+#pragma unroll
+            for (u32 q = 0; q < FR / 4; q++) {
+                const u32 n = n0 + wn * TN + i * FM + q * 8 + 4 * fc;
+                const float* v = &acc[i][j][4 * q];
+                if (n < NOUT) store4(Yv, yrow, n, f32x4{v[0], v[1], v[2], v[3]});
+            }
     }
 }

@@ -123,8 +123,7 @@ enum hb_kind {
      * 448, code = the e4m3 nearest to 448 x / a, ties to even; a group with a
      * NaN or an infinity stands for NaN.  k a multiple of 16.
      * "f8 rows" (activations): a row = its k codes, then the scales of its
-     * groups of 128 along k, their count rounded up to a multiple of 4
-     * (hb_f8_row_bytes).  "f8 matrix" (weights): the codes [n][k], then the
+     * groups of 128 along k, in all a multiple of 128 bytes (hb_f8_row_bytes).  "f8 matrix" (weights): the codes [n][k], then the
      * scales [ceil(n/128)][ceil(k/128)] of its blocks of 128 x 128
      * (hb_f8_bytes): what an 8-bit checkpoint holds, one after the other. */
     HB_KIND_F8_QUANTIZE = 20,   /* form 0: W [n][k] bf16 -> f8 matrix, m = matrices; HB_F8_ROWS: x

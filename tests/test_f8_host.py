@@ -26,7 +26,7 @@ def gpu(hb):
 
 
 def test_bytes(hb):
-    assert hb.f8_row_bytes(16) == 32 and hb.f8_row_bytes(512) == 528 and hb.f8_row_bytes(2560) == 2640 and hb.f8_row_bytes(528) == 560
+    assert hb.f8_row_bytes(16) == 128 and hb.f8_row_bytes(512) == 640 and hb.f8_row_bytes(2560) == 2688 and hb.f8_row_bytes(112) == 128
     assert hb.f8_bytes(16, 1) == 32 and hb.f8_bytes(128, 128) == 16400 and hb.f8_bytes(2560, 10240) == 2560 * 10240 + 4 * 20 * 80
     assert hb.f8_bytes(1 << 20, 1 << 24) == (1 << 44) + (1 << 32)
     for k, n in [(0, 1), (16, 0), (24, 1), (8, 1), ((1 << 20) + 16, 1), (16, (1 << 24) + 1)]:
@@ -133,13 +133,13 @@ def refused(hb, gpu, k, good, m, cases):
 
 def test_refused_launches(hb, gpu):
     R = hb.r
-    x, y = gpu.alloc(3 * 144 * 2 + 64), gpu.alloc(3 * 176 + 64)
+    x, y = gpu.alloc(3 * 144 * 2 + 64), gpu.alloc(3 * 256 + 64)
     refused(hb, gpu, gpu.pipeline(hb.f8_quantize_rows(144)), [R(x, 2), R(y)], 3, [
         ({0: R(x, 1)}, 3, "multiple of 2"), ({1: R(y, 8)}, 3, "multiple of 16"), ({0: R(x, 0, 862)}, 3, "binding 0"),
-        ({1: R(y, 0, 479)}, 3, "binding 1"), ({1: R(x)}, 1, "overlap"), ({}, 0, "0 rows"), ([R(x)], 1, "bindings"),
+        ({1: R(y, 0, 767)}, 3, "binding 1"), ({1: R(x)}, 1, "overlap"), ({}, 0, "0 rows"), ([R(x)], 1, "bindings"),
         ({}, 1 << 31, "too many|holds")])
     refused(hb, gpu, gpu.pipeline(hb.f8_dequantize_rows(144)), [R(y), R(x)], 3, [
-        ({1: R(x, 0, 862)}, 3, "binding 1"), ({0: R(y, 0, 479)}, 3, "binding 0"), ({1: R(y, 2)}, 1, "overlap")])
+        ({1: R(x, 0, 862)}, 3, "binding 1"), ({0: R(y, 0, 767)}, 3, "binding 0"), ({1: R(y, 2)}, 1, "overlap")])
     w, q = gpu.alloc(2 * 130 * 144 * 2), gpu.alloc(2 * hb.f8_bytes(144, 130))
     refused(hb, gpu, gpu.pipeline(hb.f8_quantize(144, 130)), [R(w), R(q)], 2, [
         ({0: R(w, 2)}, 2, "binding 0"), ({1: R(q, 16)}, 2, "binding 1"), ({}, 3, "binding"), ({}, 0, "0 rows"),
