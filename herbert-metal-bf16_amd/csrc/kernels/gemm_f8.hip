@@ -444,7 +444,8 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
 #pragma unroll
                 for (u32 q = 0; q < NR; q++) {
                     float hr[4];
-                    swiglu_n<4>(&acc[i][j][4 * q], &acc[i + IN / 2][j][4 * q], hr);
+#pragma unroll
+                    for (u32 e = 0; e < 4; e++) hr[e] = f8_swiglu(acc[i][j][4 * q + e], acc[i + IN / 2][j][4 * q + e]);
                     h[i][j][q] = u32x2{pack_bf16x2(hr[0], hr[1]), pack_bf16x2(hr[2], hr[3])};
                     top = f8_max2(top, f8_max2(h[i][j][q].x & 0x7fff7fffu, h[i][j][q].y & 0x7fff7fffu));
                 }

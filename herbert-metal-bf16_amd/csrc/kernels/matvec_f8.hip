@@ -182,11 +182,7 @@ HB_DEV void rows_of_w(const unsigned char* __restrict__ W, const u16* __restrict
     auto put = [&](u32 r, u32 c, u32 nr, float v, float up) HB_INLINE2 {
         const u32 o = blk * OT + r, n = o * 16 + nr;
         if (o >= ONT || c >= cols || n >= NOUT) return;
-        if (SWI) {
-            float h;
-            swiglu_n<1>(&v, &up, &h);
-            v = h;
-        }
+        if (SWI) v = f8_swiglu(v, up);
         store(yv, yrow(c), n, v);
     };
     if constexpr (SPLIT == 1 && !SWI) {

@@ -144,9 +144,11 @@ def silu(g):
 
 
 def swiglu_bound(g, u, eg, eu):
-    """|silu(g) u| off by what its f32 sums are off by (|silu'| <= 1.1), and 16
-    roundings of the arithmetic itself."""
-    return 1.1 * eg * (np.abs(u) + eu) + np.abs(silu(g)) * eu + 16 * U * np.abs(silu(g) * u)
+    """|silu(g) u| off by what its f32 sums are off by (|silu'| <= 1.1), 16
+    roundings of the arithmetic itself, and the exponent: -log2(e) g takes one
+    rounding beside the constant's own, half a step each, which moves e^-g, and
+    the sigmoid by no more, by 1.5 |g| 2^-24 of itself."""
+    return 1.1 * eg * (np.abs(u) + eu) + np.abs(silu(g)) * eu + (16 + np.abs(g)) * U * np.abs(silu(g) * u)
 
 
 HALF_BF16 = 2.0 ** -8  # one rounding to bf16, relative to the value
