@@ -10,6 +10,8 @@
 //          MxKxNf     the same with Out::F32
 //          mv:MxKxN   the decode matvec over M <= 16 rows
 //          q4:MxKxN   the same over W quantised to 4 bits, groups of 32
+//          f8:MxKxN   W quantised to 8 bits: up to 16 rows the matvec, more the
+//                     GEMM, x's rows quantised before it
 //
 // Output per shape: shape, kernel, microseconds per launch, TFLOP/s (GEMM)
 // or GB/s of algorithmic bytes (matvec).  The reference's counterpart is
@@ -31,7 +33,7 @@ int die(const char* what) {
 }
 
 struct Shape {
-    bool matvec = false, q4 = false;
+    bool matvec = false, q4 = false, f8 = false;
     uint32_t m = 0, k = 0, n = 0, out = HB_OUT_BF16;
 };
 
@@ -40,12 +42,16 @@ bool parse(const char* s, Shape* sh) {
         sh->matvec = true;
         sh->q4 = *s == 'q';
         s += 3;
+    } else if (!strncmp(s, "f8:", 3)) {
+        sh->f8 = true;
+        s += 3;
     }
     char tail[8] = "";
     if (sscanf(s, "%ux%ux%u%7s", &sh->m, &sh->k, &sh->n, tail) < 3) return false;
     if (!strcmp(tail, "r")) sh->out = HB_OUT_RESIDUAL;
     else if (!strcmp(tail, "f")) sh->out = HB_OUT_F32;
     else if (tail[0]) return false;
+    if (sh->f8) sh->matvec = sh->m <= 16;
     return sh->m && sh->k && sh->n && (!sh->matvec || sh->m <= 16);
 }
 
@@ -79,14 +85,14 @@ int main(int argc, char** argv) {
         } else {
             Shape sh;
             if (!parse(argv[i], &sh)) {
-                fprintf(stderr, "hb_gemm: bad shape '%s' (MxKxN[r|f], mv:MxKxN or q4:MxKxN, M <= 16)\n", argv[i]);
+                fprintf(stderr, "hb_gemm: bad shape '%s' (MxKxN[r|f], f8:MxKxN, mv:MxKxN or q4:MxKxN, M <= 16)\n", argv[i]);
                 return 2;
             }
             shapes.push_back(sh);
         }
     }
     if (shapes.empty() || !reps) {
-        fprintf(stderr, "usage: hb_gemm [--tune key=value,...] [--reps N] MxKxN[r|f] | mv:MxKxN | q4:MxKxN ...\n");
+        fprintf(stderr, "usage: hb_gemm [--tune key=value,...] [--reps N] MxKxN[r|f] | mv:MxKxN | q4:MxKxN | f8:MxKxN ...\n");
         return 2;
     }
     hb_gpu* g = nullptr;
@@ -105,10 +111,69 @@ int main(int argc, char** argv) {
         const uint32_t state[4] = {0, 0, 0, s.m};
         if (hb_upload(g, st, 0, state, sizeof state)) return die("state");
         int32_t kern = -1;
-        hb_op op;
-        memset(&op, 0, sizeof op);
-        op.m = s.m;
-        if (s.q4) {
+        hb_op ops[2];
+        memset(ops, 0, sizeof ops);
+        hb_op& op = ops[0];
+        hb_op& second = ops[1];
+        uint32_t nops = 1;
+        hb_buf rows8 = 0;
+        bool have_rows8 = false;
+        op.m = second.m = s.m;
+        if (s.f8) {
+            // W's place is taken by its 8-bit form.
+            hb_desc d;
+            memset(&d, 0, sizeof d);
+            d.kind = HB_KIND_F8_QUANTIZE;
+            d.k = s.k;
+            d.n = s.n;
+            const uint64_t bytes = hb_f8_bytes(s.k, s.n);
+            hb_buf q = 0;
+            int32_t quant = -1;
+            if (hb_kernel_build(g, &d, &quant) || hb_alloc(g, bytes, &q)) {
+                status = die("f8");
+                continue;
+            }
+            const hb_range b[2] = {whole(w), whole(q)};
+            if (hb_launch(g, quant, b, 2, 1) || hb_sync(g)) return die("f8_quantize");
+            hb_free(g, w);
+            w = q;
+            memset(&d, 0, sizeof d);
+            d.kind = s.matvec ? HB_KIND_MATVEC_F8 : HB_KIND_GEMM_F8;
+            d.k = s.k;
+            d.n = s.n;
+            d.out = s.out;
+            if (s.matvec) d.mv_m = s.m;
+            else d.rows_max = s.m;
+            if (hb_kernel_build(g, &d, &kern)) {
+                status = die("f8");
+                continue;
+            }
+            if (s.matvec) {
+                op.nbind = 3;
+                op.bind[0] = whole(w);
+                op.bind[1] = whole(x);
+                op.bind[2] = whole(y);
+            } else {
+                hb_desc qd;
+                memset(&qd, 0, sizeof qd);
+                qd.kind = HB_KIND_F8_QUANTIZE;
+                qd.form = HB_F8_ROWS;
+                qd.k = s.k;
+                if (hb_kernel_build(g, &qd, &op.kernel) || hb_alloc(g, s.m * hb_f8_row_bytes(s.k), &rows8)) {
+                    status = die("f8 rows");
+                    continue;
+                }
+                have_rows8 = true;
+                op.nbind = 2;
+                op.bind[0] = whole(x);
+                op.bind[1] = whole(rows8);
+                second.nbind = 6;
+                const hb_range gb[6] = {whole(st), whole(w), whole(rows8), whole(y), whole(st), whole(st)};
+                memcpy(second.bind, gb, sizeof gb);
+                second.kernel = kern;
+                nops = 2;
+            }
+        } else if (s.q4) {
             // W's place is taken by its packed form.
             const uint64_t bytes = hb_q4_bytes(s.k, s.n, 32);
             hb_desc d;
@@ -159,23 +224,24 @@ int main(int argc, char** argv) {
             op.bind[4] = whole(st);
             op.bind[5] = whole(st);
         }
-        op.kernel = kern;
+        if (nops == 1) op.kernel = kern;
         double secs = 0;
-        if (hb_time(g, &op, 1, 3, &secs) || hb_time(g, &op, 1, reps, &secs)) return die("hb_time");
+        if (hb_time(g, ops, nops, 3, &secs) || hb_time(g, ops, nops, reps, &secs)) return die("hb_time");
         const double t = secs / reps;
         if (s.matvec) {
-            const double weights = s.q4 ? (double)s.n * s.k * (0.5 + 2.0 / 32) : 2.0 * s.n * s.k;
+            const double weights = s.q4 ? (double)s.n * s.k * (0.5 + 2.0 / 32) : s.f8 ? (double)hb_f8_bytes(s.k, s.n) : 2.0 * s.n * s.k;
             // Residual reads y too, F32 writes twice the bytes.
             const double bytes = weights + 2.0 * s.m * s.k + 2.0 * s.m * s.n * (s.out == HB_OUT_BF16 ? 1 : 2);
-            printf("%s:%ux%ux%u %s %.2f us %.1f GB/s\n", s.q4 ? "q4" : "mv", s.m, s.k, s.n, hb_kernel_name(g, kern), t * 1e6,
+            printf("%s:%ux%ux%u %s %.2f us %.1f GB/s\n", s.q4 ? "q4" : s.f8 ? "f8" : "mv", s.m, s.k, s.n, hb_kernel_name(g, kern), t * 1e6,
                    bytes / t / 1e9);
         } else {
-            printf("%ux%ux%u%s %s %.2f us %.1f TFLOP/s\n", s.m, s.k, s.n,
+            printf("%s%ux%ux%u%s %s %.2f us %.1f TFLOP/s\n", s.f8 ? "f8:" : "", s.m, s.k, s.n,
                    s.out == HB_OUT_RESIDUAL ? "r" : s.out == HB_OUT_F32 ? "f" : "", hb_kernel_name(g, kern),
                    t * 1e6, 2.0 * s.m * s.n * s.k / t / 1e12);
         }
         fflush(stdout);
         for (hb_buf b : {x, w, y, st}) hb_free(g, b);
+        if (have_rows8) hb_free(g, rows8);
     }
     hb_engine_log_summary(e);
     hb_engine_close(e);

@@ -97,30 +97,129 @@ static uint64_t f8_matrix_bytes(uint64_t k, uint64_t n) {
 static bool f8_shape(uint32_t k, uint32_t n) { return k && n && k % 16 == 0 && k <= (1u << 20) && n <= (1u << 24); }
 static bool f8_rows_form(const hb_desc& d) { return d.form == HB_F8_ROWS; }
 
+// What a MATVEC_F8 workgroup holds in LDS: each wave its stages, its x codes.
+static uint64_t mv_f8_lds(const hb_desc& d) {
+    const uint64_t xi = (d.mv_m + 3) / 4, x = d.unroll * (d.rows / 16 * 2048 + xi * 1024) + xi * 512 + 64;
+    const uint64_t sums = d.rows / 16 * d.mv_m * 64;
+    return d.mv_waves * (x > sums ? x : sums);
+}
+
 // The 8-bit matvec's form by its row tiles (16 W rows) and K tiles (128 K).
+// Measured, us: 16 rows a wave and sixteen waves on K while every row tile finds
+// a CU of its own (4096 to 2560 at 1 row 4.9, eight waves 5.1); then 32, four
+// waves on K (2560 to 151936 at 4 rows 58.9, 64 rows 59.9; 5120 to 34816 at 8
+// rows 34.9, 64 rows 36), eight on a long one (17408 to 5120 at 8 rows 22.6, four
+// 29); past 8 x rows 64 where there are many row tiles, whose x codes serve four
+// tiles (2560 to 151936 at 16 rows 77, 32 rows 95).  Two stages of K, one where x
+// or a wave's tiles are many: more stages leave fewer workgroups a CU.
 static void mv_f8_defaults(hb_desc* d) {
     if (!d->mv_m) d->mv_m = d->rows_of == HB_ROWS_DENSE ? 1 : 16;
     const uint32_t nt = cdiv(d->n, 16), kt = cdiv(d->k, 128);
     const bool swi = d->out == HB_OUT_SWIGLU;
-    if (!d->rows) d->rows = d->rows_of != HB_ROWS_DENSE || nt > 256 || swi ? 32 : 16;
+    if (d->rows_of != HB_ROWS_DENSE) {
+        // The experts: 64 rows a wave and short splits once the block's pairs
+        // make 1024 workgroups of 32 rows (8 tokens of 8 experts, 2048 to 1024:
+        // 20.8, 32 rows 22.5; 1 token 4.2 with 32, 64 rows 5.1).
+        const bool many = (uint64_t)d->rows_max * d->top_k * cdiv(nt, 2) >= 1024;
+        if (!d->rows) d->rows = many ? 64 : 32;
+        if (!d->split) {
+            d->split = !many ? 4 : kt >= 8 ? 2 : 1;
+            while (d->split > kt || (d->mv_waves && d->split > d->mv_waves)) d->split /= 2;
+            if (!d->split) d->split = 1;
+        }
+        if (!d->mv_waves) d->mv_waves = 4;
+        if (!d->unroll) d->unroll = many ? 1 : 2;
+        return;
+    }
+    if (!d->rows) d->rows = nt <= 256 && !swi ? 16 : d->mv_m > 8 && nt >= 512 ? 64 : 32;
     if (!d->split) {
-        d->split = d->rows_of != HB_ROWS_DENSE ? 4 : d->rows == 16 || (kt >= 64 && nt <= 512) ? 16 : 8;
+        d->split = d->rows == 16 ? 16 : kt >= 64 ? 8 : d->rows == 64 ? 2 : 4;
         while (d->split > kt || (d->mv_waves && d->split > d->mv_waves)) d->split /= 2;
         if (!d->split) d->split = 1;
     }
     if (!d->mv_waves) d->mv_waves = d->split < 4 ? 4 : d->split;
-    if (!d->unroll) d->unroll = d->rows == 16 ? 2 : 1;
+    if (!d->unroll) {
+        d->unroll = d->rows == 64 || (d->rows == 16 && kt < 64) ? 1 : 2;
+        while (d->unroll > 1 && mv_f8_lds(*d) > 160 * 1024) d->unroll--;
+    }
 }
 
-// The 8-bit GEMM's tile by the rows it is built for (rows_max).
-static void gemm_f8_defaults(hb_desc* d) {
+// The forms of the dense 8-bit GEMM: tiles of bm X rows by bn W rows, and what
+// one takes in hundredths of a microsecond as first and else, an offset and a
+// share per K tile: the first alone on its CU, others beside it, which cover each
+// other's latency where several fit in LDS (`beside`), else in turn.
+struct GemmF8Form {
+    uint32_t bm, bn, wm, wn, stages, sched;
+    uint32_t first, first_kt, more, more_kt;
+    bool beside;
+};
+static const GemmF8Form kGemmF8[] = {
+    {256, 256, 4, 2, 2, 1, 680, 169, 680, 169, false}, {128, 256, 4, 2, 2, 1, 250, 92, 250, 92, false},
+    {64, 128, 2, 2, 2, 1, 130, 46, 100, 33, true},     {32, 64, 1, 4, 3, 0, 30, 28, 20, 12, true},
+    {32, 32, 1, 2, 4, 0, 20, 18, 10, 10, true},
+};
+static const GemmF8Form kGemmF8Swiglu[] = {
+    {256, 256, 4, 2, 2, 0, 400, 170, 400, 170, false}, {128, 256, 2, 4, 3, 0, 600, 90, 600, 90, false},
+    {64, 256, 1, 8, 3, 0, 240, 73, 240, 73, false},    {32, 256, 1, 8, 4, 0, 30, 60, 30, 60, false},
+};
+
+// The dense form and count of K parts of least time for `rows` rows by those
+// figures.  A split adds the second kernel: a launch and its slabs there and
+// back.  Measured, us, the form taken and the next best:
+//   48 rows, 2560 to 10240: 32 x 64 9.3, 64 x 64 10.2; 32 rows, 9216 to 2560:
+//   32 x 32 in eight parts 8.4, 32 x 64 in eight 8.5, unsplit past 17; 512 rows,
+//   9216 to 2560: 64 x 128 in four parts 28.6, 128 x 256 in four 30.5; 1024 rows,
+//   5120 to 34816: 128 x 256 214, 256 x 256 227; 8192 rows: 256 x 256 1264,
+//   128 x 256 1443.
+static void gemm_f8_dense(hb_desc* d, uint32_t rows) {
     const bool swi = d->out == HB_OUT_SWIGLU;
-    if (!d->bm) d->bm = d->rows_max && d->rows_max <= 32 ? 32 : d->rows_max && d->rows_max <= 64 ? 64 : 128;
+    const uint32_t kt = cdiv(d->k, 128);
+    uint64_t best = ~0ull;
+    const GemmF8Form* form = nullptr;
+    uint32_t parts = 1;
+    auto consider = [&](const GemmF8Form& f) {
+        const uint64_t tiles = (uint64_t)cdiv(rows, f.bm) * cdiv(d->n, f.bn);
+        for (uint32_t s = 1; s <= 8; s *= 2) {
+            if (s > 1 && (swi || d->n % 4 || s > kt || tiles * s > 1024)) break;
+            const uint64_t per = cdiv(kt, s), all = tiles * s;
+            uint64_t t = f.first + per * f.first_kt;
+            const uint64_t more = f.more + per * f.more_kt;
+            if (all > 256) t += f.beside ? (all - 256) * more / 256 : (all - 1) / 256 * more;
+            if (s > 1) t += 250 + (uint64_t)rows * d->n * s / 10000;
+            if (t < best) best = t, form = &f, parts = s;
+        }
+    };
+    if (swi)
+        for (const auto& f : kGemmF8Swiglu) consider(f);
+    else
+        for (const auto& f : kGemmF8) consider(f);
+    d->bm = form->bm, d->bn = form->bn, d->wm = form->wm, d->wn = form->wn;
+    d->dbuf = form->stages - 1, d->sched = form->sched, d->mfma = 16;
+    d->ksplit = parts > 1 ? parts : 0;
+}
+
+// The 8-bit GEMM's form: a dense descriptor that names none by the rows it is
+// built for (rows_max, 0 = 2048); else what it leaves open.
+static void gemm_f8_defaults(hb_desc* d) {
+    const bool swi = d->out == HB_OUT_SWIGLU, dense = d->rows_of == HB_ROWS_DENSE;
+    if (!d->band) d->band = 4;
+    if (dense && d->k && d->n && !d->bm && !d->bn && !d->wm && !d->wn && !d->dbuf && !d->mfma && !d->ksplit && !d->sched)
+        return gemm_f8_dense(d, d->rows_max ? d->rows_max : 2048);
+    if (!dense && d->bm >= 32 && d->bm <= 128 && !d->bn && !d->wm && !d->wn && !d->dbuf && !d->mfma && !d->sched) {
+        // The experts' (256 of 2048 / 512, top 8), us at 512, 1024 and 4096 rows,
+        // tiles of 32, 64 and 128: gate and up 93, 99, 152; down 41, 45, 108 (with
+        // 256 W rows a tile 43, 50 and 118).
+        d->bn = swi ? 256 : d->bm == 32 ? 64 : 128;
+        d->wm = swi || d->bm == 32 ? 2 : 4;
+        d->wn = swi ? 4 : 2;
+        d->dbuf = swi && d->bm > 32 ? 2 : 1;
+        d->sched = (swi && d->bm == 32) || (!swi && d->bm == 64) ? 1 : 0;
+    }
+    if (!d->bm) d->bm = 128;
     if (!d->bn) d->bn = swi ? 256 : 128;
     if (!d->wm) d->wm = d->bm >= 128 ? 2 : 1;
     if (!d->wn) d->wn = swi || d->wm == 1 ? 4 : 2;
-    if (!d->dbuf) d->dbuf = d->bm + d->bn >= 384 ? 1 : 2;
-    if (!d->band) d->band = 4;
+    if (!d->dbuf) d->dbuf = 1;
     if (!d->mfma) d->mfma = 16;
 }
 
@@ -295,12 +394,13 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
         case KIND_SPLITK_REDUCE:
             if (!d.n || d.n % 4 || d.ksplit < 2 || d.ksplit > 16 || d.out > HB_OUT_RESIDUAL)
                 return fail(HB_ERR_INVALID, "split-K reduce: N a multiple of 4, 2..16 parts");
-            snprintf(name, sizeof name, "gemm_splitk_%u_%s_s%u", d.n, out_tag(d.out), d.ksplit);
+            snprintf(name, sizeof name, "gemm_splitk_%u_%s_s%u%s", d.n, out_tag(d.out), d.ksplit, d.form ? "_once" : "");
             e->name = name;
             e->source = "gemm_splitk.hip";
             e->threads = 256;
             e->nbind = 3;
             e->defines = {D("HB_N", d.n), D("HB_OUT", d.out), D("HB_KSPLIT", d.ksplit)};
+            if (d.form) e->defines.push_back(D("HB_ONCE", 1));
             return HB_OK;
         case HB_KIND_GEMM_SIMT:
             if (d.rows_of != HB_ROWS_DENSE || d.out > HB_OUT_RESIDUAL || !d.k || d.k % 16 || !d.n)
@@ -584,6 +684,8 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
                 return fail(HB_ERR_UNSUPPORTED, "matvec_f8: 16, 32 or 64 rows a wave (Out::Swiglu not 16)");
             if (d.mv_waves > 16 || !pow2(d.mv_waves) || !pow2(d.split) || d.split > d.mv_waves || d.unroll > 4)
                 return fail(HB_ERR_UNSUPPORTED, "matvec_f8: 1, 2, 4, 8 or 16 waves, split no more, unroll 1..4");
+            if (mv_f8_lds(d) > 160 * 1024)
+                return fail(HB_ERR_UNSUPPORTED, "matvec_f8: the waves' stages beyond 160 KiB of LDS");
             if (experts && (!d.top_k || d.top_k > d.experts || d.experts > 1024 || !d.tiles || !d.rows_max ||
                             (uint64_t)d.rows_max * d.top_k >= (1u << 28) || d.mv_m != 16 || (d.out != HB_OUT_BF16 && !swi)))
                 return fail(HB_ERR_INVALID, "matvec_f8 over experts: top_k, experts (<= 1024), tiles and rows_max "
@@ -840,10 +942,10 @@ static AccessList accesses(const hb_desc& d, uint32_t m) {
             const uint64_t w = f8_matrix_bytes(k, n), pairs = mm * d.top_k, xrow = mv ? k * 2 : f8_row_bytes(k);
             const bool f8_out = swi && !mv;
             const uint64_t yrow = f8_out ? f8_row_bytes(n / 2) : (swi ? n / 2 : n) * out_bytes(d.out);
-            const uint32_t xa = mv ? 2 : 16, ya = f8_out ? 16 : out_bytes(d.out);
+            const uint32_t ya = f8_out ? 16 : out_bytes(d.out);
             if (!(mv && dense)) l.add("state", 16, 4, false);
             l.add("W", (dense ? 1 : d.experts) * w, 16, false);
-            l.add("X", (dense || d.rows_of == HB_ROWS_GATHER ? mm : pairs) * xrow, xa, false);
+            l.add("X", (dense || d.rows_of == HB_ROWS_GATHER ? mm : pairs) * xrow, 16, false);
             l.add("Y", (dense ? mm : pairs) * yrow, ya, true);
             if (dense) break;
             l.add("list", pairs * 4, 4, false);
@@ -944,6 +1046,9 @@ int check_bindings(const hb_desc& d, const uint64_t* s, uint32_t nbind, uint32_t
             if (!dense && m > d.rows_max) return fail(HB_ERR_INVALID, "m beyond the kernel's rows_max");
             if ((uint64_t)groups_of(d, m) * 64 * d.mv_waves >> 32)
                 return fail(HB_ERR_UNSUPPORTED, what + ": too many workgroups in one launch");
+            // Its kernel addresses X by 32 bits.
+            if (d.kind == HB_KIND_MATVEC_F8 && !dense && (d.rows_of == HB_ROWS_GATHER ? 1 : d.top_k) * (uint64_t)m * d.k * 2 > 0x7fffffffull)
+                return fail(HB_ERR_UNSUPPORTED, "matvec_f8: X at most 2 GiB - 1 bytes");
         } else if (d.kind == HB_KIND_ROUTE_TOPK) {
             if (m >= (1u << 26)) return fail(HB_ERR_UNSUPPORTED, "route_topk: too many rows in one launch");
         } else if (d.kind == HB_KIND_F8_QUANTIZE || d.kind == HB_KIND_F8_DEQUANTIZE) {
@@ -1039,8 +1144,12 @@ extern "C" uint64_t hb_f8_bytes(uint32_t k, uint32_t n) { return hb::f8_shape(k,
 extern "C" uint64_t hb_f8_row_bytes(uint32_t k) { return hb::f8_shape(k, 1) ? hb::f8_row_bytes(k) : 0; }
 
 extern "C" uint32_t hb_f8_tile_rows(uint32_t rows, uint32_t top_k, uint32_t experts) {
+    // The layer's two products, us (256 experts of 2048 / 512, top 8; for tiles
+    // past 16 rows with x's quantisation): 8 rows 32 with tiles of 16, 34 with
+    // 32; 16 rows 57 and 53; 512 rows 136 with 32, 142 with 64; 1024 rows 149 and
+    // 147; 2048 rows 187 with 64, 180 with 128.
     const uint64_t pairs = (uint64_t)rows * top_k;
-    return pairs <= 4ull * experts ? 16 : pairs <= 32ull * experts ? 32 : pairs <= 96ull * experts ? 64 : 128;
+    return 8 * pairs <= 3ull * experts ? 16 : pairs <= 24ull * experts ? 32 : pairs <= 48ull * experts ? 64 : 128;
 }
 
 extern "C" uint64_t hb_q4_bytes(uint32_t k, uint32_t n, uint32_t group) {

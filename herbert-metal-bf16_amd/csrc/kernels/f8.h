@@ -44,25 +44,25 @@ HB_DEV u32 f8_max_lanes(u32 w) {
     return w & 0xffffu;
 }
 
-// s and 448 / a of a group whose largest size has the bf16 bits `top`.
+// s, and 448 / a rounded up, of a group whose largest size has the bf16 bits
+// `top`; NaN for one that is not finite.
 struct F8Scale {
     float s, inv;
 };
 HB_DEV F8Scale f8_scale(u32 top) {
     u32 b = top << 16;
-    b = b > 0x0d800000u ? b : 0x0d800000u;  // 2^-100; a NaN stays the larger
+    b = b > 0x0d800000u ? b : 0x0d800000u;  // 2^-100
+    b = b < 0x7f800000u ? b : 0x7fc00000u;
     const float a = __builtin_bit_cast(float, b);
-    return {a / 448.0f, 448.0f / a};
+    return {a / 448.0f, __builtin_bit_cast(float, __builtin_bit_cast(u32, 448.0f / a) + 1u)};
 }
 
-// 448 x / a, near enough to round to e4m3: the product with the rounded
-// reciprocal is within 2^-22 of the quotient.  x and a have 8 bits each, so a
+// 448 x / a, near enough to round to e4m3.  x and a have 8 bits each, so a
 // quotient that lies halfway between two codes does so exactly and any other at
-// least 2^-14 from halfway; rounding the product to 19 bits restores the first
-// kind and keeps the second on its side.
-HB_DEV float f8_quotient(float x, float inv) {
-    return __builtin_bit_cast(float, (__builtin_bit_cast(u32, x * inv) + 16u) & ~31u);
-}
+// least 2^-14 from halfway.  The product with the rounded-up reciprocal is no
+// smaller than the quotient (a halfway one is itself an f32) and within 2^-21 of
+// it; cut to 19 bits it is the halfway one again, and any other keeps its side.
+HB_DEV float f8_quotient(float x, float inv) { return __builtin_bit_cast(float, __builtin_bit_cast(u32, x * inv) & ~31u); }
 // The codes of two bf16 in a word, in the low or the high half of `old`.
 template <bool high>
 HB_DEV u32 f8_codes2(u32 w, float inv, u32 old) {

@@ -15,11 +15,15 @@
 // starts (same stream), so no fence is needed between the two.
 //
 // Compile-time constants (-D): HB_N, HB_OUT (0 bf16, 1 f32, 2 residual),
-// HB_KSPLIT (the parts), HB_NAME.
+// HB_KSPLIT (the parts), HB_ONCE (Residual of the 8-bit GEMM: the sum not
+// rounded before it is added), HB_NAME.
 // Bindings: state (u32[4], state[3] = rows), P (the slabs), Y; then the
 // rows the launch was sized for (m_launch).
 #include "hb_common.h"
 
+#ifndef HB_ONCE
+#define HB_ONCE 0
+#endif
 constexpr u32 N = HB_N, KSP = HB_KSPLIT;
 constexpr int OUT = HB_OUT;
 static_assert(N % 4 == 0 && KSP >= 2 && KSP <= 16, "N a multiple of 4, 2..16 parts");
@@ -44,8 +48,13 @@ extern "C" __global__ __launch_bounds__(256) void HB_NAME(const u32* __restrict_
             u32x2 o;
             if constexpr (OUT == 2) {
                 const u32x2 old = *y;
-                o.x = pack_bf16x2(bf16_lo(old.x) + round_bf16(a.x), bf16_hi(old.x) + round_bf16(a.y));
-                o.y = pack_bf16x2(bf16_lo(old.y) + round_bf16(a.z), bf16_hi(old.y) + round_bf16(a.w));
+                if constexpr (HB_ONCE) {
+                    o.x = pack_bf16x2(bf16_lo(old.x) + a.x, bf16_hi(old.x) + a.y);
+                    o.y = pack_bf16x2(bf16_lo(old.y) + a.z, bf16_hi(old.y) + a.w);
+                } else {
+                    o.x = pack_bf16x2(bf16_lo(old.x) + round_bf16(a.x), bf16_hi(old.x) + round_bf16(a.y));
+                    o.y = pack_bf16x2(bf16_lo(old.y) + round_bf16(a.z), bf16_hi(old.y) + round_bf16(a.w));
+                }
             } else {
                 o.x = pack_bf16x2(a.x, a.y);
                 o.y = pack_bf16x2(a.z, a.w);

@@ -828,40 +828,68 @@ class MoeLayer:
     expert's codes are read again for every 16 of its rows.  256 experts of
     2048 / 512 with top 8, the whole layer: 33 us of 8 rows (bf16 66), 87 of 64
     (212), 158 of 512 (277), 239 of 1024 (304), and behind bf16 at 2048, 395
-    (346)."""
+    (346).
+
+    f8: w_gate_up and w_down are f8 matrices of all experts (f8_quantize over
+    [2 inter][hidden] and [hidden][inter]), read by experts_f8 in the form that
+    f8_tile_rows gives for `rows`: a decode batch's over bf16 rows, a prompt's
+    with x and the SwiGLU's rows as f8 rows.  Nothing is timed.
+
+    route: a route_topk descriptor in route_qwen's place, with the buffer of its
+    bias if it has one; scores are then f32 where it says so."""
 
     def __init__(self, gpu, engine, experts, top_k, hidden, inter, rows, w_gate_up, w_down,
-                 scores=None, x=None, q4_group=0):
+                 scores=None, x=None, q4_group=0, f8=False, route=None, bias=None):
+        if route is None:
+            route = Desc(kind=Kind.ROUTE, experts=experts, top_k=top_k)
+        elif route.kind != Kind.ROUTE_TOPK or route.experts != experts or route.top_k != top_k:
+            raise HerbertError(HB_ERR_INVALID, "MoeLayer: a route_topk of %d experts, top %d" % (experts, top_k))
+        if bool(route.kind == Kind.ROUTE_TOPK and route.form & 2) != (bias is not None):
+            raise HerbertError(HB_ERR_INVALID, "MoeLayer: a bias where the route takes one")
+        if f8 and q4_group:
+            raise HerbertError(HB_ERR_INVALID, "MoeLayer: experts in 8 bits or in 4")
         self.gpu, self.e, self.k, self.h, self.mi, self.rows = gpu, experts, top_k, hidden, inter, rows
         pairs = rows * top_k
         g = gpu
+        f32_scores = route.kind == Kind.ROUTE_TOPK and route.form & 8
         self.buf = {
             "state": g.alloc_with(np.array([0, 0, 0, rows], np.uint32)),
-            "scores": g.alloc(rows * experts * 2),
+            "scores": g.alloc(rows * experts * (4 if f32_scores else 2)),
             "route": g.alloc(rows * 2 * top_k * 4),
             "list": g.alloc(pairs * 4),
             "tiles": g.alloc((1 + 3 * moe_tiles(rows, top_k, experts, 16)) * 4),
             "x": g.alloc(rows * hidden * 2),
             "w_gate_up": w_gate_up,
             "egu": g.alloc(pairs * 2 * inter * 2),
-            "ehb": g.alloc(pairs * inter * 2),
+            "ehb": g.alloc(pairs * max(inter * 2, f8_row_bytes(inter) if f8 else 0)),
             "w_down": w_down,
             "ey": g.alloc(pairs * hidden * 2),
-            "xs": g.alloc(pairs * hidden * 2),
+            "xs": g.alloc(max(pairs * hidden * 2, rows * f8_row_bytes(hidden) if f8 else 0)),
             "out": g.alloc(rows * hidden * 2),
         }
+        if bias is not None:
+            self.buf["bias"] = bias
         b = self.buf
         self.io = MoeIo(*[r(b[f]) for f in ("state", "route", "list", "tiles", "x", "w_gate_up",
                                              "egu", "ehb", "w_down", "ey", "xs")])
-        self.route_k = gpu.pipeline(Desc(kind=Kind.ROUTE, experts=experts, top_k=top_k))
+        self.route_k = gpu.pipeline(route)
+        self.route_io = [r(b["scores"]), r(b["route"])] + ([r(bias)] if bias is not None else [])
         self.swiglu_k = gpu.pipeline(Desc(kind=Kind.SWIGLU, n=inter))
         self.combine_k = gpu.pipeline(Desc(kind=Kind.COMBINE, n=hidden, top_k=top_k))
         if x is not None:
             g.upload(b["x"], x)
         if scores is not None:
             g.upload(b["scores"], scores)
-            g.launch(self.route_k, [r(b["scores"]), r(b["route"])], rows)
+            g.launch(self.route_k, self.route_io, rows)
             g.sync()
+        if f8:
+            self.bm = f8_tile_rows(rows, top_k, experts)
+            descs = [Desc(kind=Kind.SORT, experts=experts, top_k=top_k, bm=self.bm, rows_max=rows),
+                     experts_f8(hidden, 2 * inter, Out.Swiglu, Rows.Gather, top_k, experts, rows, self.bm),
+                     experts_f8(inter, hidden, Out.Bf16, Rows.Scatter, top_k, experts, rows, self.bm)]
+            quantize = gpu.pipeline(f8_quantize_rows(hidden)) if self.bm > 16 else -1
+            self.kernels, self.fused = [gpu.pipeline(d) for d in descs] + [quantize], True
+            return
         if q4_group:
             self.bm = 16
             descs = [Desc(kind=Kind.SORT, experts=experts, top_k=top_k, bm=16, rows_max=rows),
@@ -877,11 +905,12 @@ class MoeLayer:
         m = self.rows if m is None else m
         b, k = self.buf, self.k
         sort, gu, dn, gather = self.kernels
-        ops = [Op(self.route_k, [r(b["scores"]), r(b["route"])], m),
+        ops = [Op(self.route_k, self.route_io, m),
                Op(sort, [r(b["state"]), r(b["route"]), r(b["list"]), r(b["tiles"])], m)]
         xin = b["x"]
         if gather >= 0:
-            ops.append(Op(gather, [r(b["state"]), r(b["list"]), r(b["x"]), r(b["xs"])], m))
+            quantize = self.gpu.kernel_kind(gather) == Kind.F8_QUANTIZE
+            ops.append(Op(gather, ([] if quantize else [r(b["state"]), r(b["list"])]) + [r(b["x"]), r(b["xs"])], m))
             xin = b["xs"]
         if self.fused:
             # The grouped gate|up writes the SwiGLU itself.
@@ -897,18 +926,18 @@ class MoeLayer:
         return ops
 
     def run(self, m=None):
-        """The layer in two host calls: route_qwen, then hb_moe_experts_run
+        """The layer in two host calls: the route, then hb_moe_experts_run
         (the rest of ops() as one native dispatch sequence)."""
         m = self.rows if m is None else m
         b = self.buf
-        self.gpu.launch(self.route_k, [r(b["scores"]), r(b["route"])], m)
+        self.gpu.launch(self.route_k, self.route_io, m)
         ks = (ctypes.c_int32 * 4)(*self.kernels)
         check(lib.hb_moe_experts_run(self.gpu.h, ks, self.swiglu_k, self.combine_k,
                                      ctypes.byref(self.io), r(b["out"]), m))
 
     def free(self):
         for name, buf in self.buf.items():
-            if name not in ("w_gate_up", "w_down"):
+            if name not in ("w_gate_up", "w_down", "bias"):
                 self.gpu.free(buf)
 
 
@@ -937,10 +966,11 @@ class MoeBlock:
     [E*2*inter][h], "w_down": [E*h][inter], "s_gate_up": [2*si][h], "s_down":
     [h][si], "shared_gate": [h]}.  `x` (host [rows][h]) is the residual
     stream the selection runs on; the block updates buf["x"] in place.
-    q4_group: w_gate_up and w_down in 4 bits, as MoeLayer takes them."""
+    q4_group, f8: w_gate_up and w_down in 4 or 8 bits, route: another route,
+    its bias w["route_bias"], as MoeLayer takes them."""
 
     def __init__(self, gpu, engine, experts, top_k, hidden, inter, shared_inter, rows, w, x,
-                 eps=1e-6, plus_one=True, q4_group=0):
+                 eps=1e-6, plus_one=True, q4_group=0, f8=False, route=None):
         g, h, si = gpu, hidden, shared_inter
         self.gpu, self.rows, self.h, self.si, self.w = gpu, rows, h, si, w
         self.buf = {"state": g.alloc_with(np.array([0, 0, 0, rows], np.uint32)),
@@ -952,19 +982,21 @@ class MoeBlock:
         self.out_k = g.pipeline(moe_out(h))
         # xn and the router's scores on the selection's input, for the
         # experts' timing on a real route (the reference's real_route).
-        xn_t, sc_t = g.alloc(rows * h * 2), g.alloc(rows * experts * 2)
+        wide = route is not None and bool(route.form & 8)  # f32 scores
+        xn_t, sc_t = g.alloc(rows * h * 2), g.alloc(rows * experts * (4 if wide else 2))
         g.launch(self.norm_k, [r(b["x"]), r(w["post_norm"]), r(xn_t)], rows)
-        self.router_k = engine.gemm(h, experts, Out.Bf16, r(b["state"]), r(w["router"]), r(xn_t),
+        self.router_k = engine.gemm(h, experts, Out.F32 if wide else Out.Bf16, r(b["state"]), r(w["router"]), r(xn_t),
                                     r(sc_t), rows)
         g.launch(self.router_k, [r(b["state"]), r(w["router"]), r(xn_t), r(sc_t), r(b["state"]),
                                  r(b["state"])], rows)
         g.sync()
         xn = g.download(xn_t, np.uint16, rows * h).reshape(rows, h)
-        scores = g.download(sc_t, np.uint16, rows * experts).reshape(rows, experts)
+        scores = g.download(sc_t, np.float32 if wide else np.uint16, rows * experts).reshape(rows, experts)
         g.free(xn_t)
         g.free(sc_t)
         self.layer = MoeLayer(g, engine, experts, top_k, h, inter, rows, w["w_gate_up"], w["w_down"],
-                              scores=scores, x=xn, q4_group=q4_group)
+                              scores=scores, x=xn, q4_group=q4_group, f8=f8, route=route,
+                              bias=w["route_bias"] if route is not None and route.form & 2 else None)
         L = self.layer.buf
         self.s_gu_k, self.s_sw_k = engine.gate_up(h, si, r(b["state"]), r(w["s_gate_up"]), r(L["x"]),
                                                   r(b["s_gu"]), r(b["s_h"]), rows)
@@ -1062,13 +1094,21 @@ class Checkpoint:
     def upload_q4(self, gpu, parts, kdim, n, group=32, count=1):
         """upload, then quantised on the GPU: `count` packed 4-bit matrices of
         n rows of kdim, the bf16 weights given back."""
+        return self._upload_as("upload_q4", gpu, parts, kdim, n, count, q4_bytes(kdim, n, group), q4_quantize(kdim, n, group))
+
+    def upload_f8(self, gpu, parts, kdim, n, count=1):
+        """upload, then quantised on the GPU: `count` f8 matrices of n rows of
+        kdim, the bf16 weights given back."""
+        return self._upload_as("upload_f8", gpu, parts, kdim, n, count, f8_bytes(kdim, n), f8_quantize(kdim, n))
+
+    def _upload_as(self, what, gpu, parts, kdim, n, count, size, quantize):
         if sum(int(c) for _, c in parts) != count * n * kdim:
-            raise HerbertError(HB_ERR_INVALID, "upload_q4: the parts hold no %d matrices of %dx%d" % (count, n, kdim))
-        q = gpu.alloc(count * q4_bytes(kdim, n, group))
+            raise HerbertError(HB_ERR_INVALID, "%s: the parts hold no %d matrices of %dx%d" % (what, count, n, kdim))
+        q = gpu.alloc(count * size)
         w = None
         try:
             w = self.upload(gpu, parts)
-            gpu.launch(gpu.pipeline(q4_quantize(kdim, n, group)), [r(w), r(q)], count)
+            gpu.launch(gpu.pipeline(quantize), [r(w), r(q)], count)
             gpu.sync()
         except Exception:
             gpu.free(q)
@@ -1140,24 +1180,35 @@ class PrefillMlp:
     over a prompt cut into blocks (blocks_of) with each block on the kernels
     picked for its bucket (the smallest of the prefill buckets, qwen.rs:
     1051-1063, holding its rows).  Weights from the checkpoint in the fused
-    layout the GEMMs read (qwen.rs:790-794)."""
+    layout the GEMMs read (qwen.rs:790-794).  f8: the weights quantised to f8
+    matrices and the block run on them: norm, x's rows quantised, [gate | up]
+    with the SwiGLU's f8 rows, down; nothing timed."""
 
-    def __init__(self, gpu, engine, ckpt, layer, hidden, inter, eps=1e-6, plus_one=True):
-        self.gpu, self.h, self.inter = gpu, hidden, inter
+    def __init__(self, gpu, engine, ckpt, layer, hidden, inter, eps=1e-6, plus_one=True, f8=False):
+        self.gpu, self.h, self.inter, self.f8 = gpu, hidden, inter, f8
         p = lambda f: "%d.%s" % (layer, f)  # noqa: E731
         mlp = "mlp.shared_expert" if ckpt.has(p("mlp.shared_expert.gate_proj.weight")) else "mlp"
+        put = ckpt.upload_f8 if f8 else lambda gpu, parts, k, n: ckpt.upload(gpu, parts)
         self.w = {"post_norm": ckpt.upload(gpu, [(p("post_attention_layernorm.weight"), hidden)]),
-                  "gate_up": ckpt.upload(gpu, [(p(mlp + ".gate_proj.weight"), inter * hidden),
-                                               (p(mlp + ".up_proj.weight"), inter * hidden)]),
-                  "down": ckpt.upload(gpu, [(p(mlp + ".down_proj.weight"), hidden * inter)])}
+                  "gate_up": put(gpu, [(p(mlp + ".gate_proj.weight"), inter * hidden),
+                                       (p(mlp + ".up_proj.weight"), inter * hidden)], hidden, 2 * inter),
+                  "down": put(gpu, [(p(mlp + ".down_proj.weight"), hidden * inter)], inter, hidden)}
         self.buckets = engine.buckets()
         self.chunk = self.buckets[-1]
         B = self.chunk
         g = gpu
-        self.buf = {"xn": g.alloc(B * hidden * 2), "gu": g.alloc(B * 2 * inter * 2),
-                    "hh": g.alloc(B * inter * 2), "x": g.alloc(B * hidden * 2)}
+        if f8:
+            self.buf = {"xn": g.alloc(B * hidden * 2), "x8": g.alloc(B * f8_row_bytes(hidden)), "h8": g.alloc(B * f8_row_bytes(inter))}
+        else:
+            self.buf = {"xn": g.alloc(B * hidden * 2), "gu": g.alloc(B * 2 * inter * 2),
+                        "hh": g.alloc(B * inter * 2), "x": g.alloc(B * hidden * 2)}
         self.norm_k = g.pipeline(rmsnorm(hidden, eps, plus_one))
         self.kern = {}
+        if f8:
+            q = g.pipeline(f8_quantize_rows(hidden))
+            self.kern = {m: (g.pipeline(gemm_f8(hidden, 2 * inter, Out.Swiglu, rows=m)), q,
+                             g.pipeline(gemm_f8(inter, hidden, Out.Residual, rows=m))) for m in self.buckets}
+            return
         for m in self.buckets:
             st = g.alloc_with(np.array([0, 0, 0, m], np.uint32))
             b, w = self.buf, self.w
@@ -1184,6 +1235,10 @@ class PrefillMlp:
         xr = r(x, start * h * 2, rows * h * 2)
         s = r(st)
         ops = [Op(self.norm_k, [xr, r(w["post_norm"]), r(b["xn"])], rows)]
+        if self.f8:
+            return ops + [Op(sw_k, [r(b["xn"]), r(b["x8"])], rows),
+                          Op(gu_k, [s, r(w["gate_up"]), r(b["x8"]), r(b["h8"]), s, s], rows),
+                          Op(dn_k, [s, r(w["down"]), r(b["h8"]), xr, s, s], rows)]
         if sw_k >= 0:
             ops.append(Op(gu_k, [s, r(w["gate_up"]), r(b["xn"]), r(b["gu"]), s, s], rows))
             ops.append(Op(sw_k, [r(b["gu"]), r(b["hh"])], rows))
@@ -1316,15 +1371,18 @@ def route_probe_rows(ckpt, block, hidden):
     return emb[np.array(probe_ids(block), dtype=np.int64) % vocab]
 
 
-def moe_weights_from_checkpoint(gpu, ckpt, layer, experts, hidden, inter, shared_inter, q4_group=0):
+def moe_weights_from_checkpoint(gpu, ckpt, layer, experts, hidden, inter, shared_inter, q4_group=0, f8=False):
     """The device weights of a qwen3_5_moe layer's sparse MLP as
     QwenEngine::load uploads them (qwen.rs:788-801): the post norm, the
     router (mlp.gate), the experts' [gate | up] rows and down rows
     (mlp.experts.gate_up_proj [E][2 inter][h], down_proj [E][h][inter]),
     the shared expert stacked [gate | up], its down and its gate; the dict
-    MoeBlock takes.  q4_group: the experts quantised to 4 bits in groups of it."""
+    MoeBlock takes.  q4_group: the experts quantised to 4 bits in groups of it;
+    f8: to 8 bits."""
     def experts_w(key, kdim, n):
         parts = [(p(key), e * n * kdim)]
+        if f8:
+            return ckpt.upload_f8(gpu, parts, kdim, n, e)
         return ckpt.upload_q4(gpu, parts, kdim, n, q4_group, e) if q4_group else ckpt.upload(gpu, parts)
 
     p = lambda f: "%d.%s" % (layer, f)  # noqa: E731

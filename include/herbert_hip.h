@@ -332,7 +332,7 @@ double hb_compile_seconds(hb_gpu *gpu);
  *     overlap.
  * The bindings of these (ROUTE_TOPK, Q4_*, F8_*, GEMM_F8, MATVEC_Q4 and _F8,
  * BLOCK_NORM) start at a multiple of their element (2 bytes,
- * f32 and u32 4, q4, f8 matrices and f8 rows 16), and what a launch writes overlaps nothing else it
+ * f32 and u32 4, q4, f8 matrices and f8 rows and MATVEC_F8's X 16), and what a launch writes overlaps nothing else it
  * binds: both are checked.  Of MATVEC_Q4: HB_OUT_BF16, _F32, _RESIDUAL
  * (y = rne(y + sum), one rounding) and _SWIGLU (n / 2 a multiple of 16, h =
  * rne(g * sigmoid(g) * u) of the f32 sums).  The sums go through

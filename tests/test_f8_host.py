@@ -74,6 +74,7 @@ def test_reference_codes():
     (lambda hb: hb.matvec_f8(128, 64, hb.Out.Bf16, waves=3), "waves"),
     (lambda hb: hb.matvec_f8(128, 64, hb.Out.Bf16, split=8, waves=4), "split"),
     (lambda hb: hb.matvec_f8(128, 64, hb.Out.Bf16, unroll=5), "unroll"),
+    (lambda hb: hb.matvec_f8(4096, 64, hb.Out.Bf16, mv_m=16, rows=64, split=16, waves=16, unroll=1), "stages"),
     (lambda hb: hb.experts_f8(128, 64, hb.Out.F32, hb.Rows.Gather, 8, 64, 4, 16), "bf16 out"),
     (lambda hb: hb.experts_f8(128, 64, hb.Out.F32, hb.Rows.Gather, 8, 64, 4, 64), "bf16 out"),
     (lambda hb: hb.experts_f8(128, 64, hb.Out.Bf16, hb.Rows.Sorted, 8, 64, 4, 16), "rows_of"),
@@ -152,9 +153,9 @@ def test_refused_launches(hb, gpu):
 def test_refused_matvec_launches(hb, gpu):
     R = hb.r
     w, x, y = gpu.alloc(hb.f8_bytes(128, 32) + 32), gpu.alloc(2 * 256 + 64), gpu.alloc(2 * 128 + 64)
-    refused(hb, gpu, gpu.pipeline(hb.matvec_f8(128, 32, hb.Out.F32, mv_m=2)), [R(w), R(x, 2), R(y, 4)], 2, [
+    refused(hb, gpu, gpu.pipeline(hb.matvec_f8(128, 32, hb.Out.F32, mv_m=2)), [R(w), R(x, 16), R(y, 4)], 2, [
         ({}, 0, "0 rows"), ({}, 3, "rows: 1..2"), ({0: R(w, 0, hb.f8_bytes(128, 32) - 1)}, 1, "binding 0"), ({0: R(w, 8)}, 1, "multiple of 16"),
-        ({1: R(x, 0, 511)}, 2, "binding 1"), ({2: R(y, 0, 255)}, 2, "binding 2"), ({1: R(x, 1)}, 1, "multiple of 2"),
+        ({1: R(x, 0, 511)}, 2, "binding 1"), ({2: R(y, 0, 255)}, 2, "binding 2"), ({1: R(x, 2)}, 1, "multiple of 16"),
         ({2: R(y, 2)}, 1, "multiple of 4"), ({2: R(x, 4)}, 1, "overlap"), ({2: R(w, 1024)}, 1, "overlap")])
 
 
@@ -200,8 +201,8 @@ def test_refused_route_launches(hb, gpu):
 
 @pytest.mark.parametrize("desc", [
     herbert_hip.f8_quantize_rows(16), herbert_hip.f8_quantize(144, 1), herbert_hip.f8_dequantize_rows(17408), herbert_hip.f8_dequantize(16, 300),
-    herbert_hip.matvec_f8(16, 1, herbert_hip.Out.Bf16), herbert_hip.matvec_f8(17408, 5120, herbert_hip.Out.F32, 16, 64, 16, 16, 4),
-    herbert_hip.matvec_f8(2560, 18432, herbert_hip.Out.Swiglu, 16, 64, 16, 16, 1),
+    herbert_hip.matvec_f8(16, 1, herbert_hip.Out.Bf16), herbert_hip.matvec_f8(17408, 5120, herbert_hip.Out.F32, 16, 64, 4, 4, 2),
+    herbert_hip.matvec_f8(2560, 18432, herbert_hip.Out.Swiglu, 16, 64, 8, 8, 1),
     herbert_hip.experts_f8(2048, 1024, herbert_hip.Out.Swiglu, herbert_hip.Rows.Gather, 8, 256, 64, 16),
     herbert_hip.experts_f8(2048, 1024, herbert_hip.Out.Swiglu, herbert_hip.Rows.Gather, 8, 256, 4096, 128),
     herbert_hip.experts_f8(512, 2048, herbert_hip.Out.Bf16, herbert_hip.Rows.Scatter, 8, 256, 4096, 32),

@@ -142,7 +142,7 @@ def matvec(gpu, codes, scales, x, out, y0=None, odd=0, **form):
     dtype = np.float32 if out == hb.Out.F32 else np.uint16
     y = np.full((m, width), 0x42, dtype) if y0 is None else y0
     with Bufs(gpu) as b:
-        w, xr, yr = b.put(f8.pack(codes, scales)), b.put(x, odd), b.put(y, odd)
+        w, xr, yr = b.put(f8.pack(codes, scales)), b.put(x, 8 * odd), b.put(y, odd)
         run(gpu, hb.matvec_f8(k, n, out, **form), [w, xr, yr], m)
         return b.get(yr, dtype, (m, width))
 
@@ -174,8 +174,8 @@ def test_matvec_exact(gpu, m, k, n):
     assert np.array_equal(got.astype(np.float64), want)
 
 
-@pytest.mark.parametrize("rows,split,waves,unroll", [(16, 1, 1, 1), (16, 16, 16, 2), (32, 8, 8, 1), (64, 4, 4, 1), (32, 2, 4, 4),
-                                                     (64, 1, 2, 2), (16, 4, 8, 3), (64, 16, 16, 1)])
+@pytest.mark.parametrize("rows,split,waves,unroll", [(16, 1, 1, 1), (16, 16, 16, 1), (32, 8, 8, 1), (64, 4, 4, 1), (32, 2, 4, 4),
+                                                     (64, 1, 2, 2), (16, 4, 8, 2), (64, 8, 8, 1)])
 @pytest.mark.parametrize("out", list(hb.Out))
 def test_matvec_forms(gpu, rows, split, waves, unroll, out):
     if out == hb.Out.Swiglu and rows == 16:
