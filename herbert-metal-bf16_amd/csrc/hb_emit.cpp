@@ -162,6 +162,11 @@ static const GemmF8Form kGemmF8Swiglu[] = {
     {256, 256, 4, 2, 2, 0, 400, 170, 400, 170, false}, {128, 256, 2, 4, 3, 0, 600, 90, 600, 90, false},
     {64, 256, 1, 8, 3, 0, 240, 73, 240, 73, false},    {32, 256, 1, 8, 4, 0, 30, 60, 30, 60, false},
 };
+// Out::F32's, whose products are bf16 (f8.h).
+static const GemmF8Form kGemmF8F32[] = {
+    {128, 128, 4, 2, 2, 1, 315, 97, 230, 93, false}, {64, 128, 2, 4, 2, 0, 253, 69, 97, 64, false},
+    {32, 64, 1, 4, 3, 0, 168, 43, 48, 20, false},    {32, 32, 1, 2, 4, 0, 145, 42, 4, 15, true},
+};
 
 // The dense form and count of K parts of least time for `rows` rows by those
 // figures.  A split adds the second kernel: a launch and its slabs there and
@@ -170,7 +175,9 @@ static const GemmF8Form kGemmF8Swiglu[] = {
 //   32 x 32 in eight parts 8.4, 32 x 64 in eight 8.5, unsplit past 17; 512 rows,
 //   9216 to 2560: 64 x 128 in four parts 28.6, 128 x 256 in four 30.5; 1024 rows,
 //   5120 to 34816: 128 x 256 214, 256 x 256 227; 8192 rows: 256 x 256 1264,
-//   128 x 256 1443.
+//   128 x 256 1443.  Of Out::F32: 17 rows, 2560 to 512: 32 x 32 in eight parts 5.7,
+//   in four 6.0; 509 rows, 5008 to 7001: 128 x 128 50.6, 64 x 128 55; 2048 rows,
+//   9216 to 2560: 128 x 128 in two parts 114, whole 130.
 static void gemm_f8_dense(hb_desc* d, uint32_t rows) {
     const bool swi = d->out == HB_OUT_SWIGLU;
     const uint32_t kt = cdiv(d->k, 128);
@@ -191,6 +198,8 @@ static void gemm_f8_dense(hb_desc* d, uint32_t rows) {
     };
     if (swi)
         for (const auto& f : kGemmF8Swiglu) consider(f);
+    else if (d->out == HB_OUT_F32)
+        for (const auto& f : kGemmF8F32) consider(f);
     else
         for (const auto& f : kGemmF8) consider(f);
     d->bm = form->bm, d->bn = form->bn, d->wm = form->wm, d->wn = form->wn;
@@ -718,7 +727,7 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             if (swi && (d.n % 256 || d.rows_of == HB_ROWS_SCATTER))
                 return fail(HB_ERR_UNSUPPORTED, "gemm_f8 Out::Swiglu: gate and up rows each a multiple of 128, no scatter");
             if (d.bm > 256 || !pow2(d.bm) || d.bm < 32 || d.bn > 256 || d.bn % 32 || !d.wm || !d.wn || d.wm * d.wn > 16 ||
-                (d.mfma != 16 && d.mfma != 32) || d.bm % (d.wm * d.mfma) || d.bn % (d.wn * d.mfma) ||
+                (d.mfma != 16 && (d.mfma != 32 || d.out == HB_OUT_F32)) || d.bm % (d.wm * d.mfma) || d.bn % (d.wn * d.mfma) ||
                 (swi && (d.bn != 256 || d.bn / d.wn % (2 * d.mfma))))
                 return fail(HB_ERR_UNSUPPORTED, "gemm_f8: tiles of 32 to 256 X rows (a power of 2) by up to 256 W rows (Out::Swiglu 256), "
                                                 "whole fragments of 16 a wave");
@@ -747,7 +756,7 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             e->nbind = 6;
             e->defines = {D("HB_K", d.k),   D("HB_N", d.n),   D("HB_OUT", d.ksplit > 1 ? (uint32_t)HB_OUT_F32 : d.out),
                           D("HB_ROWS", d.rows_of), D("HB_TOPK", experts ? d.top_k : 1), D("HB_E", experts ? d.experts : 1),
-                          D("HB_BM", d.bm), D("HB_BN", d.bn), D("HB_WM", d.wm), D("HB_WN", d.wn),
+                          D("HB_WIDE", d.out == HB_OUT_F32), D("HB_BM", d.bm), D("HB_BN", d.bn), D("HB_WM", d.wm), D("HB_WN", d.wn),
                           D("HB_STAGES", d.dbuf + 1), D("HB_BAND", d.band), D("HB_KSPLIT", d.ksplit > 1 ? d.ksplit : 1),
                           D("HB_SCHED", d.sched), D("HB_MFMA", d.mfma)};
             return HB_OK;

@@ -11,7 +11,9 @@
 // v_mfma_f32_16x16x128_f8f6f4 from zero.  W is its first operand, so that a
 // lane has four columns n of one row m: the row's scale is the lane's, W's is
 // one for all of the fragment, and their product adds the four sums to the
-// accumulators with an fma each, 16 cycles of VALU beside the MFMA's 32.
+// accumulators with an fma each, 16 cycles of VALU beside the MFMA's 32.  Its
+// sums come out some 2^-16 off, little beside the half step of 2^-8 of a bf16
+// output; an f32 output takes the bf16 products of f8.h in its place (HB_WIDE).
 //
 // X and W tiles of 128 K go straight into LDS (buffer_load_dwordx4 ... lds)
 // through HB_STAGES stages, 16-byte chunks XORed by row >> 1 so that the
@@ -28,7 +30,7 @@
 //
 // Constants: HB_K, HB_N (W rows), HB_OUT (0 bf16, 1 f32, 2 residual, 3
 // SwiGLU), HB_ROWS, HB_TOPK, HB_E, HB_BM, HB_BN, HB_WM, HB_WN, HB_STAGES,
-// HB_BAND, HB_KSPLIT.  Bindings: state, W, X, Y, list, tiles; then the rows
+// HB_BAND, HB_KSPLIT, HB_WIDE.  Bindings: state, W, X, Y, list, tiles; then the rows
 // the launch was sized for.
 #include "f8.h"
 
@@ -59,6 +61,10 @@ constexpr u32 LROWS = NWV * 8;                            // rows between a wave
 #define HB_SCHED 0
 #endif
 constexpr bool AHEAD = HB_SCHED == 1;
+#ifndef HB_WIDE
+#define HB_WIDE 0
+#endif
+static_assert(!HB_WIDE || FM == 16, "the bf16 products: blocks of 16 x 16");
 // The W row of a tile's row r, from the tile's first column on: a wave's gate
 // rows stand before the up rows of the same features.
 constexpr u32 w_row(u32 r) {
@@ -274,22 +280,32 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
         }
         return f;
     };
+#if HB_WIDE
+    typedef F8Wide Operand;
+    auto operand_of = [&](const Fragment& f) HB_INLINE -> Operand { return f8_wide(f.k[0]); };
+#else
+    typedef Fragment Operand;
+    auto operand_of = [&](const Fragment& f) HB_INLINE -> Operand { return f; };
+#endif
     typedef float block_t __attribute__((ext_vector_type(FR)));
 
     float sx[IM];
-    Fragment xf[IM];
+    Operand xf[IM];
     auto read_x = [&](u32 kt, u32 st) HB_INLINE {
         const u32x4* sX = sXa + st * XST + xbase;
         const float* sc = (const float*)(sscale + (kt / 8 & 1u) * BM * 2) + (wm * TM + fr) * 8 + (kt & 7u);
 #pragma unroll
         for (u32 j = 0; j < IM; j++) {
-            xf[j] = fragment(sX + j * FM * 8);
+            xf[j] = operand_of(fragment(sX + j * FM * 8));
             sx[j] = sc[j * FM * 8];
         }
     };
     float last_sw = 0.0f;
-    auto product_of = [&](const Fragment& w, const Fragment& x) HB_INLINE -> block_t {
+    auto product_of = [&](const Operand& w, const Operand& x) HB_INLINE -> block_t {
         block_t t = {};
+#if HB_WIDE
+        t = f8_product(w, x);
+#else
 #pragma unroll
         for (u32 q = 0; q < MK; q++) {
 #if HB_MFMA == 16
@@ -298,6 +314,7 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
             t = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w.k[q], x.k[q], t, 0, 0, 0, 0, 0, 0);
 #endif
         }
+#endif
         return t;
     };
     auto add = [&](u32 i, u32 j, const block_t& t, float s) HB_INLINE {
@@ -355,6 +372,9 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
         auto step = [&](u32 kt, u32 st, Fragment (&x)[IM], float (&sc)[IM], Fragment (&xn)[IM], float (&sn)[IM]) HB_INLINE {
             const u32x4* sW = sWa + st * WST + wbase;
             Fragment w[IN];
+            Operand xo[IM];
+#pragma unroll
+            for (u32 j = 0; j < IM; j++) xo[j] = operand_of(x[j]);
             w[0] = first;
             float sw = wscale[w_block(0) * KBP + kt];
             block_t t[2];
@@ -372,10 +392,11 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
                     ready(kt + 1, 1 - st, xn, sn);  // past the last tile: of a stage that nobody uses
                 }
                 if (!(BN % 128 == 0 && 128 % TN == 0 && !SWI) && i) sw = wscale[w_block(i) * KBP + kt];
+                const Operand wo = operand_of(w[i]);
 #pragma unroll
                 for (u32 j = 0; j < IM; j++) {
                     const u32 q = i * IM + j;
-                    t[q % 2] = product_of(w[i], x[j]);
+                    t[q % 2] = product_of(wo, xo[j]);
                     __builtin_amdgcn_sched_barrier(0);
                     if (q) {
                         const u32 p = q - 1;
@@ -415,7 +436,7 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
             read_x(kt, st);
 #pragma unroll
             for (u32 i = 0; i < IN; i++) {
-                const Fragment wf = fragment(sW + i * FM * 8);
+                const Operand wf = operand_of(fragment(sW + i * FM * 8));
                 const float sw = wscale[w_block(i) * KBP + kt];
 #pragma unroll
                 for (u32 j = 0; j < IM; j++) add(i, j, product_of(wf, xf[j]), sx[j] * sw);

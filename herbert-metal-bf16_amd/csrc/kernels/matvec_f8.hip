@@ -7,11 +7,12 @@
 //   y[m][n] = sum over blocks b of 128 K of sx[m][b] sw[n / 128][b] *
 //             (sum over k in b of qx qw)
 //
-// A block of 16 x rows by 16 W rows is one v_mfma_f32_16x16x128_f8f6f4, whose
-// f32 sums the two scales multiply: x is its first operand, so that a lane has
-// one W row's sums for four x rows.  How the MFMA orders K does not matter as
-// long as both operands have it alike: a lane takes the 16-byte chunks q and
-// q + 4 of its row's 128, q its quad of lanes.
+// A block of 16 x rows by 16 W rows is four v_mfma_f32_16x16x32_bf16 of the codes
+// as bf16 (f8.h: sums in f32, and the loads of W still bound the kernel), whose
+// sums the two scales multiply: x is the first operand, so that a lane has one W
+// row's sums for four x rows.  How the MFMA orders K does not matter as long as
+// both operands have it alike: a lane takes the 16-byte chunks q and q + 4 of
+// its row's 128, q its quad of lanes.
 //
 // Each wave loads its own W rows and x rows straight into LDS
 // (buffer_load_dwordx4 ... lds), HB_UNROLL tiles of 128 K ahead, with no barrier
@@ -46,8 +47,6 @@ static_assert(WAVES % SPLIT == 0 && MV >= 1 && MV <= 16, "waves");
 HB_DEV i32x8 operand(u32x4 a, u32x4 b) {
     return i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
 }
-// No scale operands: the plain product.
-HB_DEV f32x4 mfma(i32x8 x, i32x8 w) { return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, w, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0); }
 
 // Out of the sum of y[row][n].
 HB_DEV void store(void* yv, u64 row, u32 n, float v) {
@@ -186,7 +185,7 @@ HB_DEV void rows_of_w(const unsigned char* __restrict__ W, const u16* __restrict
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         const u32 c = col < 4 * XI ? col : 0;
-        const i32x8 xf = operand(xt[c * 8 + (quad ^ (c & 7u))], xt[c * 8 + ((quad + 4) ^ (c & 7u))]);
+        const F8Wide xf = f8_wide(operand(xt[c * 8 + (quad ^ (c & 7u))], xt[c * 8 + ((quad + 4) ^ (c & 7u))]));
         const f32x4 sx = *(const f32x4*)(xs + (quad < XI ? 4 * quad : 0));
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -197,7 +196,7 @@ HB_DEV void rows_of_w(const unsigned char* __restrict__ W, const u16* __restrict
             for (u32 i = 0; i < AR; i++) sc[j][i] = sx[i] * sw[j];
 #pragma unroll
         for (u32 r = 0; r < RT; r++) {
-            const f32x4 v = mfma(xf, wf[r]);
+            const f32x4 v = f8_product(xf, f8_wide(wf[r]));
 #pragma unroll
             for (u32 i = 0; i < AR; i++) acc[r][i] = __builtin_fmaf(sc[r / OT][i], v[i], acc[r][i]);
         }

@@ -120,14 +120,26 @@ def exact_weights(rng, n, k):
     return encode(rng.integers(-8, 9, (n, k))), np.exp2(rng.integers(-2, 2, (blocks(n), blocks(k)))).astype(np.float32)
 
 
-def exact_x(rng, m, k):
+def wide_weights(rng, n, k):
+    """The same under scales of 1, four of each 128 in a row +-256: beside x's 448
+    the products of a group span 17 bits, and every sum over 1152 is whole and
+    below 2^23."""
+    w = rng.integers(-8, 9, (n, k))
+    for b in range(blocks(k)):
+        for i in range(n):
+            at = rng.choice(np.arange(128 * b, min(128 * (b + 1), k)), 4, replace=False)
+            w[i, at] = rng.choice([-256, 256], 4)
+    return encode(w), np.ones((blocks(n), blocks(k)), np.float32)
+
+
+def exact_x(rng, m, k, powers=(-2, 2)):
     """bf16 bits of whole multiples of a power of two, each group's largest 448
     times it, so that its codes are the whole numbers and its scale the power."""
     x = rng.integers(-8, 9, (m, k)).astype(np.float64)
     for b in range(blocks(k)):
         end = min(128 * (b + 1), k)
         x[np.arange(m), rng.integers(128 * b, end, m)] = rng.choice([-448, 448], m)
-        x[:, 128 * b:end] *= np.exp2(rng.integers(-2, 2, m))[:, None]
+        x[:, 128 * b:end] *= np.exp2(rng.integers(*powers, m))[:, None]
     return hb.f32_to_bf16(x.astype(np.float32))
 
 

@@ -174,6 +174,16 @@ def test_matvec_exact(gpu, m, k, n):
     assert np.array_equal(got.astype(np.float64), want)
 
 
+@pytest.mark.parametrize("m,k,n", [(1, 1152, 40), (4, 400, 70), (16, 1024, 256)])
+def test_matvec_wide_products(gpu, m, k, n):
+    """Products far apart in size: the small ones stay in the sums."""
+    rng = np.random.default_rng(m + n)
+    codes, scales = f8.wide_weights(rng, n, k)
+    x = f8.exact_x(rng, m, k, (0, 1))
+    want = f8.f64(x) @ f8.values(codes, scales).T
+    assert np.array_equal(matvec(gpu, codes, scales, x, hb.Out.F32, mv_m=m).astype(np.float64), want)
+
+
 @pytest.mark.parametrize("rows,split,waves,unroll", [(16, 1, 1, 1), (16, 16, 16, 1), (32, 8, 8, 1), (64, 4, 4, 1), (32, 2, 4, 4),
                                                      (64, 1, 2, 2), (16, 4, 8, 2), (64, 8, 8, 1)])
 @pytest.mark.parametrize("out", list(hb.Out))

@@ -73,6 +73,16 @@ def test_exact(gpu, tile, m, k, n):
     assert np.array_equal(got.astype(np.float64), want)
 
 
+@pytest.mark.parametrize("m,k,n,ksplit", [(17, 1152, 70, 0), (50, 400, 300, 2), (300, 1152, 515, 0)])
+def test_wide_products(gpu, m, k, n, ksplit):
+    """Products far apart in size: the small ones stay in an f32 output's sums."""
+    rng = np.random.default_rng(m + n)
+    codes, scales = f8.wide_weights(rng, n, k)
+    x = f8.exact_x(rng, m, k, (0, 1))
+    want = f8.f64(x) @ f8.values(codes, scales).T
+    assert np.array_equal(gemm(gpu, codes, scales, x, hb.Out.F32, rows=m, **(dict(ksplit=ksplit) if ksplit else {})).astype(np.float64), want)
+
+
 @pytest.mark.parametrize("out", list(hb.Out))
 @pytest.mark.parametrize("m,k,n", [(17, 2560, 512), (200, 1040, 768), (513, 2064, 1280)])
 def test_outs(gpu, out, m, k, n):
