@@ -45,7 +45,7 @@ def check_h(raw, m, n, want, bound):
 def check(gpu, codes, scales, x, out, seed=0, **form):
     n = codes.shape[0]
     xv, wv = f8.row_values(*f8.quantize_rows(x)), f8.values(codes, scales)
-    want, bound = xv @ wv.T, f8.sum_bound(xv, wv)
+    want, bound = xv @ wv.T, (f8.sum_bound if out == hb.Out.F32 else f8.mfma_bound)(xv, wv)
     y0 = hb.normal_bf16(seed + 9, 1.0, want.shape) if out == hb.Out.Residual else None
     got = gemm(gpu, codes, scales, x, out, y0=y0, **form)
     if out == hb.Out.Swiglu:
@@ -71,6 +71,48 @@ def test_exact(gpu, tile, m, k, n):
     assert np.abs(want).max() * 16 < 2 ** 24
     got = gemm(gpu, codes, scales, x, hb.Out.F32, **tile)
     assert np.array_equal(got.astype(np.float64), want)
+
+
+AHEAD = [dict(bm=256, bn=256, wm=4, wn=2, stages=2, sched=1), dict(bm=128, bn=256, wm=4, wn=2, stages=2, sched=1),
+         dict(bm=64, bn=128, wm=2, wn=2, stages=2, sched=1), dict(bm=32, bn=64, wm=1, wn=4, stages=3)]
+
+
+@pytest.mark.parametrize("tile", TILES + AHEAD + [dict(ksplit=3)])
+@pytest.mark.parametrize("out", [hb.Out.Bf16, hb.Out.Residual])
+@pytest.mark.parametrize("m,k,n", [(1, 16, 1), (33, 144, 70), (257, 2192, 332)])
+def test_exact_bf16(gpu, tile, out, m, k, n):
+    """Products within 12 bits of each other, of which the f8 MFMA cuts none: the
+    exact sums, rounded once."""
+    if "ksplit" in tile and k < 1000:
+        pytest.skip("a K tile a part")
+    rng = np.random.default_rng(m + k + n)
+    codes, scales = f8.exact_weights(rng, n, k)
+    x = f8.exact_x(rng, m, k)
+    want = f8.f64(x) @ f8.values(codes, scales).T
+    y0 = None
+    if out == hb.Out.Residual:
+        y0 = hb.normal_bf16(m, 8.0, want.shape)
+        y0 = hb.f32_to_bf16(np.round(hb.bf16_to_f32(y0)).astype(np.float32))  # wholes: the sum is exact too
+        want = want + f8.f64(y0)
+    assert np.array_equal(gemm(gpu, codes, scales, x, out, y0=y0, **tile), hb.f32_to_bf16(want.astype(np.float32)))
+
+
+SWIGLU = [dict(bm=256, wm=4, wn=2, stages=2), dict(bm=128, wm=2, wn=4, stages=3), dict(bm=64, wm=1, wn=8, stages=3), dict(bm=32, wm=1, wn=8, stages=4),
+          dict(bm=32, wm=2, wn=4, stages=2, sched=1)]
+
+
+@pytest.mark.parametrize("tile", SWIGLU)
+@pytest.mark.parametrize("m,k,n", [(1, 16, 256), (300, 400, 768)])
+def test_exact_swiglu(gpu, tile, m, k, n):
+    """Exact sums under the SwiGLU: h within its own roundings."""
+    rng = np.random.default_rng(m + k + n)
+    codes, scales = f8.exact_weights(rng, n, k)
+    scales = scales * np.float32(2.0 ** -10)  # sums around 1
+    x = f8.exact_x(rng, m, k)
+    s = f8.f64(x) @ f8.values(codes, scales).T
+    g, u = s[:, :n // 2], s[:, n // 2:]
+    got = gemm(gpu, codes, scales, x, hb.Out.Swiglu, bn=256, **tile)
+    check_h(got, m, n // 2, f8.silu(g) * u, f8.swiglu_bound(g, u, 0.0, 0.0))
 
 
 @pytest.mark.parametrize("m,k,n,ksplit", [(17, 1152, 70, 0), (50, 400, 300, 2), (300, 1152, 515, 0)])
@@ -193,7 +235,8 @@ def test_experts(gpu, t, bm, skew):
     for p in range(pairs):
         e, r = flat[order[p]], order[p] // top_k
         wv, row = f8.values(*gu[e]), xv[r:r + 1]
-        s, eb = row @ wv.T, f8.sum_bound(row, wv)
+        bound_of = f8.sum_bound if mv else f8.mfma_bound
+        s, eb = row @ wv.T, bound_of(row, wv)
         g, u = s[:, :inter], s[:, inter:]
         want, bound = f8.silu(g) * u, f8.swiglu_bound(g, u, eb[:, :inter], eb[:, inter:])
         if mv:
@@ -204,7 +247,7 @@ def test_experts(gpu, t, bm, skew):
             check_h(hraw[p:p + 1], 1, inter, want, bound)
             hv = f8.row_values(*f8.unpack_rows(hraw[p:p + 1], 1, inter))
         dv = f8.values(*dn[e])
-        f8.close(got[order[p]:order[p] + 1], hv @ dv.T, f8.sum_bound(hv, dv), "y")
+        f8.close(got[order[p]:order[p] + 1], hv @ dv.T, bound_of(hv, dv), "y")
 
 
 @pytest.mark.parametrize("bm", [16, 64])
