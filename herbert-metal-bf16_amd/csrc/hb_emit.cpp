@@ -146,38 +146,42 @@ static void mv_f8_defaults(hb_desc* d) {
 
 // The forms of the dense 8-bit GEMM: tiles of bm X rows by bn W rows, and what
 // one takes in hundredths of a microsecond as first and else, an offset and a
-// share per K tile: the first alone on its CU, others beside it, which cover each
-// other's latency where several fit in LDS (`beside`), else in turn.
+// share per K tile: the first alone on its CU, others in turn, or beside it
+// (`beside`), where they cover each other's latency.  Fitted to times of 44
+// shapes, 17 to 8192 rows; the form of least time by them takes 0.8% longer than
+// the fastest in the mean, 12% at most (Out::F32: 16 shapes, 1.5% and 9%; the
+// SwiGLU: 34 shapes, the fastest of all).
 struct GemmF8Form {
     uint32_t bm, bn, wm, wn, stages, sched;
     uint32_t first, first_kt, more, more_kt;
     bool beside;
 };
 static const GemmF8Form kGemmF8[] = {
-    {256, 256, 4, 2, 2, 1, 680, 169, 680, 169, false}, {128, 256, 4, 2, 2, 1, 250, 92, 250, 92, false},
-    {64, 128, 2, 2, 2, 1, 130, 46, 100, 33, true},     {32, 64, 1, 4, 3, 0, 30, 28, 20, 12, true},
-    {32, 32, 1, 2, 4, 0, 20, 18, 10, 10, true},
+    {256, 256, 4, 2, 2, 1, 1182, 146, 215, 207, false}, {128, 160, 4, 2, 2, 1, 357, 80, 354, 78, false},
+    {128, 128, 4, 2, 2, 1, 239, 70, 391, 24, false},    {64, 128, 2, 2, 2, 1, 244, 55, 192, 19, false},
+    {32, 64, 1, 4, 3, 0, 205, 29, 6, 12, false},        {32, 32, 1, 2, 4, 0, 180, 28, 21, 6, true},
 };
 static const GemmF8Form kGemmF8Swiglu[] = {
-    {256, 256, 4, 2, 2, 0, 400, 170, 400, 170, false}, {128, 256, 2, 4, 3, 0, 600, 90, 600, 90, false},
-    {64, 256, 1, 8, 3, 0, 240, 73, 240, 73, false},    {32, 256, 1, 8, 4, 0, 30, 60, 30, 60, false},
+    {256, 256, 4, 2, 2, 0, 1080, 154, 434, 196, false}, {128, 256, 4, 4, 3, 0, 577, 96, 590, 103, false},
+    {64, 256, 2, 4, 3, 0, 324, 80, 478, 68, false},     {32, 256, 1, 8, 4, 0, 315, 56, 331, 55, false},
 };
 // Out::F32's, whose products are bf16 (f8.h).
 static const GemmF8Form kGemmF8F32[] = {
-    {128, 128, 4, 2, 2, 1, 315, 97, 230, 93, false}, {64, 128, 2, 4, 2, 0, 253, 69, 97, 64, false},
-    {32, 64, 1, 4, 3, 0, 168, 43, 48, 20, false},    {32, 32, 1, 2, 4, 0, 145, 42, 4, 15, true},
+    {128, 128, 4, 2, 2, 1, 262, 110, 255, 87, false}, {64, 128, 2, 4, 2, 0, 264, 73, 85, 61, false},
+    {32, 64, 1, 4, 3, 0, 203, 40, 30, 21, false},     {32, 32, 1, 2, 4, 0, 177, 39, 0, 15, true},
 };
 
 // The dense form and count of K parts of least time for `rows` rows by those
-// figures.  A split adds the second kernel: a launch and its slabs there and
-// back.  Measured, us, the form taken and the next best:
-//   48 rows, 2560 to 10240: 32 x 64 9.3, 64 x 64 10.2; 32 rows, 9216 to 2560:
-//   32 x 32 in eight parts 8.4, 32 x 64 in eight 8.5, unsplit past 17; 512 rows,
-//   9216 to 2560: 64 x 128 in four parts 28.6, 128 x 256 in four 30.5; 1024 rows,
-//   5120 to 34816: 128 x 256 214, 256 x 256 227; 8192 rows: 256 x 256 1264,
-//   128 x 256 1443.  Of Out::F32: 17 rows, 2560 to 512: 32 x 32 in eight parts 5.7,
-//   in four 6.0; 509 rows, 5008 to 7001: 128 x 128 50.6, 64 x 128 55; 2048 rows,
-//   9216 to 2560: 128 x 128 in two parts 114, whole 130.
+// figures.  All tiles' operands together arrive at 14 TB/s at most (128 x 128 at
+// 8192 rows, 5120 to 8192: 402 us, 256 x 256 354).  A split adds the second
+// kernel: a launch and its slabs there and back.  Measured, us, the form taken
+// and the next best:
+//   48 rows, 2560 to 10240: 32 x 32 9.5, 32 x 64 9.6; 32 rows, 5120 to 1024: 32 x 32
+//   in eight parts 5.8, in four 6.2; 512 rows, 9216 to 2560: 128 x 160 in four parts
+//   26.3, 64 x 128 in four 28.7; 2048 rows: 128 x 160 56.2, 128 x 128 63.7; 2048
+//   rows, 2560 to 10240: 128 x 128 58.9, 128 x 160 73.8.  Of Out::F32: 17 rows, 2560
+//   to 512: 32 x 32 in eight parts 5.7, in four 6.0; 509 rows, 5008 to 7001: 128 x 128
+//   50.6, 64 x 128 55; 2048 rows, 9216 to 2560: 128 x 128 in two parts 114, whole 130.
 static void gemm_f8_dense(hb_desc* d, uint32_t rows) {
     const bool swi = d->out == HB_OUT_SWIGLU;
     const uint32_t kt = cdiv(d->k, 128);
@@ -192,7 +196,9 @@ static void gemm_f8_dense(hb_desc* d, uint32_t rows) {
             uint64_t t = f.first + per * f.first_kt;
             const uint64_t more = f.more + per * f.more_kt;
             if (all > 256) t += f.beside ? (all - 256) * more / 256 : (all - 1) / 256 * more;
-            if (s > 1) t += 250 + (uint64_t)rows * d->n * s / 10000;
+            const uint64_t floor = all * (f.bm + f.bn) * per / 1100;
+            t = t > floor ? t : floor;
+            if (s > 1) t += 240 + (uint64_t)rows * d->n * s / 9000;
             if (t < best) best = t, form = &f, parts = s;
         }
     };
@@ -727,8 +733,7 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             if (swi && (d.n % 256 || d.rows_of == HB_ROWS_SCATTER))
                 return fail(HB_ERR_UNSUPPORTED, "gemm_f8 Out::Swiglu: gate and up rows each a multiple of 128, no scatter");
             if (d.bm > 256 || !pow2(d.bm) || d.bm < 32 || d.bn > 256 || d.bn % 32 || !d.wm || !d.wn || d.wm * d.wn > 16 ||
-                (d.mfma != 16 && (d.mfma != 32 || d.out == HB_OUT_F32)) || d.bm % (d.wm * d.mfma) || d.bn % (d.wn * d.mfma) ||
-                (swi && (d.bn != 256 || d.bn / d.wn % (2 * d.mfma))))
+                d.mfma != 16 || d.bm % (d.wm * 16) || d.bn % (d.wn * 16) || (swi && (d.bn != 256 || d.bn / d.wn % 32)))
                 return fail(HB_ERR_UNSUPPORTED, "gemm_f8: tiles of 32 to 256 X rows (a power of 2) by up to 256 W rows (Out::Swiglu 256), "
                                                 "whole fragments of 16 a wave");
             if (d.dbuf < 1 || d.dbuf > 3 || !d.band || gemm_f8_lds(d) > 160 * 1024)
@@ -746,10 +751,10 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             } else if (d.ksplit > 1) {
                 rows = "_ks" + std::to_string(d.ksplit);
             }
-            if (d.sched > 1 || (d.sched && (d.dbuf != 1 || d.bn / d.wn < 4 * d.mfma)))
+            if (d.sched > 1 || (d.sched && (d.dbuf != 1 || d.bn / d.wn < 64)))
                 return fail(HB_ERR_UNSUPPORTED, "gemm_f8 (fragments ahead): two stages, four fragments of W a wave");
-            snprintf(name, sizeof name, "gemm_f8_%ux%u_%s_t%ux%u_w%ux%u_x%u_d%u_b%u%s%s", d.k, d.n, swi ? "sw" : out_tag(d.out), d.bn,
-                     d.bm, d.wn, d.wm, d.mfma, d.dbuf, d.band, d.sched ? "_fa" : "", rows.c_str());
+            snprintf(name, sizeof name, "gemm_f8_%ux%u_%s_t%ux%u_w%ux%u_d%u_b%u%s%s", d.k, d.n, swi ? "sw" : out_tag(d.out), d.bn,
+                     d.bm, d.wn, d.wm, d.dbuf, d.band, d.sched ? "_fa" : "", rows.c_str());
             e->name = name;
             e->source = "gemm_f8.hip";
             e->threads = 64 * d.wm * d.wn;
@@ -758,7 +763,7 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
                           D("HB_ROWS", d.rows_of), D("HB_TOPK", experts ? d.top_k : 1), D("HB_E", experts ? d.experts : 1),
                           D("HB_WIDE", d.out == HB_OUT_F32), D("HB_BM", d.bm), D("HB_BN", d.bn), D("HB_WM", d.wm), D("HB_WN", d.wn),
                           D("HB_STAGES", d.dbuf + 1), D("HB_BAND", d.band), D("HB_KSPLIT", d.ksplit > 1 ? d.ksplit : 1),
-                          D("HB_SCHED", d.sched), D("HB_MFMA", d.mfma)};
+                          D("HB_SCHED", d.sched)};
             return HB_OK;
         }
         case HB_KIND_ROUND_PROBE:

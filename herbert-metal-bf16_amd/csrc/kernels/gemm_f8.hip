@@ -38,7 +38,7 @@ constexpr u32 K = HB_K, N = HB_N;
 constexpr int OUT = HB_OUT, ROWS = HB_ROWS;
 constexpr u32 TOPK = HB_TOPK, BM = HB_BM, BN = HB_BN, WM = HB_WM, WN = HB_WN;
 constexpr u32 NWV = WM * WN, NTH = 64 * NWV, NS = HB_STAGES, KSP = HB_KSPLIT;
-constexpr u32 FM = HB_MFMA, FR = FM * FM / 64, MK = FM / 16;  // a block of FM x FM: sums a lane, MFMAs
+constexpr u32 FM = 16, FR = 4;                           // a block of FM x FM: sums a lane
 constexpr u32 TM = BM / WM, TN = BN / WN, IM = TM / FM, IN = TN / FM;
 constexpr bool SWI = OUT == 3;
 constexpr u32 KB = f8_blocks(K), KBP = (KB + 63) / 64 * 64, NB = f8_blocks(N), NOUT = SWI ? N / 2 : N, BF = SWI ? BN / 2 : BN;
@@ -64,7 +64,6 @@ constexpr bool AHEAD = HB_SCHED == 1;
 #ifndef HB_WIDE
 #define HB_WIDE 0
 #endif
-static_assert(!HB_WIDE || FM == 16, "the bf16 products: blocks of 16 x 16");
 // The W row of a tile's row r, from the tile's first column on: a wave's gate
 // rows stand before the up rows of the same features.
 constexpr u32 w_row(u32 r) {
@@ -268,21 +267,14 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
             for (u32 e = 0; e < FR; e++) acc[i][j][e] = 0.0f;
     const u32 fr = lane % FM, fc = lane / FM, fsw = (fr >> 1) & 7u;
     const u32 wbase = (wn * TN + fr) * 8, xbase = (wm * TM + fr) * 8;
-    struct Fragment {
-        i32x8 k[MK];
-    };
+    typedef i32x8 Fragment;
     auto fragment = [&](const u32x4* p) HB_INLINE -> Fragment {
-        Fragment f;
-#pragma unroll
-        for (u32 q = 0; q < MK; q++) {
-            const u32x4 a = p[(fc + 4 * q) ^ fsw], b = p[(fc + 4 / MK + 4 * q) ^ fsw];
-            f.k[q] = i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
-        }
-        return f;
+        const u32x4 a = p[fc ^ fsw], b = p[(fc + 4) ^ fsw];
+        return i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
     };
 #if HB_WIDE
     typedef F8Wide Operand;
-    auto operand_of = [&](const Fragment& f) HB_INLINE -> Operand { return f8_wide(f.k[0]); };
+    auto operand_of = [&](const Fragment& f) HB_INLINE -> Operand { return f8_wide(f); };
 #else
     typedef Fragment Operand;
     auto operand_of = [&](const Fragment& f) HB_INLINE -> Operand { return f; };
@@ -302,20 +294,11 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
     };
     float last_sw = 0.0f;
     auto product_of = [&](const Operand& w, const Operand& x) HB_INLINE -> block_t {
-        block_t t = {};
 #if HB_WIDE
-        t = f8_product(w, x);
+        return f8_product(w, x);
 #else
-#pragma unroll
-        for (u32 q = 0; q < MK; q++) {
-#if HB_MFMA == 16
-            t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.k[q], x.k[q], t, 0, 0, 0, 0, 0, 0);
-#else
-            t = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w.k[q], x.k[q], t, 0, 0, 0, 0, 0, 0);
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, block_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
 #endif
-        }
-#endif
-        return t;
     };
     auto add = [&](u32 i, u32 j, const block_t& t, float s) HB_INLINE {
 #pragma unroll
@@ -397,11 +380,14 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
                 for (u32 j = 0; j < IM; j++) {
                     const u32 q = i * IM + j;
                     t[q % 2] = product_of(wo, xo[j]);
-                    __builtin_amdgcn_sched_barrier(0);
                     if (q) {
                         const u32 p = q - 1;
+                        // Two MFMAs, then the eight fmas of the two before them
+                        // (8192 x 34816 x 5120: 1183 us, one by one in the
+                        // order written 1257, left to the compiler 1180 to 1210).
+                        __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x2, 8, 0);
                         add(p / IM, p % IM, t[p % 2], sc[p % IM] * (p / IM == i ? sw : last_sw));
-                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
                 last_sw = sw;
@@ -427,6 +413,9 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
         else WAIT_VM(0);
         STAGE_BARRIER();
         u32 st = 0;
+        // As a loop for few tiles too: unrolled whole, 16 waves miss the
+        // instruction cache (1024 rows, 1024 to 4096 SwiGLU: 27 us, 14 as one).
+#pragma unroll 1
         for (u32 kt = kt0; kt < kt1; kt++) {
             // Tile kt + NS - 1 into the stage that tile kt - 1 used: every wave
             // has passed the barrier after its last read of it.

@@ -71,7 +71,7 @@ def test_reference_codes():
     (lambda hb: hb.matvec_f8(128, 128, hb.Out.Swiglu), "multiple of 128"),
     (lambda hb: hb.matvec_f8(128, 256, hb.Out.Swiglu, rows=16), "rows a wave"),
     (lambda hb: hb.matvec_f8(128, 64, hb.Out.Bf16, rows=128), "rows a wave"),
-    (lambda hb: hb.gemm_f8(128, 64, hb.Out.F32, mfma=32), "16 a wave"),
+    (lambda hb: hb.Desc(kind=hb.Kind.GEMM_F8, k=128, n=64, out=hb.Out.Bf16, mfma=32), "16 a wave"),
     (lambda hb: hb.matvec_f8(128, 64, hb.Out.Bf16, waves=3), "waves"),
     (lambda hb: hb.matvec_f8(128, 64, hb.Out.Bf16, split=8, waves=4), "split"),
     (lambda hb: hb.matvec_f8(128, 64, hb.Out.Bf16, unroll=5), "unroll"),
