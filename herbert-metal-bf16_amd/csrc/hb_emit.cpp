@@ -117,13 +117,15 @@ static void mv_f8_defaults(hb_desc* d) {
     const uint32_t nt = cdiv(d->n, 16), kt = cdiv(d->k, 128);
     const bool swi = d->out == HB_OUT_SWIGLU;
     if (d->rows_of != HB_ROWS_DENSE) {
-        // The experts: 64 rows a wave and short splits once the block's pairs
-        // make 1024 workgroups of 32 rows (8 tokens of 8 experts, 2048 to 1024:
-        // 20.8, 32 rows 22.5; 1 token 4.2 with 32, 64 rows 5.1).
+        // The experts: 64 rows a wave once the block's pairs make 1024 workgroups
+        // of 32 rows (1 token of 8 experts, 2048 to 1024: 4.2 with 32, 64 rows
+        // 5.1), and four parts of K, of a short one none (4 tokens 11.7, two
+        // parts 15.5; 16 tokens 38.2 and 39.9; 512 to 2048 at 8 tokens 11.6, two
+        // parts 12.3).
         const bool many = (uint64_t)d->rows_max * d->top_k * cdiv(nt, 2) >= 1024;
         if (!d->rows) d->rows = many ? 64 : 32;
         if (!d->split) {
-            d->split = !many ? 4 : kt >= 8 ? 2 : 1;
+            d->split = !many || kt >= 8 ? 4 : 1;
             while (d->split > kt || (d->mv_waves && d->split > d->mv_waves)) d->split /= 2;
             if (!d->split) d->split = 1;
         }
@@ -191,7 +193,7 @@ static void gemm_f8_dense(hb_desc* d, uint32_t rows) {
     auto consider = [&](const GemmF8Form& f) {
         const uint64_t tiles = (uint64_t)cdiv(rows, f.bm) * cdiv(d->n, f.bn);
         for (uint32_t s = 1; s <= 8; s *= 2) {
-            if (s > 1 && (swi || d->n % 4 || s > kt || tiles * s > 1024)) break;
+            if (s > 1 && (swi || s > kt || tiles * s > 1024)) break;
             const uint64_t per = cdiv(kt, s), all = tiles * s;
             uint64_t t = f.first + per * f.first_kt;
             const uint64_t more = f.more + per * f.more_kt;
@@ -407,7 +409,7 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             return HB_OK;
         }
         case KIND_SPLITK_REDUCE:
-            if (!d.n || d.n % 4 || d.ksplit < 2 || d.ksplit > 16 || d.out > HB_OUT_RESIDUAL)
+            if (!d.n || (d.n % 4 && !d.form) || d.ksplit < 2 || d.ksplit > 16 || d.out > HB_OUT_RESIDUAL)
                 return fail(HB_ERR_INVALID, "split-K reduce: N a multiple of 4, 2..16 parts");
             snprintf(name, sizeof name, "gemm_splitk_%u_%s_s%u%s", d.n, out_tag(d.out), d.ksplit, d.form ? "_once" : "");
             e->name = name;
@@ -738,8 +740,8 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
                                                 "whole fragments of 16 a wave");
             if (d.dbuf < 1 || d.dbuf > 3 || !d.band || gemm_f8_lds(d) > 160 * 1024)
                 return fail(HB_ERR_UNSUPPORTED, "gemm_f8: 2 to 4 stages within 160 KiB of LDS, a band");
-            if (d.ksplit > 16 || (d.ksplit > 1 && (experts || swi || d.n % 4 || d.ksplit > cdiv(d.k, 128))))
-                return fail(HB_ERR_UNSUPPORTED, "gemm_f8 split K: 2..16 parts of whole K tiles, dense rows, N a multiple of 4");
+            if (d.ksplit > 16 || (d.ksplit > 1 && (experts || swi || d.ksplit > cdiv(d.k, 128))))
+                return fail(HB_ERR_UNSUPPORTED, "gemm_f8 split K: 2..16 parts of whole K tiles, dense rows");
             if (experts && (!d.top_k || d.top_k > d.experts || d.experts > 1024 || !d.tiles || !d.rows_max ||
                             (uint64_t)d.rows_max * d.top_k >= (1u << 28) || (d.out != HB_OUT_BF16 && !swi)))
                 return fail(HB_ERR_INVALID, "gemm_f8 over experts: top_k, experts (<= 1024), tiles and rows_max (below 2^28 pairs), bf16 out");
@@ -817,7 +819,7 @@ uint32_t groups_of(const hb_desc& d, uint32_t m) {
             return cdiv(m, bm) * nt * (d.ksplit > 1 ? d.ksplit : 1);  // gemm_mma_groups
         }
         case KIND_SPLITK_REDUCE: {  // 4 outputs a thread, at most 8 workgroups a CU
-            const uint64_t g = ((uint64_t)m * (d.n / 4) + 255) / 256;
+            const uint64_t g = (((uint64_t)m * d.n + 3) / 4 + 255) / 256;
             return (uint32_t)(g < 2048 ? g : 2048);
         }
         case HB_KIND_MATVEC: {  // matvec_groups / matvec_split_groups / matvec_full_groups
@@ -1159,11 +1161,11 @@ extern "C" uint64_t hb_f8_row_bytes(uint32_t k) { return hb::f8_shape(k, 1) ? hb
 
 extern "C" uint32_t hb_f8_tile_rows(uint32_t rows, uint32_t top_k, uint32_t experts) {
     // The layer's two products, us (256 experts of 2048 / 512, top 8; for tiles
-    // past 16 rows with x's quantisation): 8 rows 32 with tiles of 16, 34 with
-    // 32; 16 rows 57 and 53; 512 rows 136 with 32, 142 with 64; 1024 rows 149 and
+    // past 16 rows with x's quantisation): 8 rows 34 with tiles of 16, 35 with
+    // 32; 12 rows 50 and 45; 16 rows 58 and 53; 512 rows 136 with 32, 142 with 64; 1024 rows 149 and
     // 147; 2048 rows 187 with 64, 180 with 128.
     const uint64_t pairs = (uint64_t)rows * top_k;
-    return 8 * pairs <= 3ull * experts ? 16 : pairs <= 24ull * experts ? 32 : pairs <= 48ull * experts ? 64 : 128;
+    return 4 * pairs <= experts ? 16 : pairs <= 24ull * experts ? 32 : pairs <= 48ull * experts ? 64 : 128;
 }
 
 extern "C" uint64_t hb_q4_bytes(uint32_t k, uint32_t n, uint32_t group) {

@@ -553,7 +553,7 @@ int hb_kernel_precompile(const hb_desc* desc) {
         rd.n = d.n;
         rd.out = d.out;
         rd.ksplit = d.ksplit;
-        rd.form = d.kind == HB_KIND_GEMM_F8 && d.out == HB_OUT_RESIDUAL;  // one rounding
+        rd.form = d.kind == HB_KIND_GEMM_F8;  // any N, one rounding
         return hb_kernel_precompile(&rd);
     }
     return HB_OK;
@@ -579,7 +579,7 @@ int hb_kernel_build(hb_gpu* g, const hb_desc* desc, int32_t* kernel) {
         rd.n = d.n;
         rd.out = d.out;
         rd.ksplit = d.ksplit;
-        rd.form = d.kind == HB_KIND_GEMM_F8 && d.out == HB_OUT_RESIDUAL;  // one rounding
+        rd.form = d.kind == HB_KIND_GEMM_F8;  // any N, one rounding
         if ((rc = hb_kernel_build(g, &rd, &k.reduce))) {
             hipModuleUnload(k.module);
             return rc;

@@ -22,6 +22,11 @@
 // does not matter).  X's scales of eight K tiles at a time go the same way into
 // one of two places, 32 bytes a row; W's, all of a tile's blocks, are read once.
 //
+// 8192 x 34816 x 5120: 1183 us, 2.47 PFLOP/s (the library's product under one
+// scale for all 1059); the MFMAs are busy for 55 to 60% of it, the scales' fmas and
+// the barrier a K tile hold the rest.  509 x 7001 x 5008 in f32 by bf16 products:
+// 47 us with x quantised, one tile on each of 220 CUs.
+//
 // Out::Swiglu: W holds [gate (N / 2) | up (N / 2)] rows; a tile covers 128
 // features, a wave's first fragments their gate rows and its others the up
 // rows, so a lane has both sums of a feature.  h = rne(g * sigmoid(g) * u) in
@@ -74,7 +79,7 @@ static_assert(!SWI || LROWS % TN == 0 || (TN / 2) % LROWS == 0, "SwiGLU rows of 
 static_assert(!AHEAD || (NS == 2 && IN >= 4), "fragments ahead: two stages, four fragments of W a wave");
 static_assert(K % 16 == 0 && BM % 32 == 0 && BN % 16 == 0 && TM % FM == 0 && TN % FM == 0, "tile");
 static_assert(!SWI || (BN == 256 && IN % 2 == 0 && N % 256 == 0 && KSP == 1 && ROWS != 2), "SwiGLU");
-static_assert(KSP == 1 || (OUT == 1 && ROWS == 0 && N % 4 == 0), "split K: f32 partial sums");
+static_assert(KSP == 1 || (OUT == 1 && ROWS == 0), "split K: f32 partial sums");
 static_assert(NS >= 2 && NS <= 4, "stages");
 
 #define HB_INLINE __attribute__((always_inline))

@@ -17,7 +17,8 @@
 // Each wave loads its own W rows and x rows straight into LDS
 // (buffer_load_dwordx4 ... lds), HB_UNROLL tiles of 128 K ahead, with no barrier
 // in its loop: whole lines of 8 W rows and of 4 x rows a load.  (W loaded as the
-// operand, 64 bytes of 16 rows at a time, reached 4.4 TB/s.)  The 16 lanes of an
+// operand, 64 bytes of 16 rows at a time, reached 4.4 TB/s; now 2560 to 151936
+// at 4 rows 64 us, 6.1 TB/s, and a short matrix its launch, 4096 to 2560 4.7.)  The 16 lanes of an
 // x row find its block's scale and codes, which go back to LDS as the operand;
 // chunks stand at chunk ^ row there, and W's at chunk ^ row >> 1.
 #include "f8.h"

@@ -123,14 +123,17 @@ enum hb_kind {
      * 448, code = the e4m3 nearest to 448 x / a, ties to even; a group with a
      * NaN or an infinity stands for NaN.  k a multiple of 16.
      * "f8 rows" (activations): a row = its k codes, then the scales of its
-     * groups of 128 along k, in all a multiple of 128 bytes (hb_f8_row_bytes).  "f8 matrix" (weights): the codes [n][k], then the
-     * scales [ceil(n/128)][ceil(k/128)] of its blocks of 128 x 128
-     * (hb_f8_bytes): what an 8-bit checkpoint holds, one after the other. */
+     * groups of 128 along k, in all a multiple of 128 bytes (hb_f8_row_bytes).
+     * "f8 matrix" (weights): the codes [n][k], then the scales
+     * [ceil(n/128)][ceil(k/128)] of its blocks of 128 x 128 (hb_f8_bytes): what
+     * an 8-bit checkpoint holds, one after the other. */
     HB_KIND_F8_QUANTIZE = 20,   /* form 0: W [n][k] bf16 -> f8 matrix, m = matrices; HB_F8_ROWS: x
                                  * [m][k] bf16 -> f8 rows */
     HB_KIND_F8_DEQUANTIZE = 21, /* the same back, code * scale rounded once to bf16 */
-    HB_KIND_GEMM_F8 = 22,       /* Y[m][n] = X.W^T of f8 rows X and an f8 matrix W, f32 sums; dense,
-                                 * or the experts' over moe_sort's tiles of bm rows (rows_of) */
+    HB_KIND_GEMM_F8 = 22,       /* Y[m][n] = X.W^T of f8 rows X and an f8 matrix W; dense, or the
+                                 * experts' over moe_sort's tiles of bm rows (rows_of).  f32 sums
+                                 * for HB_OUT_F32; else those of the f8 MFMA within each 128 of K,
+                                 * some 2^-16 off on normal operands */
     HB_KIND_MATVEC_F8 = 23      /* the same for m <= mv_m <= 16 rows of bf16 x, quantised as they are
                                  * loaded; or the experts' over tiles of 16 rows (rows_of) */
 };
@@ -331,9 +334,9 @@ double hb_compile_seconds(hb_gpu *gpu);
  *     or y, h may be y or x, or either an element gate, as a whole; no other
  *     overlap.
  * The bindings of these (ROUTE_TOPK, Q4_*, F8_*, GEMM_F8, MATVEC_Q4 and _F8,
- * BLOCK_NORM) start at a multiple of their element (2 bytes,
- * f32 and u32 4, q4, f8 matrices and f8 rows and MATVEC_F8's X 16), and what a launch writes overlaps nothing else it
- * binds: both are checked.  Of MATVEC_Q4: HB_OUT_BF16, _F32, _RESIDUAL
+ * BLOCK_NORM) start at a multiple of their element (2 bytes, f32 and u32 4;
+ * q4, f8 matrices, f8 rows and MATVEC_F8's X 16), and what a launch writes
+ * overlaps nothing else it binds: both are checked.  Of MATVEC_Q4: HB_OUT_BF16, _F32, _RESIDUAL
  * (y = rne(y + sum), one rounding) and _SWIGLU (n / 2 a multiple of 16, h =
  * rne(g * sigmoid(g) * u) of the f32 sums).  The sums go through
  * 31 |x|: an infinite x, or 128 of them past 2^116, give NaN.  Over experts (rows_of HB_ROWS_GATHER: x rows through the list,
@@ -342,7 +345,8 @@ double hb_compile_seconds(hb_gpu *gpu);
  * Of MATVEC_F8 the same Outs, with n / 2 a multiple of 128 for _SWIGLU; of
  * GEMM_F8 too, whose _SWIGLU (dense or gathered) writes h, rounded to bf16 and
  * quantised, as f8 rows: the next GEMM_F8's X.  Its tiles' rows are bm, the
- * sort's.  X and each W of a GEMM_F8 hold less than 2 GiB.
+ * sort's.  X and each W of a GEMM_F8, and X of MATVEC_F8's experts, hold less
+ * than 2 GiB.
  * `m` is the rows of the block (the kernels read state[3], never beyond m).
  * A split-K GEMM (ksplit > 1) launched over more rows than any earlier
  * split launch on this context first grows the context's workspace: the

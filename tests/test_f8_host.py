@@ -99,7 +99,7 @@ def test_reference_codes():
     (lambda hb: hb.gemm_f8(128, 64, hb.Out.Bf16, bm=256, bn=256, stages=3), "stages within"),
     (lambda hb: hb.gemm_f8(128, 64, hb.Out.Bf16, stages=5), "stages"),
     (lambda hb: hb.gemm_f8(128, 64, hb.Out.Bf16, ksplit=2), "split K"),
-    (lambda hb: hb.gemm_f8(4096, 66, hb.Out.Bf16, ksplit=2), "split K"),
+    (lambda hb: hb.gemm_f8(4096, 66, hb.Out.Bf16, ksplit=17), "split K"),
     (lambda hb: hb.gemm_f8(4096, 256, hb.Out.Swiglu, ksplit=2), "split K"),
     (lambda hb: hb.gemm_f8(128, 64, 4), "out"),
     (lambda hb: hb.route_topk(0, 1), "1 to 1024"),

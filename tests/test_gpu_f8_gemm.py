@@ -149,6 +149,21 @@ def test_split_k(gpu, parts, out):
     check(gpu, codes, scales, hb.normal_bf16(parts, 1.0, (50, 2704)), out, rows=50, ksplit=parts)
 
 
+@pytest.mark.parametrize("n", [1, 3, 301, 334])
+@pytest.mark.parametrize("out", [hb.Out.Bf16, hb.Out.F32, hb.Out.Residual])
+def test_split_k_ragged(gpu, out, n):
+    """Any N and fewer rows than launched: exact sums, the rows behind left as they are."""
+    rng = np.random.default_rng(n)
+    codes, scales = f8.exact_weights(rng, n, 1040)
+    x = f8.exact_x(rng, 53, 1040)
+    want = f8.f64(x) @ f8.values(codes, scales).T
+    for m in (53, 31):
+        y0 = np.zeros(want.shape, np.uint16) if out == hb.Out.Residual else None
+        got = gemm(gpu, codes, scales, x, out, m=m, y0=y0, rows=53, ksplit=4)
+        exact = want[:m].astype(np.float32)
+        assert np.array_equal(got, exact if out == hb.Out.F32 else hb.f32_to_bf16(exact + np.float32(0)))
+
+
 @pytest.mark.parametrize("out", [hb.Out.Bf16, hb.Out.Swiglu])
 def test_fewer_rows_than_launched(gpu, out):
     """state[3] below the launch's rows: the rows behind stay as they are."""
