@@ -277,7 +277,9 @@ typedef struct hb_desc {
      * adding the parts in order 0..ksplit-1 and applying Out -- for shapes
      * whose tiles fill less than a round of the CUs.  Each part must hold a
      * whole number of K tiles (sched 3: an even number), and N must be a
-     * multiple of 4 (the second kernel's vector width).  One launch handle:
+     * multiple of 4 (the second kernel's vector width).  Of a dense GEMM_F8,
+     * unless HB_OUT_SWIGLU: parts of whole K tiles of 128, equal or one
+     * apart, and any N.  One launch handle:
      * hb_launch / hb_time run both kernels.  The workspace grows on the
      * first launch over more rows than any before it on the context: that
      * launch synchronizes the stream and calls hipFree / hipMalloc (not
