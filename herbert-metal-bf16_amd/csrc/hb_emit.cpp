@@ -738,6 +738,9 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
                 d.mfma != 16 || d.bm % (d.wm * 16) || d.bn % (d.wn * 16) || (swi && (d.bn != 256 || d.bn / d.wn % 32)))
                 return fail(HB_ERR_UNSUPPORTED, "gemm_f8: tiles of 32 to 256 X rows (a power of 2) by up to 256 W rows (Out::Swiglu 256), "
                                                 "whole fragments of 16 a wave");
+            // A wave's loads are 8 rows a wave of the workgroup apart: the swizzle
+            // of the first is that of the others where these are multiples of 16.
+            if (d.wm * d.wn % 2) return fail(HB_ERR_UNSUPPORTED, "gemm_f8: an even number of waves");
             if (d.dbuf < 1 || d.dbuf > 3 || !d.band || gemm_f8_lds(d) > 160 * 1024)
                 return fail(HB_ERR_UNSUPPORTED, "gemm_f8: 2 to 4 stages within 160 KiB of LDS, a band");
             if (d.ksplit > 16 || (d.ksplit > 1 && (experts || swi || d.ksplit > cdiv(d.k, 128))))

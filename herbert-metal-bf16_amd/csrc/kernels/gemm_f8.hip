@@ -76,6 +76,8 @@ constexpr u32 w_row(u32 r) {
 }
 // Its rows LROWS apart lie as far from each other wherever they start.
 static_assert(!SWI || LROWS % TN == 0 || (TN / 2) % LROWS == 0, "SwiGLU rows of a wave's loads");
+static_assert(LROWS % 16 == 0, "the rows of a wave's loads share their swizzle");
+static_assert((NS - 2) * LMIN < 64, "vmcnt");
 static_assert(!AHEAD || (NS == 2 && IN >= 4), "fragments ahead: two stages, four fragments of W a wave");
 static_assert(K % 16 == 0 && BM % 32 == 0 && BN % 16 == 0 && TM % FM == 0 && TN % FM == 0, "tile");
 static_assert(!SWI || (BN == 256 && IN % 2 == 0 && N % 256 == 0 && KSP == 1 && ROWS != 2), "SwiGLU");
@@ -194,8 +196,8 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
 
     // This wave's loads of a stage, wave loads wave, wave + NWV, ..: LDS slot p
     // of the operand's stage holds (row p / 8, chunk p % 8 ^ row >> 1), so that a
-    // lane's chunk is the same in each, and its rows LROWS apart: one address
-    // a lane and constants.  Rows past the operand's end lie past its
+    // lane's chunk is the same in each (LROWS is a multiple of 16), and its rows
+    // LROWS apart: one address a lane and constants.  Rows past the operand's end lie past its
     // resource's range, an experts' tile's rows past its own are put there:
     // zeros without a memory access.  (The scalar offset, which the range
     // check takes off the range, stays within a row.)

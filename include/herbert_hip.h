@@ -212,7 +212,8 @@ typedef struct hb_desc {
     /* GEMM tile: bm rows of X x bn rows of W per workgroup, K by bk,
      * wm x wn wavefronts, MFMA block 16 or 32, dbuf = LDS stages - 1 (0..3),
      * LDS swizzle (0 = conflict-free for the K step, s + 1 = shift s), tile
-     * order (0 plain, 1 XCD-contiguous). 0 = the kind's default. */
+     * order (0 plain, 1 XCD-contiguous). 0 = the kind's default.  GEMM_F8: an
+     * even number of wavefronts. */
     uint32_t bm, bn, bk, wm, wn, mfma, dbuf, swz, order;
     /* matvec: rows of x (1..16); waves sharing a row block's K (split: 1,
      * 2, 4; 8 and 16 with at least as many mv_waves); persistent workgroups
