@@ -269,20 +269,28 @@ extern "C" __global__ __launch_bounds__(256) void HB_NAME(const void* __restrict
     // Lane i has choice i.
     const bool has = lane < TOPK && counts;
     const float s = has ? score(scores, base + expert) : -HB_INF;
+    // e^(s - mx).  A difference of -60 rounded to f32 would leave the exponential
+    // 2e-6 off: its rest goes in by the first term.
+    auto relative = [&]() __attribute__((always_inline)) {
+        const float d = s == mx ? 0.0f : s - mx, back = d - s, rest = (s - (d - back)) + (-mx - back);
+        const float e = has ? hb_expf(d) : 0.0f;
+        return has && s != mx && e > 0.0f ? __builtin_fmaf(e, rest, e) : e;
+    };
+    if constexpr (RENORM) {
+        // The chosen ones alone, over their own sum.
+        const u32 top = wave_max(has ? ordered(s) : 0u);
+        mx = top ? unordered(top) : 0.0f;
+    }
     float p;
     if constexpr (SIGMOID) {
-        p = has ? hb_sigmoid(s) : 0.0f;
+        // 1 / (1 + e^-s) is subnormal below -87 and 0 from -88.73 on, where e^s,
+        // the same to f32, is not.
+        p = !has ? 0.0f : s < -87.0f ? hb_expf(s) : hb_sigmoid(s);
+        // Where all chosen lie below 0, e^s / (1 + e^s) over e^mx: no row's sum
+        // comes near 0, however low its scores.
+        if (RENORM && mx < 0.0f) p = has ? relative() / (1.0f + hb_expf(s)) : 0.0f;
     } else {
-        if constexpr (RENORM) {
-            // The chosen ones' exponentials over their own sum.
-            const u32 top = wave_max(has ? ordered(s) : 0u);
-            mx = top ? unordered(top) : 0.0f;
-        }
-        // A difference of -60 rounded to f32 would leave the exponential 2e-6
-        // off: its rest goes in by the first term.
-        const float d = s == mx ? 0.0f : s - mx, back = d - s, rest = (s - (d - back)) + (-mx - back);
-        p = has ? hb_expf(d) : 0.0f;
-        p = has && s != mx && p > 0.0f ? __builtin_fmaf(p, rest, p) : p;
+        p = relative();
         if constexpr (!RENORM) p = sum > 0.0f ? p / sum : 0.0f;
     }
     if constexpr (RENORM) {
