@@ -1019,6 +1019,10 @@ static int need(const uint64_t* sizes, uint32_t i, uint64_t bytes, const char* w
     return HB_OK;
 }
 
+// Whole workgroups of 256 threads, `each` threads an item, past what a grid
+// holds: fewer than 2^32 threads.
+static bool past_grid(uint64_t items, uint64_t each) { return items > ((1ull << 32) - 256) / each; }
+
 int check_bindings(const hb_desc& d, const uint64_t* s, uint32_t nbind, uint32_t m) {
     int rc = HB_OK;
     (void)nbind;
@@ -1069,11 +1073,16 @@ int check_bindings(const hb_desc& d, const uint64_t* s, uint32_t nbind, uint32_t
             if (d.kind == HB_KIND_MATVEC_F8 && !dense && (d.rows_of == HB_ROWS_GATHER ? 1 : d.top_k) * (uint64_t)m * d.k * 2 > 0x7fffffffull)
                 return fail(HB_ERR_UNSUPPORTED, "matvec_f8: X at most 2 GiB - 1 bytes");
         } else if (d.kind == HB_KIND_ROUTE_TOPK) {
-            if (m >= (1u << 26)) return fail(HB_ERR_UNSUPPORTED, "route_topk: too many rows in one launch");
+            if (past_grid(m, 64)) return fail(HB_ERR_UNSUPPORTED, "route_topk: too many rows in one launch");
         } else if (d.kind == HB_KIND_F8_QUANTIZE || d.kind == HB_KIND_F8_DEQUANTIZE) {
-            // Rows of at most 2^20, matrices of at most 2^44 elements.
-            const uint64_t each = f8_rows_form(d) ? cdiv(d.k, 16) : (uint64_t)cdiv(d.n, 128) * 128 * (cdiv(d.k, 128) * 8);
-            if (each >> 32 || m * each >> 32) return fail(HB_ERR_UNSUPPORTED, "f8: too many elements in one launch");
+            // groups_of's: 16 lanes a group of a row, a workgroup a block of a
+            // matrix, 16 elements a thread back.  Rows of at most 2^20 elements,
+            // matrices of at most 2^44.
+            const uint64_t kb = cdiv(d.k, 128);
+            const uint64_t each = d.kind == HB_KIND_F8_DEQUANTIZE ? (uint64_t)d.k / 16 * (f8_rows_form(d) ? 1 : d.n)
+                                  : f8_rows_form(d)               ? 16 * kb
+                                                                  : 256 * kb * cdiv(d.n, 128);
+            if (past_grid(m, each)) return fail(HB_ERR_UNSUPPORTED, "f8: too many elements in one launch");
         } else if (d.kind == HB_KIND_GEMM_F8) {
             const bool dense = d.rows_of == HB_ROWS_DENSE;
             if (!dense && m > d.rows_max) return fail(HB_ERR_INVALID, "m beyond the kernel's rows_max");
@@ -1086,7 +1095,7 @@ int check_bindings(const hb_desc& d, const uint64_t* s, uint32_t nbind, uint32_t
         } else if (d.kind == HB_KIND_BLOCK_NORM) {
             if ((uint64_t)m * norm_threads(d.n) >> 32)
                 return fail(HB_ERR_UNSUPPORTED, "block_norm: too many rows in one launch");
-        } else if (m * q4_tiles(d.k, d.n) >= (1u << 26)) {
+        } else if (past_grid(m * q4_tiles(d.k, d.n), 64)) {
             return fail(HB_ERR_UNSUPPORTED, "q4: too many matrices in one launch");
         }
         const AccessList l = accesses(d, m);

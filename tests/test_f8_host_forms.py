@@ -57,3 +57,58 @@ def test_odd_waves_refused(hb, gpu, tile, out):
 def test_odd_waves_of_experts_refused(hb, gpu, bm):
     with pytest.raises(hb.HerbertError, match="even number of waves"):
         gpu.pipeline(hb.experts_f8(256, 512, hb.Out.Bf16, hb.Rows.Gather, 2, 8, 64, bm, wm=1, wn=1, bn=32))
+
+
+def limit(hb, gpu, desc, most, refusal="too many"):
+    """A launch over `most` rows or matrices gets as far as its buffers' sizes, one more does not."""
+    kern = gpu.pipeline(desc)
+    b = [hb.r(gpu.alloc(64)), hb.r(gpu.alloc(64))]
+    for call in (lambda m: gpu.launch(kern, b, m), lambda m: gpu.graph([hb.Op(kern, b, m)]), lambda m: gpu.time_ops([hb.Op(kern, b, m)])):
+        with pytest.raises(hb.HerbertError) as e:
+            call(most)
+        assert refusal not in str(e.value) and "binding" in str(e.value), e.value
+        with pytest.raises(hb.HerbertError, match=refusal):
+            call(most + 1)
+
+
+# Whole workgroups of 256 threads below 2^32 threads.
+THREADS = 2 ** 32 - 256
+
+
+@pytest.mark.parametrize("k", [16, 112, 128, 144, 2560, 17408, 1 << 20])
+def test_grid_of_rows(hb, gpu, k):
+    """Quantised rows take 16 threads a group of 128, read back one for 16 elements."""
+    assert gpu.groups(gpu.pipeline(hb.f8_quantize_rows(k)), 1 << 12) * 256 >= 16 * -(-k // 128) << 12
+    limit(hb, gpu, hb.f8_quantize_rows(k), THREADS // (16 * -(-k // 128)))
+    if k > 16:  # of 16: one thread a row, more rows than m holds
+        limit(hb, gpu, hb.f8_dequantize_rows(k), THREADS // (k // 16))
+
+
+def test_rows_past_the_grid(hb, gpu):
+    """80 GiB of rows, 1.25 2^32 threads."""
+    kern = gpu.pipeline(hb.f8_quantize_rows(2560))
+    with pytest.raises(hb.HerbertError, match="too many"):
+        gpu.launch(kern, [hb.r(gpu.alloc(64)), hb.r(gpu.alloc(64))], 1 << 24)
+
+
+@pytest.mark.parametrize("k,n", [(16, 1), (144, 130), (5120, 34816)])
+def test_grid_of_matrices(hb, gpu, k, n):
+    """A workgroup a block of 128 x 128; read back, a thread for 16 elements."""
+    limit(hb, gpu, hb.f8_quantize(k, n), THREADS // (256 * -(-k // 128) * -(-n // 128)))
+    if k * n > 16:
+        limit(hb, gpu, hb.f8_dequantize(k, n), THREADS // (k // 16 * n))
+
+
+def test_grid_of_routes(hb, gpu):
+    """A wave a row, four of them a workgroup."""
+    limit(hb, gpu, hb.route_topk(64, 4), THREADS // 64)
+
+
+@pytest.mark.parametrize("k,n", [(64, 16), (2560, 18432)])
+def test_grid_of_q4_matrices(hb, gpu, k, n):
+    """A wave a tile, four of them a workgroup."""
+    kern = gpu.pipeline(hb.q4_dequantize(k, n))
+    per = gpu.groups(kern, 1 << 10) * 4 >> 10  # tiles a matrix
+    limit(hb, gpu, hb.q4_dequantize(k, n), THREADS // (64 * per))
+    with pytest.raises(hb.HerbertError, match="too many"):
+        gpu.launch(kern, [hb.r(gpu.alloc(64)), hb.r(gpu.alloc(64))], 0xFFFFFFFF)
