@@ -82,15 +82,15 @@ CHECKS = {
         "-DHB_TOPK=8 -DHB_E=256",
     ],
     "gemm_f8.hip": [
-        "-DHB_K=2560 -DHB_N=10240 -DHB_OUT=0 -DHB_ROWS=0 -DHB_TOPK=1 -DHB_E=1 -DHB_BM=128 -DHB_BN=128 -DHB_WM=2 -DHB_WN=2 "
+        "-DHB_K=2560 -DHB_N=10240 -DHB_OUT=0 -DHB_ROWS=0 -DHB_TOPK=1 -DHB_E=1 -DHB_TILES=0 -DHB_BM=128 -DHB_BN=128 -DHB_WM=2 -DHB_WN=2 "
         "-DHB_STAGES=3 -DHB_BAND=4 -DHB_KSPLIT=1",
-        "-DHB_K=5008 -DHB_N=7001 -DHB_OUT=2 -DHB_ROWS=0 -DHB_TOPK=1 -DHB_E=1 -DHB_BM=64 -DHB_BN=192 -DHB_WM=1 -DHB_WN=4 "
+        "-DHB_K=5008 -DHB_N=7001 -DHB_OUT=2 -DHB_ROWS=0 -DHB_TOPK=1 -DHB_E=1 -DHB_TILES=0 -DHB_BM=64 -DHB_BN=192 -DHB_WM=1 -DHB_WN=4 "
         "-DHB_STAGES=3 -DHB_BAND=4 -DHB_KSPLIT=1",
-        "-DHB_K=2048 -DHB_N=1024 -DHB_OUT=3 -DHB_ROWS=1 -DHB_TOPK=8 -DHB_E=256 -DHB_BM=64 -DHB_BN=256 -DHB_WM=1 -DHB_WN=4 "
+        "-DHB_K=2048 -DHB_N=1024 -DHB_OUT=3 -DHB_ROWS=1 -DHB_TOPK=8 -DHB_E=256 -DHB_TILES=768 -DHB_BM=64 -DHB_BN=256 -DHB_WM=1 -DHB_WN=4 "
         "-DHB_STAGES=2 -DHB_BAND=4 -DHB_KSPLIT=1",
-        "-DHB_K=512 -DHB_N=2048 -DHB_OUT=0 -DHB_ROWS=2 -DHB_TOPK=8 -DHB_E=256 -DHB_BM=128 -DHB_BN=128 -DHB_WM=2 -DHB_WN=2 "
+        "-DHB_K=512 -DHB_N=2048 -DHB_OUT=0 -DHB_ROWS=2 -DHB_TOPK=8 -DHB_E=256 -DHB_TILES=768 -DHB_BM=128 -DHB_BN=128 -DHB_WM=2 -DHB_WN=2 "
         "-DHB_STAGES=3 -DHB_BAND=4 -DHB_KSPLIT=1",
-        "-DHB_K=5008 -DHB_N=7001 -DHB_OUT=1 -DHB_ROWS=0 -DHB_TOPK=1 -DHB_E=1 -DHB_BM=128 -DHB_BN=128 -DHB_WM=2 -DHB_WN=2 "
+        "-DHB_K=5008 -DHB_N=7001 -DHB_OUT=1 -DHB_ROWS=0 -DHB_TOPK=1 -DHB_E=1 -DHB_TILES=0 -DHB_BM=128 -DHB_BN=128 -DHB_WM=2 -DHB_WN=2 "
         "-DHB_STAGES=2 -DHB_BAND=4 -DHB_KSPLIT=1 -DHB_SCHED=1 -DHB_WIDE=1",
     ],
     "block_norm.hip": [

@@ -766,7 +766,7 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             e->nbind = 6;
             e->defines = {D("HB_K", d.k),   D("HB_N", d.n),   D("HB_OUT", d.ksplit > 1 ? (uint32_t)HB_OUT_F32 : d.out),
                           D("HB_ROWS", d.rows_of), D("HB_TOPK", experts ? d.top_k : 1), D("HB_E", experts ? d.experts : 1),
-                          D("HB_WIDE", d.out == HB_OUT_F32), D("HB_BM", d.bm), D("HB_BN", d.bn), D("HB_WM", d.wm), D("HB_WN", d.wn),
+                          D("HB_TILES", experts ? d.tiles : 0), D("HB_WIDE", d.out == HB_OUT_F32), D("HB_BM", d.bm), D("HB_BN", d.bn), D("HB_WM", d.wm), D("HB_WN", d.wn),
                           D("HB_STAGES", d.dbuf + 1), D("HB_BAND", d.band), D("HB_KSPLIT", d.ksplit > 1 ? d.ksplit : 1),
                           D("HB_SCHED", d.sched)};
             return HB_OK;

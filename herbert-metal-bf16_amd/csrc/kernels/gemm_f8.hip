@@ -34,7 +34,7 @@
 // whose largest is met over the waves in LDS.
 //
 // Constants: HB_K, HB_N (W rows), HB_OUT (0 bf16, 1 f32, 2 residual, 3
-// SwiGLU), HB_ROWS, HB_TOPK, HB_E, HB_BM, HB_BN, HB_WM, HB_WN, HB_STAGES,
+// SwiGLU), HB_ROWS, HB_TOPK, HB_E, HB_TILES (what the table holds), HB_BM, HB_BN, HB_WM, HB_WN, HB_STAGES,
 // HB_BAND, HB_KSPLIT, HB_WIDE.  Bindings: state, W, X, Y, list, tiles; then the rows
 // the launch was sized for.
 #include "f8.h"
@@ -161,8 +161,12 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
         row0 = gm * BM;
         rows = m - row0 < BM ? m - row0 : BM;
     } else {
-        // The table's tiles alone, each XCD a contiguous range of them.
-        const u32 total = tiles[0] * NTILES, per = (total + 7) / 8, i = g >> 3;
+        // The table's tiles alone, no more than it has room for and the launch
+        // has workgroups, each XCD a contiguous range of them.
+        u32 held = tiles[0];
+        held = held < HB_TILES ? held : HB_TILES;
+        held = held < m_launch * TOPK ? held : m_launch * TOPK;
+        const u32 total = held * NTILES, per = (total + 7) / 8, i = g >> 3;
         if (i >= per) return;
         g = (g & 7u) * per + i;
         if (g >= total) return;
