@@ -184,7 +184,7 @@ static const GemmF8Form kGemmF8F32[] = {
 //   rows, 2560 to 10240: 128 x 128 58.9, 128 x 160 73.8.  Of Out::F32: 17 rows, 2560
 //   to 512: 32 x 32 in eight parts 5.7, in four 6.0; 509 rows, 5008 to 7001: 128 x 128
 //   50.6, 64 x 128 55; 2048 rows, 9216 to 2560: 128 x 128 in two parts 114, whole 130.
-static void gemm_f8_dense(hb_desc* d, uint32_t rows) {
+static void gemm_f8_dense(hb_desc* d, uint32_t rows, bool whole) {
     const bool swi = d->out == HB_OUT_SWIGLU;
     const uint32_t kt = cdiv(d->k, 128);
     uint64_t best = ~0ull;
@@ -193,7 +193,7 @@ static void gemm_f8_dense(hb_desc* d, uint32_t rows) {
     auto consider = [&](const GemmF8Form& f) {
         const uint64_t tiles = (uint64_t)cdiv(rows, f.bm) * cdiv(d->n, f.bn);
         for (uint32_t s = 1; s <= 8; s *= 2) {
-            if (s > 1 && (swi || s > kt || tiles * s > 1024)) break;
+            if (s > 1 && (swi || whole || s > kt || tiles * s > 1024)) break;
             const uint64_t per = cdiv(kt, s), all = tiles * s;
             uint64_t t = f.first + per * f.first_kt;
             const uint64_t more = f.more + per * f.more_kt;
@@ -216,12 +216,13 @@ static void gemm_f8_dense(hb_desc* d, uint32_t rows) {
 }
 
 // The 8-bit GEMM's form: a dense descriptor that names none by the rows it is
-// built for (rows_max, 0 = 2048); else what it leaves open.
-static void gemm_f8_defaults(hb_desc* d) {
+// built for (rows_max, 0 = 2048), `whole` without a split of K; else what it
+// leaves open.
+static void gemm_f8_defaults(hb_desc* d, bool whole) {
     const bool swi = d->out == HB_OUT_SWIGLU, dense = d->rows_of == HB_ROWS_DENSE;
     if (!d->band) d->band = 4;
     if (dense && d->k && d->n && !d->bm && !d->bn && !d->wm && !d->wn && !d->dbuf && !d->mfma && !d->ksplit && !d->sched)
-        return gemm_f8_dense(d, d->rows_max ? d->rows_max : 2048);
+        return gemm_f8_dense(d, d->rows_max ? d->rows_max : 2048, whole);
     if (!dense && d->bm >= 32 && d->bm <= 128 && !d->bn && !d->wm && !d->wn && !d->dbuf && !d->mfma && !d->sched) {
         // The experts' (256 of 2048 / 512, top 8), us at 512, 1024 and 4096 rows,
         // tiles of 32, 64 and 128: gate and up 93, 99, 152; down 41, 45, 108 (with
@@ -278,7 +279,7 @@ hb_desc with_defaults(const hb_desc& in) {
     } else if (d.kind == HB_KIND_MATVEC_F8) {
         mv_f8_defaults(&d);
     } else if (d.kind == HB_KIND_GEMM_F8) {
-        gemm_f8_defaults(&d);
+        gemm_f8_defaults(&d, in.ksplit == 1);
     } else if (d.kind == HB_KIND_ROUTE_TOPK) {
         if (!d.bm) d.bm = 1;
         if (!d.bn) d.bn = d.bm;

@@ -280,7 +280,8 @@ typedef struct hb_desc {
      * whole number of K tiles (sched 3: an even number), and N must be a
      * multiple of 4 (the second kernel's vector width).  Of a dense GEMM_F8,
      * unless HB_OUT_SWIGLU: parts of whole K tiles of 128, equal or one
-     * apart, and any N.  One launch handle:
+     * apart, and any N; 0 leaves the parts to the library where it names no
+     * tile either, 1 = no split.  One launch handle:
      * hb_launch / hb_time run both kernels.  The workspace grows on the
      * first launch over more rows than any before it on the context: that
      * launch synchronizes the stream and calls hipFree / hipMalloc (not

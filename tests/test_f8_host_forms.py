@@ -112,3 +112,21 @@ def test_grid_of_q4_matrices(hb, gpu, k, n):
     limit(hb, gpu, hb.q4_dequantize(k, n), THREADS // (64 * per))
     with pytest.raises(hb.HerbertError, match="too many"):
         gpu.launch(kern, [hb.r(gpu.alloc(64)), hb.r(gpu.alloc(64))], 0xFFFFFFFF)
+
+
+@pytest.mark.parametrize("out", ["Bf16", "F32", "Residual"])
+@pytest.mark.parametrize("rows", [17, 64, 256, 1024])
+def test_no_split(hb, gpu, out, rows):
+    """ksplit 1 on a shape whose defaults split K: whole, and no workspace."""
+    assert "_ks" in gpu.kernel_name(gpu.pipeline(hb.gemm_f8(9216, 2560, hb.Out[out], rows=rows)))
+    whole = gpu.pipeline(hb.gemm_f8(9216, 2560, hb.Out[out], rows=rows, ksplit=1))
+    assert "_ks" not in gpu.kernel_name(whole)
+    size = 4 if out == "F32" else 2
+    sizes = [16, hb.f8_bytes(9216, 2560), rows * hb.f8_row_bytes(9216), rows * 2560 * size]
+    other = hb.Gpu(0)
+    k = other.pipeline(hb.gemm_f8(9216, 2560, hb.Out[out], rows=rows, ksplit=1))
+    b = [other.alloc(s) for s in sizes]
+    held = hb.lib.fake_in_use()
+    other.launch(k, [hb.r(v) for v in b + b[:1] * 2], rows)
+    assert hb.lib.fake_in_use() == held
+    other.close()
