@@ -216,13 +216,13 @@ static void gemm_f8_dense(hb_desc* d, uint32_t rows, bool whole) {
 }
 
 // The 8-bit GEMM's form: a dense descriptor that names none by the rows it is
-// built for (rows_max, 0 = 2048), `whole` without a split of K; else what it
+// built for (rows_max, 0 = kGemmF8Rows), `whole` without a split of K; else what it
 // leaves open.
 static void gemm_f8_defaults(hb_desc* d, bool whole) {
     const bool swi = d->out == HB_OUT_SWIGLU, dense = d->rows_of == HB_ROWS_DENSE;
     if (!d->band) d->band = 4;
     if (dense && d->k && d->n && !d->bm && !d->bn && !d->wm && !d->wn && !d->dbuf && !d->mfma && !d->ksplit && !d->sched)
-        return gemm_f8_dense(d, d->rows_max ? d->rows_max : 2048, whole);
+        return gemm_f8_dense(d, d->rows_max ? d->rows_max : kGemmF8Rows, whole);
     if (!dense && d->bm >= 32 && d->bm <= 128 && !d->bn && !d->wm && !d->wn && !d->dbuf && !d->mfma && !d->sched) {
         // The experts' (256 of 2048 / 512, top 8), us at 512, 1024 and 4096 rows,
         // tiles of 32, 64 and 128: gate and up 93, 99, 152; down 41, 45, 108 (with

@@ -51,6 +51,8 @@ inline bool writes_swiglu(const hb_desc& d) {
     return d.kind == HB_KIND_GEMM_SWIGLU ||
            ((d.kind == HB_KIND_MATVEC_Q4 || d.kind == HB_KIND_MATVEC_F8 || d.kind == HB_KIND_GEMM_F8) && d.out == HB_OUT_SWIGLU);
 }
+// The rows that a dense 8-bit GEMM is built for where rows_max names none.
+constexpr uint32_t kGemmF8Rows = 2048;
 // A GEMM in parts of K, whose launches are two kernels.
 inline bool splits_k(const hb_desc& d) { return (d.kind == HB_KIND_GEMM || d.kind == HB_KIND_GEMM_F8) && d.ksplit > 1; }
 // Fills defaults of the descriptor's zero fields (tile sizes, ...).

@@ -564,6 +564,15 @@ int hb_kernel_build(hb_gpu* g, const hb_desc* desc, int32_t* kernel) {
     Emitted em;
     int rc = emit(d, &em);
     if (rc) return rc;
+    // The 8-bit GEMM's slabs for the rows it is built for, here and not in the
+    // middle of a step; where they cannot be had (a recorded graph holds the
+    // workspace, or no memory) a split that the defaults chose is left.
+    if (d.kind == HB_KIND_GEMM_F8 && splits_k(d) && (d.rows_max || !desc->ksplit) &&
+        ensure_ws(g, workspace_of(d, d.rows_max ? d.rows_max : kGemmF8Rows)) != HB_OK && !desc->ksplit) {
+        hb_desc whole = *desc;
+        whole.ksplit = 1;
+        return hb_kernel_build(g, &whole, kernel);
+    }
     auto it = g->by_name.find(em.name);
     if (it != g->by_name.end()) {
         *kernel = it->second;

@@ -434,9 +434,10 @@ def f8_dequantize_rows(kdim):
 
 def gemm_f8(kdim, n, out, rows=0, bm=0, bn=0, wm=0, wn=0, stages=0, band=0, sched=0, ksplit=0):
     """Y[m][n] = X.W^T of f8 rows X and an f8 matrix W (bindings state, W, X, Y, list, tiles, the
-    last two not read).  rows: those of a launch, which the defaults go by; any may be launched (a
-    split form's workspace grows with them).  ksplit: parts of K, 1 = none; 0, where no tile is
-    named either, as many as the defaults take.
+    last two not read).  rows: those of a launch, which the defaults go by and a split form's workspace
+    is sized for when it is built; any may be launched (the workspace grows with them).  ksplit: parts
+    of K, 1 = none; 0, where no tile is named either, as many as the defaults take, none where the
+    workspace cannot grow.
     out Residual adds with one rounding; Swiglu: W [gate (n / 2) | up (n / 2)], h as f8 rows."""
     return Desc(kind=Kind.GEMM_F8, k=kdim, n=n, out=out, rows_max=rows, bm=bm, bn=bn, wm=wm, wn=wn, dbuf=max(0, stages - 1),
                 band=band, sched=sched, ksplit=ksplit)

@@ -281,7 +281,9 @@ typedef struct hb_desc {
      * multiple of 4 (the second kernel's vector width).  Of a dense GEMM_F8,
      * unless HB_OUT_SWIGLU: parts of whole K tiles of 128, equal or one
      * apart, and any N; 0 leaves the parts to the library where it names no
-     * tile either, 1 = no split.  One launch handle:
+     * tile either, 1 = no split; its workspace is grown when it is built, to
+     * rows_max rows (0 = 2048), and a split that the library chose is left
+     * where that fails.  One launch handle:
      * hb_launch / hb_time run both kernels.  The workspace grows on the
      * first launch over more rows than any before it on the context: that
      * launch synchronizes the stream and calls hipFree / hipMalloc (not

@@ -130,3 +130,87 @@ def test_no_split(hb, gpu, out, rows):
     other.launch(k, [hb.r(v) for v in b + b[:1] * 2], rows)
     assert hb.lib.fake_in_use() == held
     other.close()
+
+
+class Down:
+    """A context with a down product of up to 1024 rows, whose defaults split K, and its buffers."""
+    K, N, ROWS = 9216, 2560, (128, 256, 512, 1024)
+
+    def __init__(self, hb):
+        self.hb, self.g = hb, hb.Gpu(0)
+        sizes = [16, hb.f8_bytes(self.K, self.N), 1024 * hb.f8_row_bytes(self.K), 1024 * self.N * 2]
+        b = [hb.r(self.g.alloc(s)) for s in sizes]
+        self.bind = b + b[:1] * 2
+
+    def build(self, rows, **form):
+        return self.g.pipeline(self.hb.gemm_f8(self.K, self.N, self.hb.Out.Residual, rows=rows, **form))
+
+    def graph(self, kern, rows):
+        return self.g.graph([self.hb.Op(kern, self.bind, rows)])
+
+    def close(self):
+        self.hb.lib.fake_limit(2 ** 64 - 1)
+        self.g.close()
+
+
+@pytest.fixture()
+def down(hb):
+    d = Down(hb)
+    yield d
+    d.close()
+
+
+def test_workspace_when_built(hb, down):
+    """Kernels of every bucket, a graph of the shortest one's, the others' launches beside it: the
+    building made their room, no launch allocates."""
+    kern = {m: down.build(m) for m in down.ROWS}
+    assert all("_ks" in down.g.kernel_name(k) for k in kern.values())
+    tries = hb.lib.fake_malloc_tries()
+    graph = down.graph(kern[128], 128)
+    for m in down.ROWS:
+        down.g.launch(kern[m], down.bind, m)
+    graph.launch()
+    assert hb.lib.fake_malloc_tries() == tries
+    graph.free()
+
+
+def test_same_form_for_more_rows(hb, down):
+    """A kernel that is there already, built again for more rows, makes their room too."""
+    form = dict(bm=128, bn=128, ksplit=2)
+    kern = down.build(128, **form)
+    assert down.build(1024, **form) == kern
+    graph = down.graph(kern, 128)
+    down.g.launch(kern, down.bind, 1024)
+    graph.free()
+
+
+def test_built_beside_a_graph(hb, down):
+    """A recorded graph holds the workspace: the defaults' product for more rows is unsplit and runs,
+    a split that the caller named is refused at its launch, and after the graph both split."""
+    small = down.build(128)
+    graph = down.graph(small, 64)
+    whole = down.build(1024)
+    assert "_ks" not in down.g.kernel_name(whole)
+    down.g.launch(whole, down.bind, 1024)
+    named = down.build(1024, bm=128, bn=128, ksplit=8)
+    with pytest.raises(hb.HerbertError, match="recorded graph"):
+        down.g.launch(named, down.bind, 1024)
+    graph.free()
+    assert "_ks" in down.g.kernel_name(down.build(1024))
+    down.g.launch(named, down.bind, 1024)
+
+
+def test_built_without_memory(hb, down):
+    """No memory for the slabs: unsplit, and as much in use as before."""
+    held = hb.lib.fake_in_use()
+    hb.lib.fake_limit(held + (1 << 20))
+    kern = down.build(1024)
+    assert "_ks" not in down.g.kernel_name(kern) and hb.lib.fake_in_use() == held
+    down.g.launch(kern, down.bind, 1024)
+
+
+def test_no_rows_named(hb, down):
+    """Without rows the product is built for 2048, its workspace too."""
+    kern = down.g.pipeline(hb.gemm_f8(17408, 1024, hb.Out.Bf16))
+    assert "_ks" in down.g.kernel_name(kern)
+    assert hb.lib.fake_in_use() > 2 * 2048 * 1024 * 4
