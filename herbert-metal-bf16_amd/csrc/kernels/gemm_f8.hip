@@ -515,11 +515,12 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
                         u32x2{pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])};
         STAGE_BARRIER();
         constexpr u32 CPR = BN / 8;
+        typedef u32x4 loose_chunk __attribute__((aligned(2)));  // Y may start at any element
         for (u32 c = tid; c < BM * CPR; c += NTH) {
             const u32 r = c / CPR, n = n0 + c % CPR * 8;
             if (r >= rows || n >= NOUT) continue;
             const u32x4 v = *(const u32x4*)(t + r * EPIROW + c % CPR * 16);
-            __builtin_nontemporal_store(v, (u32x4*)((u16*)Yv + (u64)y_row(r) * NOUT + n));
+            __builtin_nontemporal_store(v, (loose_chunk*)((u16*)Yv + (u64)y_row(r) * NOUT + n));
         }
         return;
     }
