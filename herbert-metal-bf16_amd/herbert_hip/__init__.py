@@ -843,14 +843,10 @@ class MoeLayer:
 
     def __init__(self, gpu, engine, experts, top_k, hidden, inter, rows, w_gate_up, w_down,
                  scores=None, x=None, q4_group=0, f8=False, route=None, bias=None):
-        if route is None:
-            route = Desc(kind=Kind.ROUTE, experts=experts, top_k=top_k)
-        elif route.kind != Kind.ROUTE_TOPK or route.experts != experts or route.top_k != top_k:
-            raise HerbertError(HB_ERR_INVALID, "MoeLayer: a route_topk of %d experts, top %d" % (experts, top_k))
-        if bool(route.kind == Kind.ROUTE_TOPK and route.form & 2) != (bias is not None):
-            raise HerbertError(HB_ERR_INVALID, "MoeLayer: a bias where the route takes one")
-        if f8 and q4_group:
-            raise HerbertError(HB_ERR_INVALID, "MoeLayer: experts in 8 bits or in 4")
+        # The kernels first: a layer that is refused has allocated nothing.
+        route, self.route_k, self.bm, self.kernels = self._built(gpu, experts, top_k, hidden, inter, rows, q4_group, f8, route, bias)
+        self.swiglu_k = gpu.pipeline(Desc(kind=Kind.SWIGLU, n=inter))
+        self.combine_k = gpu.pipeline(Desc(kind=Kind.COMBINE, n=hidden, top_k=top_k))
         self.gpu, self.e, self.k, self.h, self.mi, self.rows = gpu, experts, top_k, hidden, inter, rows
         pairs = rows * top_k
         g = gpu
@@ -875,33 +871,45 @@ class MoeLayer:
         b = self.buf
         self.io = MoeIo(*[r(b[f]) for f in ("state", "route", "list", "tiles", "x", "w_gate_up",
                                              "egu", "ehb", "w_down", "ey", "xs")])
-        self.route_k = gpu.pipeline(route)
         self.route_io = [r(b["scores"]), r(b["route"])] + ([r(bias)] if bias is not None else [])
-        self.swiglu_k = gpu.pipeline(Desc(kind=Kind.SWIGLU, n=inter))
-        self.combine_k = gpu.pipeline(Desc(kind=Kind.COMBINE, n=hidden, top_k=top_k))
         if x is not None:
             g.upload(b["x"], x)
         if scores is not None:
             g.upload(b["scores"], scores)
             g.launch(self.route_k, self.route_io, rows)
             g.sync()
-        if f8:
-            self.bm = f8_tile_rows(rows, top_k, experts)
-            descs = [Desc(kind=Kind.SORT, experts=experts, top_k=top_k, bm=self.bm, rows_max=rows),
-                     experts_f8(hidden, 2 * inter, Out.Swiglu, Rows.Gather, top_k, experts, rows, self.bm),
-                     experts_f8(inter, hidden, Out.Bf16, Rows.Scatter, top_k, experts, rows, self.bm)]
-            quantize = gpu.pipeline(f8_quantize_rows(hidden)) if self.bm > 16 else -1
-            self.kernels, self.fused = [gpu.pipeline(d) for d in descs] + [quantize], True
-            return
-        if q4_group:
-            self.bm = 16
-            descs = [Desc(kind=Kind.SORT, experts=experts, top_k=top_k, bm=16, rows_max=rows),
-                     experts_q4(hidden, 2 * inter, Out.Swiglu, q4_group, Rows.Gather, top_k, experts, rows),
-                     experts_q4(inter, hidden, Out.Bf16, q4_group, Rows.Scatter, top_k, experts, rows)]
-            self.kernels, self.fused = [gpu.pipeline(d) for d in descs] + [-1], True
+        if self.kernels:
+            self.fused = True
             return
         self.kernels, self.bm = engine.experts(experts, top_k, hidden, inter, rows, self.io)
         self.fused = gpu.kernel_kind(self.kernels[1]) == Kind.GEMM_SWIGLU
+
+    @staticmethod
+    def _built(gpu, experts, top_k, hidden, inter, rows, q4_group, f8, route, bias):
+        """(route descriptor, its kernel, tile rows, the experts' kernels): of bf16 experts, which
+        the engine picks, no kernels and 0 tile rows."""
+        if route is None:
+            route = Desc(kind=Kind.ROUTE, experts=experts, top_k=top_k)
+        elif route.kind != Kind.ROUTE_TOPK or route.experts != experts or route.top_k != top_k:
+            raise HerbertError(HB_ERR_INVALID, "MoeLayer: a route_topk of %d experts, top %d" % (experts, top_k))
+        if bool(route.kind == Kind.ROUTE_TOPK and route.form & 2) != (bias is not None):
+            raise HerbertError(HB_ERR_INVALID, "MoeLayer: a bias where the route takes one")
+        if f8 and q4_group:
+            raise HerbertError(HB_ERR_INVALID, "MoeLayer: experts in 8 bits or in 4")
+        route_k, bm, kernels = gpu.pipeline(route), 0, []
+        if f8:
+            bm = f8_tile_rows(rows, top_k, experts)
+            descs = [Desc(kind=Kind.SORT, experts=experts, top_k=top_k, bm=bm, rows_max=rows),
+                     experts_f8(hidden, 2 * inter, Out.Swiglu, Rows.Gather, top_k, experts, rows, bm),
+                     experts_f8(inter, hidden, Out.Bf16, Rows.Scatter, top_k, experts, rows, bm)]
+            kernels = [gpu.pipeline(d) for d in descs] + [gpu.pipeline(f8_quantize_rows(hidden)) if bm > 16 else -1]
+        elif q4_group:
+            bm = 16
+            descs = [Desc(kind=Kind.SORT, experts=experts, top_k=top_k, bm=16, rows_max=rows),
+                     experts_q4(hidden, 2 * inter, Out.Swiglu, q4_group, Rows.Gather, top_k, experts, rows),
+                     experts_q4(inter, hidden, Out.Bf16, q4_group, Rows.Scatter, top_k, experts, rows)]
+            kernels = [gpu.pipeline(d) for d in descs] + [-1]
+        return route, route_k, bm, kernels
 
     def ops(self, m=None):
         """The layer's dispatches over m rows (m <= rows; state[3] must be m)."""
@@ -975,6 +983,8 @@ class MoeBlock:
     def __init__(self, gpu, engine, experts, top_k, hidden, inter, shared_inter, rows, w, x,
                  eps=1e-6, plus_one=True, q4_group=0, f8=False, route=None):
         g, h, si = gpu, hidden, shared_inter
+        bias = w["route_bias"] if route is not None and route.form & 2 else None
+        MoeLayer._built(gpu, experts, top_k, hidden, inter, rows, q4_group, f8, route, bias)  # or refused, before the rest
         self.gpu, self.rows, self.h, self.si, self.w = gpu, rows, h, si, w
         self.buf = {"state": g.alloc_with(np.array([0, 0, 0, rows], np.uint32)),
                     "x": g.alloc_with(x),
@@ -998,8 +1008,7 @@ class MoeBlock:
         g.free(xn_t)
         g.free(sc_t)
         self.layer = MoeLayer(g, engine, experts, top_k, h, inter, rows, w["w_gate_up"], w["w_down"],
-                              scores=scores, x=xn, q4_group=q4_group, f8=f8, route=route,
-                              bias=w["route_bias"] if route is not None and route.form & 2 else None)
+                              scores=scores, x=xn, q4_group=q4_group, f8=f8, route=route, bias=bias)
         L = self.layer.buf
         self.s_gu_k, self.s_sw_k = engine.gate_up(h, si, r(b["state"]), r(w["s_gate_up"]), r(L["x"]),
                                                   r(b["s_gu"]), r(b["s_h"]), rows)
@@ -1192,26 +1201,25 @@ class PrefillMlp:
         p = lambda f: "%d.%s" % (layer, f)  # noqa: E731
         mlp = "mlp.shared_expert" if ckpt.has(p("mlp.shared_expert.gate_proj.weight")) else "mlp"
         put = ckpt.upload_f8 if f8 else lambda gpu, parts, k, n: ckpt.upload(gpu, parts)
-        self.w = {"post_norm": ckpt.upload(gpu, [(p("post_attention_layernorm.weight"), hidden)]),
-                  "gate_up": put(gpu, [(p(mlp + ".gate_proj.weight"), inter * hidden),
-                                       (p(mlp + ".up_proj.weight"), inter * hidden)], hidden, 2 * inter),
-                  "down": put(gpu, [(p(mlp + ".down_proj.weight"), hidden * inter)], inter, hidden)}
         self.buckets = engine.buckets()
         self.chunk = self.buckets[-1]
         B = self.chunk
         g = gpu
-        if f8:
-            self.buf = {"xn": g.alloc(B * hidden * 2), "x8": g.alloc(B * f8_row_bytes(hidden)), "h8": g.alloc(B * f8_row_bytes(inter))}
-        else:
-            self.buf = {"xn": g.alloc(B * hidden * 2), "gu": g.alloc(B * 2 * inter * 2),
-                        "hh": g.alloc(B * inter * 2), "x": g.alloc(B * hidden * 2)}
         self.norm_k = g.pipeline(rmsnorm(hidden, eps, plus_one))
         self.kern = {}
-        if f8:
+        if f8:  # the kernels first: a shape that they refuse has allocated nothing
             q = g.pipeline(f8_quantize_rows(hidden))
             self.kern = {m: (g.pipeline(gemm_f8(hidden, 2 * inter, Out.Swiglu, rows=m)), q,
                              g.pipeline(gemm_f8(inter, hidden, Out.Residual, rows=m))) for m in self.buckets}
+        self.w = {"post_norm": ckpt.upload(gpu, [(p("post_attention_layernorm.weight"), hidden)]),
+                  "gate_up": put(gpu, [(p(mlp + ".gate_proj.weight"), inter * hidden),
+                                       (p(mlp + ".up_proj.weight"), inter * hidden)], hidden, 2 * inter),
+                  "down": put(gpu, [(p(mlp + ".down_proj.weight"), hidden * inter)], inter, hidden)}
+        if f8:
+            self.buf = {"xn": g.alloc(B * hidden * 2), "x8": g.alloc(B * f8_row_bytes(hidden)), "h8": g.alloc(B * f8_row_bytes(inter))}
             return
+        self.buf = {"xn": g.alloc(B * hidden * 2), "gu": g.alloc(B * 2 * inter * 2),
+                    "hh": g.alloc(B * inter * 2), "x": g.alloc(B * hidden * 2)}
         for m in self.buckets:
             st = g.alloc_with(np.array([0, 0, 0, m], np.uint32))
             b, w = self.buf, self.w

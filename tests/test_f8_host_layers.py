@@ -1,0 +1,67 @@
+"""The layers over 8-bit experts and their routes on the CPU, over a HIP runtime
+on host memory: what a refused one leaves behind, what a layer allocates."""
+import numpy as np
+import pytest
+
+import host_gpu
+
+
+@pytest.fixture(scope="module")
+def hb(tmp_path_factory):
+    mp = pytest.MonkeyPatch()
+    mp.setenv("HB_CACHE_DIR", "")
+    yield host_gpu.load(tmp_path_factory.mktemp("host"))
+    mp.undo()
+
+
+@pytest.fixture()
+def gpu(hb):
+    g = hb.Gpu(0)
+    yield g
+    g.close()
+
+
+E, K = 16, 4
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("kw", [dict(hidden=264), dict(hidden=100), dict(inter=64), dict(route=lambda hb: hb.route_topk(E, K, groups=5)),
+                                dict(route=lambda hb: hb.route_topk(E, K + 1)), dict(route=lambda hb: hb.route_topk(E, K, bias=True)),
+                                dict(q4_group=32)])
+def test_refused_layer(hb, gpu, rows, kw):
+    """A MoeLayer, and a MoeBlock around it, that are refused hold no memory."""
+    kw = dict(kw)
+    h, mi = kw.pop("hidden", 256), kw.pop("inter", 128)
+    if "route" in kw:
+        kw["route"] = kw["route"](hb)
+    w = gpu.alloc(64)
+    held = hb.lib.fake_in_use()
+    with pytest.raises(hb.HerbertError):
+        hb.MoeLayer(gpu, None, E, K, h, mi, rows, w, w, f8=True, **kw)
+    assert hb.lib.fake_in_use() == held
+    names = {n: w for n in ("post_norm", "router", "w_gate_up", "w_down", "s_gate_up", "s_down", "shared_gate")}
+    names["route_bias"] = None
+    with pytest.raises(hb.HerbertError):
+        hb.MoeBlock(gpu, None, E, K, h, mi, 128, rows, names, np.zeros((rows, h), np.uint16), f8=True, **kw)
+    assert hb.lib.fake_in_use() == held
+
+
+class NoWeights:
+    """A checkpoint whose reading would be one too many."""
+
+    def has(self, key):
+        return False
+
+    def upload(self, *a):
+        raise AssertionError("uploaded")
+
+    upload_f8 = upload
+
+
+@pytest.mark.parametrize("hidden,inter", [(264, 128), (256, 64), (256, 200)])
+def test_refused_mlp(hb, gpu, hidden, inter):
+    with hb.Engine(gpu, "prefill.block=128") as e:
+        held = hb.lib.fake_in_use()
+        with pytest.raises(hb.HerbertError):
+            hb.PrefillMlp(gpu, e, NoWeights(), 0, hidden, inter, f8=True)
+        assert hb.lib.fake_in_use() == held
