@@ -851,6 +851,7 @@ class MoeLayer:
         pairs = rows * top_k
         g = gpu
         f32_scores = route.kind == Kind.ROUTE_TOPK and route.form & 8
+        f8_rows = f8 and self.bm > 16
         self.buf = {
             "state": g.alloc_with(np.array([0, 0, 0, rows], np.uint32)),
             "scores": g.alloc(rows * experts * (4 if f32_scores else 2)),
@@ -859,18 +860,23 @@ class MoeLayer:
             "tiles": g.alloc((1 + 3 * moe_tiles(rows, top_k, experts, 16)) * 4),
             "x": g.alloc(rows * hidden * 2),
             "w_gate_up": w_gate_up,
-            "egu": g.alloc(pairs * 2 * inter * 2),
-            "ehb": g.alloc(pairs * max(inter * 2, f8_row_bytes(inter) if f8 else 0)),
+            "ehb": g.alloc(pairs * (f8_row_bytes(inter) if f8_rows else inter * 2)),
             "w_down": w_down,
             "ey": g.alloc(pairs * hidden * 2),
-            "xs": g.alloc(max(pairs * hidden * 2, rows * f8_row_bytes(hidden) if f8 else 0)),
             "out": g.alloc(rows * hidden * 2),
         }
+        if not f8:
+            self.buf["egu"] = g.alloc(pairs * 2 * inter * 2)
+            self.buf["xs"] = g.alloc(pairs * hidden * 2)
+        elif f8_rows:
+            self.buf["xs"] = g.alloc(rows * f8_row_bytes(hidden))
         if bias is not None:
             self.buf["bias"] = bias
         b = self.buf
-        self.io = MoeIo(*[r(b[f]) for f in ("state", "route", "list", "tiles", "x", "w_gate_up",
-                                             "egu", "ehb", "w_down", "ey", "xs")])
+        # Experts in 8 bits write no gate and up rows, a decode batch's no xs: those
+        # ranges are not looked at.
+        self.io = MoeIo(*[r(b.get(f, b["state"])) for f in ("state", "route", "list", "tiles", "x", "w_gate_up",
+                                                            "egu", "ehb", "w_down", "ey", "xs")])
         self.route_io = [r(b["scores"]), r(b["route"])] + ([r(bias)] if bias is not None else [])
         if x is not None:
             g.upload(b["x"], x)

@@ -21,7 +21,7 @@ def gpu(hb):
     g.close()
 
 
-E, K = 16, 4
+E, K = 64, 4  # route_qwen takes experts by 64
 
 
 @pytest.mark.parametrize("rows", [1, 40])
@@ -65,3 +65,24 @@ def test_refused_mlp(hb, gpu, hidden, inter):
         with pytest.raises(hb.HerbertError):
             hb.PrefillMlp(gpu, e, NoWeights(), 0, hidden, inter, f8=True)
         assert hb.lib.fake_in_use() == held
+
+
+@pytest.mark.parametrize("rows,bm", [(1, 16), (40, 32), (1000, 128)])
+def test_layer_memory(hb, gpu, rows, bm):
+    """An 8-bit layer's buffers are those its launches bind: no gate and up rows, x's quantised rows
+    only where a kernel writes them."""
+    h, mi, pairs = 256, 128, rows * K
+    w = gpu.alloc(E * hb.f8_bytes(h, 2 * mi)), gpu.alloc(E * hb.f8_bytes(mi, h))
+    held = hb.lib.fake_in_use()
+    layer = hb.MoeLayer(gpu, None, E, K, h, mi, rows, *w, f8=True)
+    assert layer.bm == bm
+    want = {"state": 16, "scores": rows * E * 2, "route": rows * 8 * K, "list": pairs * 4, "tiles": (1 + 3 * hb.moe_tiles(rows, K, E, 16)) * 4,
+            "x": rows * h * 2, "ehb": pairs * (2 * mi if bm == 16 else hb.f8_row_bytes(mi)), "ey": pairs * h * 2, "out": rows * h * 2}
+    if bm > 16:
+        want["xs"] = rows * hb.f8_row_bytes(h)
+    assert {n: gpu.size(b) for n, b in layer.buf.items() if n not in ("w_gate_up", "w_down")} == want
+    assert hb.lib.fake_in_use() - held == sum(-(-v // 256) * 256 for v in want.values())  # each a multiple of 256
+    names = [gpu.kernel_name(op.kernel) for op in layer.ops()]
+    assert len(names) == (6 if bm > 16 else 5) and not any("swiglu" in n for n in names)
+    layer.free()
+    assert hb.lib.fake_in_use() == held
