@@ -468,6 +468,8 @@ def route_topk(experts, top_k, score=Score.Softmax, bias=False, groups=1, top_gr
     plus a bias in the choice if any, among the top_groups groups of the largest best (group_top 1)
     or two best summed (2); weights renormalised over the chosen if renorm, times scale (bindings
     scores, route[, bias])."""
+    if score not in list(Score):
+        raise HerbertError(HB_ERR_INVALID, "route_topk: softmax or sigmoid scores")
     if group_top not in (1, 2):
         raise HerbertError(HB_ERR_INVALID, "route_topk: a group's best one or two experts")
     bits = struct.unpack("<I", struct.pack("<f", scale))[0]

@@ -214,3 +214,11 @@ def test_no_rows_named(hb, down):
     kern = down.g.pipeline(hb.gemm_f8(17408, 1024, hb.Out.Bf16))
     assert "_ks" in down.g.kernel_name(kern)
     assert hb.lib.fake_in_use() > 2 * 2048 * 1024 * 4
+
+
+@pytest.mark.parametrize("score", [2, 4, -1, 3.5])
+def test_unknown_score_refused(hb, score):
+    """A score that is none would set another of the descriptor's parts, a bias's binding for one."""
+    with pytest.raises(hb.HerbertError, match="softmax or sigmoid"):
+        hb.route_topk(64, 4, score=score)
+    assert hb.route_topk(64, 4, score=hb.Score.Sigmoid).form & 1 and not hb.route_topk(64, 4, score=hb.Score.Softmax).form & 1
