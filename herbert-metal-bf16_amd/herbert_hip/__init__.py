@@ -849,10 +849,12 @@ class MoeLayer:
         route, self.route_k, self.bm, self.kernels = self._built(gpu, experts, top_k, hidden, inter, rows, q4_group, f8, route, bias)
         self.swiglu_k = gpu.pipeline(Desc(kind=Kind.SWIGLU, n=inter))
         self.combine_k = gpu.pipeline(Desc(kind=Kind.COMBINE, n=hidden, top_k=top_k))
+        f32_scores = route.kind == Kind.ROUTE_TOPK and route.form & 8
+        if scores is not None and np.asarray(scores).itemsize != (4 if f32_scores else 2):
+            raise HerbertError(HB_ERR_INVALID, "MoeLayer: scores in %s, as the route takes them" % ("f32" if f32_scores else "bf16"))
         self.gpu, self.e, self.k, self.h, self.mi, self.rows = gpu, experts, top_k, hidden, inter, rows
         pairs = rows * top_k
         g = gpu
-        f32_scores = route.kind == Kind.ROUTE_TOPK and route.form & 8
         f8_rows = f8 and self.bm > 16
         self.buf = {
             "state": g.alloc_with(np.array([0, 0, 0, rows], np.uint32)),

@@ -86,3 +86,14 @@ def test_layer_memory(hb, gpu, rows, bm):
     assert len(names) == (6 if bm > 16 else 5) and not any("swiglu" in n for n in names)
     layer.free()
     assert hb.lib.fake_in_use() == held
+
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_scores_of_another_type(hb, gpu, f32):
+    """bf16 scores where the route reads f32 would fill half of the buffer, f32 ones be read as bf16."""
+    w = gpu.alloc(64)
+    held = hb.lib.fake_in_use()
+    scores = np.zeros((4, E), np.uint16 if f32 else np.float32)
+    with pytest.raises(hb.HerbertError, match="scores in %s" % ("f32" if f32 else "bf16")):
+        hb.MoeLayer(gpu, None, E, K, 256, 128, 4, w, w, f8=True, scores=scores, route=hb.route_topk(E, K, f32=f32))
+    assert hb.lib.fake_in_use() == held
