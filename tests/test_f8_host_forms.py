@@ -1,6 +1,10 @@
 """The 8-bit kernels' forms and launches on the CPU over a HIP runtime on host
 memory: forms that are refused, grids at their limit, what a split of K takes of
 the workspace, and which forms the defaults take."""
+import math
+import random
+import re
+
 import pytest
 
 import host_gpu
@@ -222,3 +226,39 @@ def test_unknown_score_refused(hb, score):
     with pytest.raises(hb.HerbertError, match="softmax or sigmoid"):
         hb.route_topk(64, 4, score=score)
     assert hb.route_topk(64, 4, score=hb.Score.Sigmoid).form & 1 and not hb.route_topk(64, 4, score=hb.Score.Softmax).form & 1
+
+
+def test_defaults_are_tested(hb, gpu):
+    """Every form that the defaults take, over the shapes from one row and 16 K to long prompts of the
+    largest matrices, is one that the GPU tests run; and they take all of those."""
+    import test_gpu_f8_forms as forms
+
+    def tag(f):
+        return "_t%dx%d_w%dx%d_d%d_b4%s" % (f["bn"], f["bm"], f["wn"], f["wm"], f["stages"] - 1, "_fa" if f["sched"] else "")
+
+    tested = {"sw": forms.SWIGLU, "f32": forms.F32, "bf16": forms.DENSE, "res": forms.DENSE}
+    tested = {out: {tag(f) for f in fs} for out, fs in tested.items()}
+    taken = {out: set() for out in tested}
+    rng = random.Random(5)
+
+    def size(lo, hi):
+        return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+    for _ in range(3000):
+        out = rng.choice(list(hb.Out))
+        n = 256 * size(1, 136) if out == hb.Out.Swiglu else size(16, 34816)
+        name = gpu.kernel_name(gpu.pipeline(hb.gemm_f8(16 * size(1, 1088), n, out, rows=size(1, 8192))))
+        kind, form, parts = re.search(r"gemm_f8_\d+x\d+_(sw|f32|bf16|res)(_t.*?)(_ks\d)?$", name).groups()
+        assert form in tested[kind] and parts in (None, "_ks2", "_ks4", "_ks8"), name
+        taken[kind].add(form)
+    assert taken == tested
+
+
+@pytest.mark.parametrize("hidden,inter", [(400, 256), (2048, 512), (5120, 1536)])
+def test_experts_defaults_are_tested(hb, gpu, hidden, inter):
+    """One form a tile size and product, whatever the sizes: those of the GPU tests."""
+    for bm, gate_up in [(32, True), (64, True), (128, True), (32, False), (64, False), (128, False)]:
+        k, n, out, rows = (hidden, 2 * inter, hb.Out.Swiglu, hb.Rows.Gather) if gate_up else (inter, hidden, hb.Out.Bf16, hb.Rows.Scatter)
+        tags = {re.search("_t.*?(?=_gather|_scatter)", gpu.kernel_name(gpu.pipeline(hb.experts_f8(a, b, out, rows, 2, 5, 100, bm)))).group()
+                for a, b in ((k, n), (400, 512))}
+        assert len(tags) == 1, tags
