@@ -6,7 +6,7 @@ import pytest
 
 import f8_ref as f8
 import herbert_hip as hb
-from test_gpu_f8 import Bufs, marked, run
+from test_gpu_f8 import Bufs, marked, quantized_rows, run, same_rows
 from test_gpu_f8_gemm import check_h
 
 pytestmark = pytest.mark.gpu
@@ -176,3 +176,34 @@ def test_default_experts(gpu, bm, gate_up):
             swiglu_close(got[p:p + 1], 1, n // 2, want)
         else:
             np.testing.assert_array_equal(got[order[p]], hb.f32_to_bf16(want.astype(np.float32))[0])
+
+
+def quotient_rows():
+    """bf16 rows of groups of 128, each its largest, t, beside 127 others, so that every x below or
+    equal to it stands beside it at every distance of their exponents: at each, t twice, the first
+    group without the last x, the second without the first, the one the largest's place."""
+    rows = []
+    for d in range(24):
+        x = (0x3F80 - (d << 7) + np.arange(128)).astype(np.uint16)  # 2^-d .. 2^(1-d)
+        for t in (0x3F80 + np.arange(128)).astype(np.uint16):
+            for at in (127, 0):
+                g = np.where(x > t, np.uint16(0), x)
+                g[at] = t
+                rows.append(g)
+    return np.array(rows, np.uint16)
+
+
+def test_every_quotient_beside_its_largest(gpu):
+    groups = quotient_rows()
+    top = groups.max(1)
+    seen = np.zeros((24, 128, 128), bool)  # distance, mantissa of the largest, of the other
+    for d in range(24):
+        part = groups[256 * d:256 * (d + 1)]
+        in_range = part >> 7 == 127 - d
+        seen[d, np.repeat(top[256 * d:256 * (d + 1)] & 127, 128)[in_range.ravel()], (part & 127)[in_range]] = True
+    assert (top >> 7 == 127).all() and seen[1:].all()
+    below = np.arange(128)[:, None] >= np.arange(128)[None, :]
+    assert (seen[0] == below).all()
+    x = groups.reshape(-1, 128 * 16)
+    x[1::2] ^= 0x8000
+    same_rows(*quantized_rows(gpu, x), x)
