@@ -96,6 +96,8 @@ static uint64_t f8_matrix_bytes(uint64_t k, uint64_t n) {
 // k and n within what keeps every byte count of a launch in 64 bits.
 static bool f8_shape(uint32_t k, uint32_t n) { return k && n && k % 16 == 0 && k <= (1u << 20) && n <= (1u << 24); }
 static bool f8_rows_form(const hb_desc& d) { return d.form == HB_F8_ROWS; }
+// A GEMM_F8 whose sums are f32's.
+static bool f8_wide_sums(const hb_desc& d) { return d.out == HB_OUT_F32 || d.form == HB_F8_SUMS_F32; }
 
 // What a MATVEC_F8 workgroup holds in LDS: each wave its stages, its x codes.
 static uint64_t mv_f8_lds(const hb_desc& d) {
@@ -167,7 +169,8 @@ static const GemmF8Form kGemmF8Swiglu[] = {
     {256, 256, 4, 2, 2, 0, 1080, 154, 434, 196, false}, {128, 256, 4, 4, 3, 0, 577, 96, 590, 103, false},
     {64, 256, 2, 4, 3, 0, 324, 80, 478, 68, false},     {32, 256, 1, 8, 4, 0, 315, 56, 331, 55, false},
 };
-// Out::F32's, whose products are bf16 (f8.h).
+// Those of f32 sums, whose products are bf16 (f8.h); the SwiGLU's are the same
+// as without.
 static const GemmF8Form kGemmF8F32[] = {
     {128, 128, 4, 2, 2, 1, 262, 110, 255, 87, false}, {64, 128, 2, 4, 2, 0, 264, 73, 85, 61, false},
     {32, 64, 1, 4, 3, 0, 203, 40, 30, 21, false},     {32, 32, 1, 2, 4, 0, 177, 39, 0, 15, true},
@@ -206,7 +209,7 @@ static void gemm_f8_dense(hb_desc* d, uint32_t rows, bool whole) {
     };
     if (swi)
         for (const auto& f : kGemmF8Swiglu) consider(f);
-    else if (d->out == HB_OUT_F32)
+    else if (f8_wide_sums(*d))
         for (const auto& f : kGemmF8F32) consider(f);
     else
         for (const auto& f : kGemmF8) consider(f);
@@ -731,6 +734,7 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             const bool experts = d.rows_of != HB_ROWS_DENSE, swi = d.out == HB_OUT_SWIGLU;
             if (d.out > HB_OUT_SWIGLU || d.rows_of > HB_ROWS_SCATTER)
                 return fail(HB_ERR_INVALID, "gemm_f8: out / rows_of out of range");
+            if (d.form > HB_F8_SUMS_F32) return fail(HB_ERR_INVALID, "gemm_f8: sums of the f8 MFMA or in f32");
             if (!f8_shape(d.k, d.n) || d.k > 65536 || (uint64_t)d.k * d.n > 0x7fffffffull)
                 return fail(HB_ERR_UNSUPPORTED, "gemm_f8: K a multiple of 16 up to 2^16, K N below 2^31");
             if (swi && (d.n % 256 || d.rows_of == HB_ROWS_SCATTER))
@@ -760,14 +764,15 @@ static int emit_kind(const hb_desc& d, Emitted* e) {
             if (d.sched > 1 || (d.sched && (d.dbuf != 1 || d.bn / d.wn < 64)))
                 return fail(HB_ERR_UNSUPPORTED, "gemm_f8 (fragments ahead): two stages, four fragments of W a wave");
             snprintf(name, sizeof name, "gemm_f8_%ux%u_%s_t%ux%u_w%ux%u_d%u_b%u%s%s", d.k, d.n, swi ? "sw" : out_tag(d.out), d.bn,
-                     d.bm, d.wn, d.wm, d.dbuf, d.band, d.sched ? "_fa" : "", rows.c_str());
+                     d.bm, d.wn, d.wm, d.dbuf, d.band, d.sched ? "_fa" : "",
+                     ((d.form && d.out != HB_OUT_F32 ? "_wide" : "") + rows).c_str());
             e->name = name;
             e->source = "gemm_f8.hip";
             e->threads = 64 * d.wm * d.wn;
             e->nbind = 6;
             e->defines = {D("HB_K", d.k),   D("HB_N", d.n),   D("HB_OUT", d.ksplit > 1 ? (uint32_t)HB_OUT_F32 : d.out),
                           D("HB_ROWS", d.rows_of), D("HB_TOPK", experts ? d.top_k : 1), D("HB_E", experts ? d.experts : 1),
-                          D("HB_TILES", experts ? d.tiles : 0), D("HB_WIDE", d.out == HB_OUT_F32), D("HB_BM", d.bm), D("HB_BN", d.bn), D("HB_WM", d.wm), D("HB_WN", d.wn),
+                          D("HB_TILES", experts ? d.tiles : 0), D("HB_WIDE", f8_wide_sums(d)), D("HB_BM", d.bm), D("HB_BN", d.bn), D("HB_WM", d.wm), D("HB_WN", d.wn),
                           D("HB_STAGES", d.dbuf + 1), D("HB_BAND", d.band), D("HB_KSPLIT", d.ksplit > 1 ? d.ksplit : 1),
                           D("HB_SCHED", d.sched)};
             return HB_OK;

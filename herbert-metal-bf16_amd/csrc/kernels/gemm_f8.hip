@@ -13,7 +13,8 @@
 // one for all of the fragment, and their product adds the four sums to the
 // accumulators with an fma each, 16 cycles of VALU beside the MFMA's 32.  Its
 // sums come out some 2^-16 off, little beside the half step of 2^-8 of a bf16
-// output; an f32 output takes the bf16 products of f8.h in its place (HB_WIDE).
+// output; an f32 output, and any that the caller asks f32 sums for, takes the
+// bf16 products of f8.h in its place (HB_WIDE), at half the rate.
 //
 // X and W tiles of 128 K go straight into LDS (buffer_load_dwordx4 ... lds)
 // through HB_STAGES stages, 16-byte chunks XORed by row >> 1 so that the

@@ -432,15 +432,16 @@ def f8_dequantize_rows(kdim):
     return Desc(kind=Kind.F8_DEQUANTIZE, k=kdim, form=1)
 
 
-def gemm_f8(kdim, n, out, rows=0, bm=0, bn=0, wm=0, wn=0, stages=0, band=0, sched=0, ksplit=0):
+def gemm_f8(kdim, n, out, rows=0, bm=0, bn=0, wm=0, wn=0, stages=0, band=0, sched=0, ksplit=0, f32_sums=False):
     """Y[m][n] = X.W^T of f8 rows X and an f8 matrix W (bindings state, W, X, Y, list, tiles, the
     last two not read).  rows: those of a launch, which the defaults go by and a split form's workspace
     is sized for when it is built; any may be launched (the workspace grows with them).  ksplit: parts
     of K, 1 = none; 0, where no tile is named either, as many as the defaults take, none where the
     workspace cannot grow.
-    out Residual adds with one rounding; Swiglu: W [gate (n / 2) | up (n / 2)], h as f8 rows."""
+    out Residual adds with one rounding; Swiglu: W [gate (n / 2) | up (n / 2)], h as f8 rows.
+    f32_sums: sums in f32 throughout (HB_F8_SUMS_F32), as out F32's always are, at half the rate."""
     return Desc(kind=Kind.GEMM_F8, k=kdim, n=n, out=out, rows_max=rows, bm=bm, bn=bn, wm=wm, wn=wn, dbuf=max(0, stages - 1),
-                band=band, sched=sched, ksplit=ksplit)
+                band=band, sched=sched, ksplit=ksplit, form=1 if f32_sums else 0)
 
 
 def matvec_f8(kdim, n, out, mv_m=1, rows=0, split=0, waves=0, unroll=0):
@@ -450,16 +451,16 @@ def matvec_f8(kdim, n, out, mv_m=1, rows=0, split=0, waves=0, unroll=0):
     return Desc(kind=Kind.MATVEC_F8, k=kdim, n=n, out=out, mv_m=mv_m, rows=rows, split=split, mv_waves=waves, unroll=unroll)
 
 
-def experts_f8(kdim, n, out, rows_of, top_k, experts, rows_max, bm, **form):
+def experts_f8(kdim, n, out, rows_of, top_k, experts, rows_max, bm, f32_sums=False, **form):
     """The routed experts' product over 8-bit matrices for blocks of up to rows_max rows, over tiles
     of moe_sort with this bm (f8_tile_rows; bindings state, W of every expert, X, Y, list, tiles):
     bm 16 matvec_f8's form, which takes bf16 rows and with out Swiglu writes them; 32 to 256
-    gemm_f8's, f8 rows."""
+    gemm_f8's, f8 rows.  f32_sums as gemm_f8's; matvec_f8's sums are f32."""
     common = dict(k=kdim, n=n, out=out, rows_of=rows_of, top_k=top_k, experts=experts, rows_max=rows_max,
                   tiles=moe_tiles(rows_max, top_k, experts, bm))
     if bm == 16:
         return Desc(kind=Kind.MATVEC_F8, mv_m=16, **common, **form)
-    return Desc(kind=Kind.GEMM_F8, bm=bm, **common, **form)
+    return Desc(kind=Kind.GEMM_F8, bm=bm, form=1 if f32_sums else 0, **common, **form)
 
 
 def route_topk(experts, top_k, score=Score.Softmax, bias=False, groups=1, top_groups=None, group_top=1, renorm=True, scale=1.0,
@@ -838,15 +839,16 @@ class MoeLayer:
     f8: w_gate_up and w_down are f8 matrices of all experts (f8_quantize over
     [2 inter][hidden] and [hidden][inter]), read by experts_f8 in the form that
     f8_tile_rows gives for `rows`: a decode batch's over bf16 rows, a prompt's
-    with x and the SwiGLU's rows as f8 rows.  Nothing is timed.
+    with x and the SwiGLU's rows as f8 rows.  Nothing is timed.  f32_sums: a
+    prompt's products keep f32 sums as a decode batch's do (gemm_f8).
 
     route: a route_topk descriptor in route_qwen's place, with the buffer of its
     bias if it has one; scores are then f32 where it says so."""
 
     def __init__(self, gpu, engine, experts, top_k, hidden, inter, rows, w_gate_up, w_down,
-                 scores=None, x=None, q4_group=0, f8=False, route=None, bias=None):
+                 scores=None, x=None, q4_group=0, f8=False, route=None, bias=None, f32_sums=False):
         # The kernels first: a layer that is refused has allocated nothing.
-        route, self.route_k, self.bm, self.kernels = self._built(gpu, experts, top_k, hidden, inter, rows, q4_group, f8, route, bias)
+        route, self.route_k, self.bm, self.kernels = self._built(gpu, experts, top_k, hidden, inter, rows, q4_group, f8, route, bias, f32_sums)
         self.swiglu_k = gpu.pipeline(Desc(kind=Kind.SWIGLU, n=inter))
         self.combine_k = gpu.pipeline(Desc(kind=Kind.COMBINE, n=hidden, top_k=top_k))
         f32_scores = route.kind == Kind.ROUTE_TOPK and route.form & 8
@@ -895,7 +897,7 @@ class MoeLayer:
         self.fused = gpu.kernel_kind(self.kernels[1]) == Kind.GEMM_SWIGLU
 
     @staticmethod
-    def _built(gpu, experts, top_k, hidden, inter, rows, q4_group, f8, route, bias):
+    def _built(gpu, experts, top_k, hidden, inter, rows, q4_group, f8, route, bias, f32_sums):
         """(route descriptor, its kernel, tile rows, the experts' kernels): of bf16 experts, which
         the engine picks, no kernels and 0 tile rows."""
         if route is None:
@@ -910,8 +912,8 @@ class MoeLayer:
         if f8:
             bm = f8_tile_rows(rows, top_k, experts)
             descs = [Desc(kind=Kind.SORT, experts=experts, top_k=top_k, bm=bm, rows_max=rows),
-                     experts_f8(hidden, 2 * inter, Out.Swiglu, Rows.Gather, top_k, experts, rows, bm),
-                     experts_f8(inter, hidden, Out.Bf16, Rows.Scatter, top_k, experts, rows, bm)]
+                     experts_f8(hidden, 2 * inter, Out.Swiglu, Rows.Gather, top_k, experts, rows, bm, f32_sums),
+                     experts_f8(inter, hidden, Out.Bf16, Rows.Scatter, top_k, experts, rows, bm, f32_sums)]
             kernels = [gpu.pipeline(d) for d in descs] + [gpu.pipeline(f8_quantize_rows(hidden)) if bm > 16 else -1]
         elif q4_group:
             bm = 16
@@ -987,14 +989,14 @@ class MoeBlock:
     [E*2*inter][h], "w_down": [E*h][inter], "s_gate_up": [2*si][h], "s_down":
     [h][si], "shared_gate": [h]}.  `x` (host [rows][h]) is the residual
     stream the selection runs on; the block updates buf["x"] in place.
-    q4_group, f8: w_gate_up and w_down in 4 or 8 bits, route: another route,
-    its bias w["route_bias"], as MoeLayer takes them."""
+    q4_group, f8, f32_sums: w_gate_up and w_down in 4 or 8 bits, route: another
+    route, its bias w["route_bias"], as MoeLayer takes them."""
 
     def __init__(self, gpu, engine, experts, top_k, hidden, inter, shared_inter, rows, w, x,
-                 eps=1e-6, plus_one=True, q4_group=0, f8=False, route=None):
+                 eps=1e-6, plus_one=True, q4_group=0, f8=False, route=None, f32_sums=False):
         g, h, si = gpu, hidden, shared_inter
         bias = w["route_bias"] if route is not None and route.form & 2 else None
-        MoeLayer._built(gpu, experts, top_k, hidden, inter, rows, q4_group, f8, route, bias)  # or refused, before the rest
+        MoeLayer._built(gpu, experts, top_k, hidden, inter, rows, q4_group, f8, route, bias, f32_sums)  # or refused, before the rest
         self.gpu, self.rows, self.h, self.si, self.w = gpu, rows, h, si, w
         self.buf = {"state": g.alloc_with(np.array([0, 0, 0, rows], np.uint32)),
                     "x": g.alloc_with(x),
@@ -1018,7 +1020,8 @@ class MoeBlock:
         g.free(xn_t)
         g.free(sc_t)
         self.layer = MoeLayer(g, engine, experts, top_k, h, inter, rows, w["w_gate_up"], w["w_down"],
-                              scores=scores, x=xn, q4_group=q4_group, f8=f8, route=route, bias=bias)
+                              scores=scores, x=xn, q4_group=q4_group, f8=f8, route=route, bias=bias,
+                              f32_sums=f32_sums)
         L = self.layer.buf
         self.s_gu_k, self.s_sw_k = engine.gate_up(h, si, r(b["state"]), r(w["s_gate_up"]), r(L["x"]),
                                                   r(b["s_gu"]), r(b["s_h"]), rows)
@@ -1204,9 +1207,10 @@ class PrefillMlp:
     1051-1063, holding its rows).  Weights from the checkpoint in the fused
     layout the GEMMs read (qwen.rs:790-794).  f8: the weights quantised to f8
     matrices and the block run on them: norm, x's rows quantised, [gate | up]
-    with the SwiGLU's f8 rows, down; nothing timed."""
+    with the SwiGLU's f8 rows, down; nothing timed; f32_sums: with sums in f32
+    (gemm_f8)."""
 
-    def __init__(self, gpu, engine, ckpt, layer, hidden, inter, eps=1e-6, plus_one=True, f8=False):
+    def __init__(self, gpu, engine, ckpt, layer, hidden, inter, eps=1e-6, plus_one=True, f8=False, f32_sums=False):
         self.gpu, self.h, self.inter, self.f8 = gpu, hidden, inter, f8
         p = lambda f: "%d.%s" % (layer, f)  # noqa: E731
         mlp = "mlp.shared_expert" if ckpt.has(p("mlp.shared_expert.gate_proj.weight")) else "mlp"
@@ -1219,8 +1223,8 @@ class PrefillMlp:
         self.kern = {}
         if f8:  # the kernels first: a shape that they refuse has allocated nothing
             q = g.pipeline(f8_quantize_rows(hidden))
-            self.kern = {m: (g.pipeline(gemm_f8(hidden, 2 * inter, Out.Swiglu, rows=m)), q,
-                             g.pipeline(gemm_f8(inter, hidden, Out.Residual, rows=m))) for m in self.buckets}
+            self.kern = {m: (g.pipeline(gemm_f8(hidden, 2 * inter, Out.Swiglu, rows=m, f32_sums=f32_sums)), q,
+                             g.pipeline(gemm_f8(inter, hidden, Out.Residual, rows=m, f32_sums=f32_sums))) for m in self.buckets}
         self.w = {"post_norm": ckpt.upload(gpu, [(p("post_attention_layernorm.weight"), hidden)]),
                   "gate_up": put(gpu, [(p(mlp + ".gate_proj.weight"), inter * hidden),
                                        (p(mlp + ".up_proj.weight"), inter * hidden)], hidden, 2 * inter),

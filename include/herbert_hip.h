@@ -132,13 +132,15 @@ enum hb_kind {
     HB_KIND_F8_DEQUANTIZE = 21, /* the same back, code * scale rounded once to bf16 */
     HB_KIND_GEMM_F8 = 22,       /* Y[m][n] = X.W^T of f8 rows X and an f8 matrix W; dense, or the
                                  * experts' over moe_sort's tiles of bm rows (rows_of).  f32 sums
-                                 * for HB_OUT_F32; else those of the f8 MFMA within each 128 of K,
-                                 * some 2^-16 off on normal operands */
+                                 * for HB_OUT_F32 and with HB_F8_SUMS_F32 in `form`; else those of
+                                 * the f8 MFMA within each 128 of K, some 2^-16 off on normal
+                                 * operands, at twice the rate */
     HB_KIND_MATVEC_F8 = 23      /* the same for m <= mv_m <= 16 rows of bf16 x, quantised as they are
                                  * loaded; or the experts' over tiles of 16 rows (rows_of) */
 };
 
 enum hb_f8_form { HB_F8_MATRIX = 0, HB_F8_ROWS = 1 };
+enum hb_f8_sums { HB_F8_SUMS_MFMA = 0, HB_F8_SUMS_F32 = 1 }; /* of GEMM_F8; MATVEC_F8's are f32 */
 
 /* HB_KIND_ROUTE_TOPK: of the scores s [m][experts] (bf16, or f32), per row
  *   p = softmax(s) or sigmoid(s),  c = p, or p + bias

@@ -262,3 +262,16 @@ def test_experts_defaults_are_tested(hb, gpu, hidden, inter):
         tags = {re.search("_t.*?(?=_gather|_scatter)", gpu.kernel_name(gpu.pipeline(hb.experts_f8(a, b, out, rows, 2, 5, 100, bm)))).group()
                 for a, b in ((k, n), (400, 512))}
         assert len(tags) == 1, tags
+
+
+def test_sums(hb, gpu):
+    """f32 sums are a kernel of their own for outputs of two bytes and the SwiGLU, and none for f32's; other
+    values of the part are refused."""
+    for out in hb.Out:
+        names = {gpu.kernel_name(gpu.pipeline(hb.gemm_f8(2560, 512, out, rows=64, f32_sums=f))) for f in (False, True)}
+        assert len(names) == (1 if out == hb.Out.F32 else 2), names
+    for bm, n in ((16, 1), (64, 2)):
+        made = [hb.experts_f8(256, 512, hb.Out.Swiglu, hb.Rows.Gather, 2, 8, 64, bm, f32_sums=f) for f in (False, True)]
+        assert len({gpu.kernel_name(gpu.pipeline(d)) for d in made}) == n
+    with pytest.raises(hb.HerbertError, match="sums"):
+        gpu.pipeline(hb.gemm_f8(2560, 512, hb.Out.Bf16).replace(form=2))
