@@ -276,27 +276,34 @@ extern "C" __global__ __launch_bounds__(256) void HB_NAME(const void* __restrict
         const float e = has ? hb_expf(d) : 0.0f;
         return has && s != mx && e > 0.0f ? __builtin_fmaf(e, rest, e) : e;
     };
-    if constexpr (RENORM) {
-        // The chosen ones alone, over their own sum.
+    auto largest = [&]() __attribute__((always_inline)) -> float {  // of the chosen ones' scores
         const u32 top = wave_max(has ? ordered(s) : 0u);
-        mx = top ? unordered(top) : 0.0f;
-    }
-    float p;
+        return top ? unordered(top) : 0.0f;
+    };
+    float p, total = 0.0f;
     if constexpr (SIGMOID) {
+        p = has ? hb_sigmoid(s) : 0.0f;
+        if constexpr (RENORM) total = butterfly_sum(p);
         // 1 / (1 + e^-s) is subnormal below -87 and 0 from -88.73 on, where e^s,
-        // the same to f32, is not.
-        p = !has ? 0.0f : s < -87.0f ? hb_expf(s) : hb_sigmoid(s);
-        // Where all chosen lie below 0, e^s / (1 + e^s) over e^mx: no row's sum
-        // comes near 0, however low its scores.
-        if (RENORM && mx < 0.0f) p = has ? relative() / (1.0f + hb_expf(s)) : 0.0f;
+        // the same to f32, is not; and where all chosen lie far below 0 their
+        // weights come from e^s / (1 + e^s) over e^largest.  Both are rare, and a
+        // row without them pays for neither (8192 rows of 256: 1.2 us).
+        const bool far = has && s < -87.0f;
+        if (__builtin_expect(__ballot(far || (RENORM && total < 0.00390625f)) != 0, 0)) {
+            p = far ? hb_expf(s) : p;
+            if constexpr (RENORM) {
+                mx = largest();
+                if (mx < 0.0f) p = has ? relative() / (1.0f + hb_expf(s)) : 0.0f;
+                total = butterfly_sum(p);
+            }
+        }
     } else {
+        if constexpr (RENORM) mx = largest();  // the chosen ones alone, over their own sum
         p = relative();
-        if constexpr (!RENORM) p = sum > 0.0f ? p / sum : 0.0f;
+        if constexpr (RENORM) total = butterfly_sum(p);
+        else p = sum > 0.0f ? p / sum : 0.0f;
     }
-    if constexpr (RENORM) {
-        const float total = butterfly_sum(p);
-        p = total > 0.0f ? p / total : 0.0f;
-    }
+    if constexpr (RENORM) p = p / (total > 0.0f ? total : 1.0f);  // no branch: all p are 0 beside a sum of 0
     p *= __builtin_bit_cast(float, (u32)HB_SCALE);
     u32 rank = 0;
 #pragma unroll
