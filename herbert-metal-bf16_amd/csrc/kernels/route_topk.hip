@@ -287,7 +287,7 @@ extern "C" __global__ __launch_bounds__(256) void HB_NAME(const void* __restrict
         // 1 / (1 + e^-s) is subnormal below -87 and 0 from -88.73 on, where e^s,
         // the same to f32, is not; and where all chosen lie far below 0 their
         // weights come from e^s / (1 + e^s) over e^largest.  Both are rare, and a
-        // row without them pays for neither (8192 rows of 256: 1.2 us).
+        // row without them pays for neither (8192 rows of 256: 0.5 us of 13.6).
         const bool far = has && s < -87.0f;
         if (__builtin_expect(__ballot(far || (RENORM && total < 0.00390625f)) != 0, 0)) {
             p = far ? hb_expf(s) : p;
