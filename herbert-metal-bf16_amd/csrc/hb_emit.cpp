@@ -119,10 +119,10 @@ static void mv_f8_defaults(hb_desc* d) {
     const uint32_t nt = cdiv(d->n, 16), kt = cdiv(d->k, 128);
     const bool swi = d->out == HB_OUT_SWIGLU;
     if (d->rows_of != HB_ROWS_DENSE) {
-        // The experts: 64 rows a wave once the block's pairs make 1024 workgroups
-        // of 32 rows (1 token of 8 experts, 2048 to 1024: 4.2 with 32, 64 rows
-        // 5.1), and four parts of K, of a short one none (4 tokens 11.7, two
-        // parts 15.5; 16 tokens 38.2 and 39.9; 512 to 2048 at 8 tokens 11.6, two
+        // The experts, measured on one shape (256 of 2048 / 512, top 8): 64 rows a
+        // wave once the block's pairs make 1024 workgroups of 32 rows (1 token of 8
+        // experts, 2048 to 1024: 4.2 with 32, 64 rows 5.1), and four parts of K, of a
+        // short one none (4 tokens 11.7, two parts 15.5; 16 tokens 38.2 and 39.9; 512 to 2048 at 8 tokens 11.6, two
         // parts 12.3).
         const bool many = (uint64_t)d->rows_max * d->top_k * cdiv(nt, 2) >= 1024;
         if (!d->rows) d->rows = many ? 64 : 32;
@@ -169,8 +169,9 @@ static const GemmF8Form kGemmF8Swiglu[] = {
     {256, 256, 4, 2, 2, 0, 1080, 154, 434, 196, false}, {128, 256, 4, 4, 3, 0, 577, 96, 590, 103, false},
     {64, 256, 2, 4, 3, 0, 324, 80, 478, 68, false},     {32, 256, 1, 8, 4, 0, 315, 56, 331, 55, false},
 };
-// Those of f32 sums, whose products are bf16 (f8.h); the SwiGLU's are the same
-// as without.
+// Those of f32 sums, whose products are bf16 (f8.h): fitted to Out::F32's times.
+// The SwiGLU's forms are those without f32 sums (2048 x 18432 x 2560 in an MLP of
+// 2048 rows: the MLP 347 us, 203 without).
 static const GemmF8Form kGemmF8F32[] = {
     {128, 128, 4, 2, 2, 1, 262, 110, 255, 87, false}, {64, 128, 2, 4, 2, 0, 264, 73, 85, 61, false},
     {32, 64, 1, 4, 3, 0, 203, 40, 30, 21, false},     {32, 32, 1, 2, 4, 0, 177, 39, 0, 15, true},
@@ -227,8 +228,8 @@ static void gemm_f8_defaults(hb_desc* d, bool whole) {
     if (dense && d->k && d->n && !d->bm && !d->bn && !d->wm && !d->wn && !d->dbuf && !d->mfma && !d->ksplit && !d->sched)
         return gemm_f8_dense(d, d->rows_max ? d->rows_max : kGemmF8Rows, whole);
     if (!dense && d->bm >= 32 && d->bm <= 128 && !d->bn && !d->wm && !d->wn && !d->dbuf && !d->mfma && !d->sched) {
-        // The experts' (256 of 2048 / 512, top 8), us at 512, 1024 and 4096 rows,
-        // tiles of 32, 64 and 128: gate and up 93, 99, 152; down 41, 45, 108 (with
+        // The experts', of one shape (256 of 2048 / 512, top 8), us at 512, 1024 and
+        // 4096 rows, tiles of 32, 64 and 128: gate and up 93, 99, 152; down 41, 45, 108 (with
         // 256 W rows a tile 43, 50 and 118).
         d->bn = swi ? 256 : d->bm == 32 ? 64 : 128;
         d->wm = swi || d->bm == 32 ? 2 : 4;
@@ -1181,7 +1182,10 @@ extern "C" uint32_t hb_f8_tile_rows(uint32_t rows, uint32_t top_k, uint32_t expe
     // The layer's two products, us (256 experts of 2048 / 512, top 8; for tiles
     // past 16 rows with x's quantisation): 8 rows 34 with tiles of 16, 35 with
     // 32; 12 rows 50 and 45; 16 rows 58 and 53; 512 rows 136 with 32, 142 with 64; 1024 rows 149 and
-    // 147; 2048 rows 187 with 64, 180 with 128.
+    // 147; 2048 rows 187 with 64, 180 with 128.  By pairs an expert alone: of 64
+    // experts of 2560 / 1024, top 4, and 16 of 5120 / 2048, top 2, at ten counts
+    // of rows each, it takes the fastest or within 8% of it but twice (64 experts,
+    // 384 rows 120 with 32, 103 with 64; 16 experts, 8 rows 75 with 32, 60 with 64).
     const uint64_t pairs = (uint64_t)rows * top_k;
     return 4 * pairs <= experts ? 16 : pairs <= 24ull * experts ? 32 : pairs <= 48ull * experts ? 64 : 128;
 }

@@ -76,7 +76,7 @@ HB_DEV u32x2 f8_codes8(u32x4 v, float inv) {
 // The codes of an MFMA operand's lane (32 along K) as bf16, which holds each of
 // them, and the products of two such lanes.  v_mfma_f32_16x16x128_f8f6f4 adds
 // each lane's products in eights, aligned to the largest of an eight and cut
-// some 14 bits below it: sums of normal operands come out 1.5e-5 off (2-norm),
+// 13 bits below its power of two: sums of normal operands come out 1.5e-5 off (2-norm),
 // with an outlier a row 2.2e-5.  The bf16 MFMA's sums are f32's (1e-8), at half
 // the rate and a conversion for every two codes.
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -107,7 +107,9 @@ HB_DEV f32x4 f8_product(const F8Wide& a, const F8Wide& b) {
 }
 
 // g sigmoid(g) u by the hardware's exp2 and reciprocal: some (8 + 1.5 |g|) 2^-24
-// of it off, where swiglu_n keeps an expf's bits at four times the instructions.
+// of it off, far below the half step of 2^-8 of the bf16 h that it is rounded to,
+// where swiglu_n keeps an expf's bits at four times the instructions (an MLP's
+// gate and up of 2048 rows, 2560 to 18432: 130 us against 180).
 HB_DEV float f8_swiglu(float g, float u) {
     return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g)) * u;
 }

@@ -23,10 +23,13 @@
 // does not matter).  X's scales of eight K tiles at a time go the same way into
 // one of two places, 32 bytes a row; W's, all of a tile's blocks, are read once.
 //
-// 8192 x 34816 x 5120: 1183 us, 2.47 PFLOP/s (the library's product under one
-// scale for all 1059); the MFMAs are busy for 55 to 60% of it, the scales' fmas and
-// the barrier a K tile hold the rest.  509 x 7001 x 5008 in f32 by bf16 products:
-// 47 us with x quantised, one tile on each of 220 CUs.
+// 8192 x 34816 x 5120: 1260 us in the mean of 40 launches, 1180 to 1210 at the
+// least, 2.32 to 2.47 PFLOP/s (the library's product under one scale for all 1059);
+// the MFMAs are busy for 60% of it, the scales' fmas and the barrier a K tile hold
+// the rest; with f32 sums 2470.  509 x 7001 x 5008 in f32 by bf16 products: 47 us
+// with x quantised, one tile on each of 220 CUs, and each wave converts its own
+// fragments (96 for 32 products a K tile and wave): W's by the four waves that
+// share them, X's by two.
 //
 // Out::Swiglu: W holds [gate (N / 2) | up (N / 2)] rows; a tile covers 128
 // features, a wave's first fragments their gate rows and its others the up
