@@ -275,3 +275,36 @@ def test_sums(hb, gpu):
         assert len({gpu.kernel_name(gpu.pipeline(d)) for d in made}) == n
     with pytest.raises(hb.HerbertError, match="sums"):
         gpu.pipeline(hb.gemm_f8(2560, 512, hb.Out.Bf16).replace(form=2))
+
+
+def test_matvec_defaults_are_tested(hb, gpu):
+    """The same of the matvec's forms, dense and over experts; a form of more than 8 x rows is tested
+    there with 10 and 16."""
+    import test_gpu_f8_mv_forms as forms
+
+    taken = {False: set(), True: set()}
+    rng = random.Random(7)
+
+    def size(lo, hi):
+        return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+    for _ in range(6000):
+        k, m, experts = 16 * size(1, 1088), size(1, 16), rng.random() < 0.3
+        if experts:
+            gate_up = rng.random() < 0.5
+            d = hb.experts_f8(k, 256 * size(1, 40), hb.Out.Swiglu if gate_up else hb.Out.Bf16, hb.Rows.Gather if gate_up else hb.Rows.Scatter,
+                              rng.choice([1, 2, 4, 8]), rng.choice([8, 64, 256]), m, 16)
+        else:
+            out = rng.choice(list(hb.Out))
+            d = hb.matvec_f8(k, 256 * size(1, 136) if out == hb.Out.Swiglu else size(16, 151936), out, mv_m=m)
+        f = tuple(int(v) for v in re.search(r"_r(\d+)_k(\d+)_w(\d+)_u(\d+)_m", gpu.kernel_name(gpu.pipeline(d))).groups())
+        assert experts or (f in forms.FORMS and (f != forms.FORMS[1] or m <= 8)), (f, m)
+        taken[experts].add(f)
+    assert taken[False] == set(forms.FORMS)
+    # The experts' by their cases there: few pairs and many, long K and short.
+    made = set()
+    for t, k, n in [(40, 1040, 512), (2, 1040, 512), (2, 272, 256), (2, 144, 256), (2, 128, 256), (60, 272, 512)]:
+        for out, rows in ((hb.Out.Swiglu, hb.Rows.Gather), (hb.Out.Bf16, hb.Rows.Scatter)):
+            name = gpu.kernel_name(gpu.pipeline(hb.experts_f8(k, n, out, rows, 2, 3, t, 16)))
+            made.add(tuple(int(v) for v in re.search(r"_r(\d+)_k(\d+)_w(\d+)_u(\d+)_m", name).groups()))
+    assert taken[True] <= made, taken[True] - made
