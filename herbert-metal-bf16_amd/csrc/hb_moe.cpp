@@ -36,6 +36,10 @@ int moe_experts_run(hb_gpu* g, const int32_t kernels[4], int32_t swiglu, int32_t
             return fail(HB_ERR_INVALID, "moe experts in 8 bits: a sort of the products' tiles, gathered gate|up rows with the "
                                         "SwiGLU, scattered down rows, kernels[3] the quantise kernel of x's rows");
     }
+    // The 8-bit products' rows: gate and up's h is down's x, both of the sort's pairs.
+    if ((mv_f8 || f8) && (gd->n != 2 * dd->k || gd->k != dd->n || gd->top_k != sd->top_k || dd->top_k != sd->top_k ||
+                          gd->experts != sd->experts || dd->experts != sd->experts))
+        return fail(HB_ERR_INVALID, "moe experts in 8 bits: kernels of other sizes, experts or top_k than one another's");
     // Its rows would be half as long as the combine reads them.
     if (writes_swiglu(*dd)) return fail(HB_ERR_INVALID, "moe experts: a down kernel that writes a SwiGLU");
     const bool fused = writes_swiglu(*gd);

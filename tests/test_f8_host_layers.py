@@ -1,5 +1,7 @@
 """The layers over 8-bit experts and their routes on the CPU, over a HIP runtime
 on host memory: what a refused one leaves behind, what a layer allocates."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -97,3 +99,31 @@ def test_scores_of_another_type(hb, gpu, f32):
     with pytest.raises(hb.HerbertError, match="scores in %s" % ("f32" if f32 else "bf16")):
         hb.MoeLayer(gpu, None, E, K, 256, 128, 4, w, w, f8=True, scores=scores, route=hb.route_topk(E, K, f32=f32))
     assert hb.lib.fake_in_use() == held
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_kernels_of_another_layer(hb, gpu, rows):
+    """hb_moe_experts_run refuses 8-bit kernels whose sizes, experts or top_k differ: h would be read as
+    rows of another length, or experts' rows be left unwritten."""
+    h, mi = 256, 128
+    w = gpu.alloc(2 * E * hb.f8_bytes(h, 4 * mi)), gpu.alloc(2 * E * hb.f8_bytes(2 * mi, h))
+    layer = hb.MoeLayer(gpu, None, E, K, h, mi, rows, *w, f8=True)
+    sort, gu, dn, quantize = layer.kernels
+
+    def experts(kdim, n, gate_up, top_k=K, count=E):
+        out, of = (hb.Out.Swiglu, hb.Rows.Gather) if gate_up else (hb.Out.Bf16, hb.Rows.Scatter)
+        return gpu.pipeline(hb.experts_f8(kdim, n, out, of, top_k, count, rows, layer.bm))
+
+    def sorted_by(top_k, count):
+        return gpu.pipeline(hb.Desc(kind=hb.Kind.SORT, experts=count, top_k=top_k, bm=layer.bm, rows_max=rows))
+
+    for ks in ([sort, experts(h, 4 * mi, True), dn, quantize], [sort, gu, experts(2 * mi, h, False), quantize],
+               [sort, gu, experts(mi, 2 * h, False), quantize], [sort, experts(h, 2 * mi, True, K // 2), dn, quantize],
+               [sort, gu, experts(mi, h, False, K // 2), quantize], [sort, experts(h, 2 * mi, True, K, E // 2), dn, quantize],
+               [sort, gu, experts(mi, h, False, K, 2 * E), quantize], [sorted_by(K, 2 * E), gu, dn, quantize],
+               [sorted_by(K // 2, E), gu, dn, quantize]):
+        hb.lib.fake_forget()
+        rc = hb.lib.hb_moe_experts_run(gpu.h, (ctypes.c_int32 * 4)(*ks), layer.swiglu_k, layer.combine_k, ctypes.byref(layer.io),
+                                       hb.r(layer.buf["out"]), rows)
+        assert rc == hb.ERR_INVALID and "moe experts in 8 bits" in hb.last_error(), ks
+        assert hb.lib.fake_launches() == 0
