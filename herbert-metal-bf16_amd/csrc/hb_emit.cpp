@@ -122,8 +122,8 @@ static void mv_f8_defaults(hb_desc* d) {
         // The experts, measured on one shape (256 of 2048 / 512, top 8): 64 rows a
         // wave once the block's pairs make 1024 workgroups of 32 rows (1 token of 8
         // experts, 2048 to 1024: 4.2 with 32, 64 rows 5.1), and four parts of K, of a
-        // short one none (4 tokens 11.7, two parts 15.5; 16 tokens 38.2 and 39.9; 512 to 2048 at 8 tokens 11.6, two
-        // parts 12.3).
+        // short one none (4 tokens 11.7, two parts 15.5; 16 tokens 38.2 and 39.9;
+        // 512 to 2048 at 8 tokens 11.6, two parts 12.3).
         const bool many = (uint64_t)d->rows_max * d->top_k * cdiv(nt, 2) >= 1024;
         if (!d->rows) d->rows = many ? 64 : 32;
         if (!d->split) {

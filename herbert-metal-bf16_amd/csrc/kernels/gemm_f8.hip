@@ -38,9 +38,9 @@
 // whose largest is met over the waves in LDS.
 //
 // Constants: HB_K, HB_N (W rows), HB_OUT (0 bf16, 1 f32, 2 residual, 3
-// SwiGLU), HB_ROWS, HB_TOPK, HB_E, HB_TILES (what the table holds), HB_BM, HB_BN, HB_WM, HB_WN, HB_STAGES,
-// HB_BAND, HB_KSPLIT, HB_WIDE.  Bindings: state, W, X, Y, list, tiles; then the rows
-// the launch was sized for.
+// SwiGLU), HB_ROWS, HB_TOPK, HB_E, HB_TILES (what the table holds), HB_BM,
+// HB_BN, HB_WM, HB_WN, HB_STAGES, HB_BAND, HB_KSPLIT, HB_WIDE.  Bindings: state,
+// W, X, Y, list, tiles; then the rows the launch was sized for.
 #include "f8.h"
 
 constexpr u32 K = HB_K, N = HB_N;
@@ -205,8 +205,8 @@ extern "C" __global__ __launch_bounds__(NTH) void HB_NAME(const u32* __restrict_
     // This wave's loads of a stage, wave loads wave, wave + NWV, ..: LDS slot p
     // of the operand's stage holds (row p / 8, chunk p % 8 ^ row >> 1), so that a
     // lane's chunk is the same in each (LROWS is a multiple of 16), and its rows
-    // LROWS apart: one address a lane and constants.  Rows past the operand's end lie past its
-    // resource's range, an experts' tile's rows past its own are put there:
+    // LROWS apart: one address a lane and constants.  Rows past the operand's end
+    // lie past its resource's range, an experts' tile's rows past its own are put there:
     // zeros without a memory access.  (The scalar offset, which the range
     // check takes off the range, stays within a row.)
     constexpr u32 AWAY = 0x80000000u;
